@@ -106,6 +106,31 @@ class KvAppendArgs(ctypes.Structure):
     ]
 
 
+class Kv4Cache(ctypes.Structure):
+    _fields_ = [
+        ("pool_dev", c_vp), ("dev_pages", c_i64), ("pool_host", c_vp), ("host_pages", c_i64),
+        ("block_table", c_vp), ("table_stride", c_i64), ("max_pages", c_int),
+        ("batch", c_int), ("kv_heads", c_int), ("page_size", c_int), ("group", c_int),
+    ]
+
+
+class Kv4AppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("qkv", c_vp), ("ld", c_i64), ("positions", c_vp), ("seq_index", c_vp), ("inv_freq", c_vp),
+        ("rope_scale", ctypes.c_float), ("q_out", c_vp), ("tokens", c_int), ("q_heads", c_int),
+        ("rotary_dim", c_int), ("interleaved", c_int), ("dtype", c_int),
+    ]
+
+
+class AttnQ4Args(ctypes.Structure):
+    _fields_ = [
+        ("query", c_vp), ("q_stride_b", c_i64), ("q_stride_h", c_i64), ("seq_lens", c_vp),
+        ("out", c_vp), ("o_stride_b", c_i64), ("o_stride_h", c_i64), ("partial_o", c_vp), ("partial_ml", c_vp),
+        ("merge_counters", c_vp), ("num_q_heads", c_int), ("max_seq_len", c_int), ("split_size", c_int),
+        ("scaling", ctypes.c_float), ("dtype", c_int),
+    ]
+
+
 # name -> (restype, argtypes); the full list of entry points of include/dak_b200.h.
 _I64P = ctypes.POINTER(c_i64)
 SIGNATURES = {
@@ -137,6 +162,12 @@ SIGNATURES = {
     "dak_rope_qk": (c_int, [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_vp]),
     "dak_silu_mul": (c_int, [c_vp, c_i64, c_vp, c_int, c_int, c_int, c_vp]),
     "dak_attn_decode_noalloc": (c_int, [ctypes.POINTER(AttnDecodeArgs), c_vp]),
+    "dak_rotary": (c_int, [c_vp, c_i64, c_i64, c_vp, c_vp, ctypes.c_float, c_int, c_vp, c_i64, c_i64, c_int, c_int,
+                           c_int, c_int, c_int, c_vp]),
+    "dak_rope_kv_append_q4": (c_int, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4AppendArgs), c_vp]),
+    "dak_kv_read_q4": (c_int, [ctypes.POINTER(Kv4Cache), c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_vp]),
+    "dak_attn_decode_paged_q4": (c_int, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(AttnQ4Args), c_vp]),
+    "dak_copy_pages": (c_int, [c_vp, c_i64, c_vp, c_i64, c_i64, c_int, c_i64, c_i64, c_vp, c_vp, c_int, c_vp]),
     "dak_device_status": (c_int, [c_int, ctypes.POINTER(c_int)]),
     "dak_selftest_wait_timeout": (c_int, [ctypes.c_uint, c_vp]),
     "dak_probe_stream_read": (c_int, [c_vp, ctypes.c_size_t, c_int, c_int, c_int, c_vp, c_vp]),

@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <utility>
 
+#include "../../include/dak_b200.h"
 #include "dak_linear.cuh"
 
 namespace dak {
@@ -26,6 +27,13 @@ uint64_t current_context_id();
 int *device_status_word();
 // DAK_OK if `p` is memory of the current device or pinned host memory.
 int check_gpu_accessible(const void *p, const char *what);
+// DAK_OK if the rotary kernels serve this part of a head.
+int check_rotary_dim(int rotary_dim, int head_dim, int interleaved);
+// Checks a 4-bit cache's sizes (kv4_check), then its pointers, and fills the
+// kernels' view of it (kv4_view).
+struct Kv4Cache;
+int kv4_check(const dak_kv4_cache *a);
+int kv4_view(const dak_kv4_cache *a, Kv4Cache *out);
 
 // Programmatic dependent launch of the decode-step kernels (RMSNorm, rotary,
 // SiLU-gate, KV append, decode attention and its merge): on unless

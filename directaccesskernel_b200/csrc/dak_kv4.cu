@@ -1,0 +1,373 @@
+// dak_kv4.cu - writing and reading the 4-bit paged KV cache (dak_kv4.cuh).
+//
+// Append, for each token: q heads are rotated into q_out; k heads are rotated
+// and v heads taken as they are, and each head's 128 values become 4-bit codes,
+// group by group (32, 64 or 128 dims):
+//   zero  = fp16(min), scale = fp16((max - min) / 15)   (saturated at +-65504)
+//   code  = clamp(rint((x - zero) * (1 / scale)), 0, 15) (0 when scale is 0)
+// from the rounded zero and scale, in FP32 from the rotated FP32 values: k is
+// not rounded to 16 bits first.  Read-back: value = scale * code + zero, one
+// rounding to the 16-bit type.
+//
+// Both are bound by memory.  Eight lanes own a (token, head) row, 16 dims each
+// (two 16-byte loads, one 8-byte code store), so a group's minimum and maximum
+// are 1, 2 or 3 shuffles away; a warp takes the same head of four neighbouring
+// tokens, whose code rows are neighbours in the page.
+#include <cstring>
+
+#include "dak_host.h"
+#include "dak_kv4.cuh"
+#include "dak_rotary.cuh"
+
+namespace dak {
+
+int kv4_check(const dak_kv4_cache *a) {
+  if (!a) return fail(DAK_ERR_INVALID_ARG, "cache is null");
+  if (a->page_size != 16 && a->page_size != 32 && a->page_size != 64)
+    return fail(DAK_ERR_UNSUPPORTED, "page_size must be 16, 32 or 64");
+  if (a->group != 32 && a->group != 64 && a->group != 128)
+    return fail(DAK_ERR_UNSUPPORTED, "group must be 32, 64 or 128");
+  if (a->batch <= 0 || a->kv_heads <= 0 || a->max_pages <= 0)
+    return fail(DAK_ERR_INVALID_ARG, "batch, kv_heads and max_pages must be positive");
+  if (a->table_stride < a->max_pages) return fail(DAK_ERR_INVALID_ARG, "table_stride below max_pages");
+  if (!a->block_table) return fail(DAK_ERR_INVALID_ARG, "block_table is required");
+  if (a->dev_pages < 0 || a->host_pages < 0 || (a->dev_pages > 0) != (a->pool_dev != nullptr) ||
+      (a->host_pages > 0) != (a->pool_host != nullptr))
+    return fail(DAK_ERR_INVALID_ARG, "each tier needs a pool and a positive page count, or neither");
+  if (a->dev_pages == 0 && a->host_pages == 0) return fail(DAK_ERR_INVALID_ARG, "no KV pool given");
+  if ((reinterpret_cast<uintptr_t>(a->pool_dev) | reinterpret_cast<uintptr_t>(a->pool_host)) & 15u)
+    return fail(DAK_ERR_ALIGNMENT, "KV pools must be 16-byte aligned");
+  return DAK_OK;
+}
+
+int kv4_view(const dak_kv4_cache *a, Kv4Cache *out) {
+  const void *ptrs[3] = {a->pool_dev, a->pool_host, a->block_table};
+  for (const void *q : ptrs) {
+    if (!q) continue;
+    int st = check_gpu_accessible(q, "KV buffer");
+    if (st) return st;
+  }
+  Kv4Cache &c = *out;
+  std::memset(&c, 0, sizeof(c));
+  c.pool[0] = static_cast<uint8_t *>(a->pool_dev);
+  c.pool[1] = static_cast<uint8_t *>(a->pool_host);
+  c.pages[0] = a->dev_pages;
+  c.pages[1] = a->host_pages;
+  c.ng = kKv4Dim / a->group;
+  c.slab_bytes = 2 * kv4_half_bytes(a->page_size, c.ng);
+  c.page_bytes = (long long)c.slab_bytes * a->kv_heads;
+  c.table = a->block_table;
+  c.table_stride = a->table_stride;
+  c.max_pages = a->max_pages;
+  c.rows = a->batch;
+  c.kv_heads = a->kv_heads;
+  c.page_size = a->page_size;
+  c.status = device_status_word();
+  if (!c.status) return fail(DAK_ERR_CUDA, "no device status word");
+  return DAK_OK;
+}
+
+namespace {
+
+constexpr int kKv4Threads = 256;
+constexpr int kKv4Warps = kKv4Threads / 32;
+
+struct AppendParams {
+  Kv4Cache c;
+  const uint16_t *qkv;
+  long long ld;
+  const int32_t *positions, *seq_index;
+  const float *inv_freq;
+  float scale;
+  uint16_t *q_out;
+  int tokens, q_heads, rotary_dim, interleaved, units;
+  int q_groups, kv_groups;  // warps that share a token's q heads, and its k (and v) heads
+  int pdl;
+};
+
+// Codes of a lane's 16 values and, in the group's first lane, the (scale, zero)
+// pair, from the group's minimum and maximum over the lanes that share it.
+template <int NG>
+__device__ __forceinline__ void kv4_quantise(const float (&x)[16], int lane8, uint8_t *codes, uint8_t *pairs) {
+  float mn = x[0], mx = x[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) {
+    mn = fminf(mn, x[i]);  // a NaN gives way to any number
+    mx = fmaxf(mx, x[i]);
+  }
+#pragma unroll
+  for (int m = 1; m < 8 / NG; m <<= 1) {
+    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, m));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, m));
+  }
+  const __half z = __float2half_rn(fminf(fmaxf(mn, -65504.f), 65504.f));
+  const __half s = __float2half_rn(fminf(fmaxf(__fdiv_rn(mx - mn, 15.f), 0.f), 65504.f));
+  const float zf = __half2float(z), sf = __half2float(s);
+  const float inv = sf > 0.f ? __frcp_rn(sf) : 0.f;
+  uint32_t w[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float n = fminf(fmaxf(rintf((x[i] - zf) * inv), 0.f), 15.f);  // NaN: 0
+    w[i >> 3] |= (uint32_t)n << (4 * (i & 7));
+  }
+  if (codes) {
+    *reinterpret_cast<uint2 *>(codes + lane8 * 8) = make_uint2(w[0], w[1]);
+    if (lane8 % (8 / NG) == 0)
+      reinterpret_cast<uint32_t *>(pairs)[lane8 / (8 / NG)] =
+          (uint32_t)__half_as_ushort(s) | ((uint32_t)__half_as_ushort(z) << 16);
+  }
+}
+
+// A warp's roles for its four tokens: q head groups first, then k, then v.
+template <typename T, int NG>
+__global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const __grid_constant__ AppendParams p) {
+  pdl_enter(p.pdl);
+  const int roles = p.q_groups + 2 * p.kv_groups;
+  const long long w = (long long)blockIdx.x * kKv4Warps + warp_id();
+  const int role = (int)(w % roles);
+  const int lane8 = lane_id() & 7;
+  const long long t64 = (w / roles) * 4 + (lane_id() >> 3);
+  const bool live = t64 < p.tokens;
+  const int t = live ? (int)t64 : 0;  // idle lanes stay for the shuffles
+  const int pos = p.positions[t];
+  const uint16_t *row = p.qkv + t * p.ld;
+  if (role < p.q_groups) {
+    if (!live) return;  // no shuffles below
+    for (int u = lane8; u < p.units; u += 8) {
+      const RopeUnit unit = rope_unit(u, p.rotary_dim, p.interleaved);
+      float c[8], s[8];
+      rope_unit_angles(unit, pos, p.inv_freq, p.scale, c, s);
+      for (int h = role; h < p.q_heads; h += p.q_groups) {
+        const uint4 *src = reinterpret_cast<const uint4 *>(row + h * kKv4Dim);
+        uint4 *dst = reinterpret_cast<uint4 *>(p.q_out + ((long long)t * p.q_heads + h) * kKv4Dim);
+        const uint4 a = src[unit.v0];
+        const uint4 b = unit.v1 >= 0 ? src[unit.v1] : a;
+        rope_unit_apply<T>(unit, p.interleaved, a, b, c, s, dst);
+      }
+    }
+    return;
+  }
+  const int isv = role >= p.q_groups + p.kv_groups ? 1 : 0;
+  const int g = role - p.q_groups - isv * p.kv_groups;
+  const int P = p.c.page_size;
+  int tier = 0;
+  uint8_t *page = nullptr;
+  if (live) {
+    page = pos < 0 ? nullptr : kv4_page(p.c, p.seq_index ? p.seq_index[t] : t, pos / P, &tier);
+    if (!page && lane8 == 0) atomicCAS(p.c.status, 0, DAK_ERR_INVALID_ARG);
+  }
+  const int half = kv4_half_bytes(P, NG);
+  const long long in_slab = (long long)isv * half + (pos % P) * 64;
+  const long long pair_off = (long long)isv * half + P * 64 + (pos % P) * 4 * NG;
+  // Half layout: dims 16 lane8 .. +15 and, R/2 dims away, their partners; each
+  // lane keeps its own side of the pairs.
+  const int R = isv ? 0 : p.rotary_dim;
+  const int part = R / 16;  // vectors between partners
+  float c[16], s[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    c[i] = 1.f;
+    s[i] = 0.f;
+    const int d = lane8 * 16 + i;
+    if (d < R) {
+      if (p.interleaved) {
+        if (i % 2 == 0) rope_cos_sin(pos, p.inv_freq[d / 2], p.scale, c[i], s[i]);
+      } else {
+        rope_cos_sin(pos, p.inv_freq[d < R / 2 ? d : d - R / 2], p.scale, c[i], s[i]);
+        if (d < R / 2) s[i] = -s[i];
+      }
+    }
+  }
+  for (int h = g; h < p.c.kv_heads; h += p.kv_groups) {
+    const uint4 *src =
+        reinterpret_cast<const uint4 *>(row + (long long)(p.q_heads + isv * p.c.kv_heads + h) * kKv4Dim);
+    float x[16];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int v = lane8 * 2 + k;
+      float y[8];
+      unpack8<T>(src[v], y);
+      if (!p.interleaved && v < 2 * part) {
+        float z[8];
+        unpack8<T>(src[v < part ? v + part : v - part], z);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = fmaf(y[i], c[8 * k + i], z[i] * s[8 * k + i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[8 * k + i] = y[i];
+    }
+    if (p.interleaved) {
+#pragma unroll
+      for (int i = 0; i < 16; i += 2)
+        if (lane8 * 16 + i < R) rope_turn(x[i], x[i + 1], c[i], s[i]);
+    }
+    uint8_t *slab = page ? page + (long long)h * p.c.slab_bytes : nullptr;
+    kv4_quantise<NG>(x, lane8, slab ? slab + in_slab : nullptr, slab ? slab + pair_off : nullptr);
+  }
+  // Host pages are read back over the host link by the next kernels of the
+  // stream; make the writes visible system-wide before this grid completes.
+  if (tier == 1) __threadfence_system();
+}
+
+struct ReadParams {
+  Kv4Cache c;
+  const int32_t *positions, *seq_index;
+  uint16_t *out[2];  // k, v: [tokens, kv_heads, 128]
+  int tokens, groups, pdl;
+};
+
+template <typename T, int NG>
+__global__ void __launch_bounds__(kKv4Threads) kv4_read_kernel(const __grid_constant__ ReadParams p) {
+  pdl_enter(p.pdl);
+  const int roles = 2 * p.groups;
+  const long long w = (long long)blockIdx.x * kKv4Warps + warp_id();
+  const int role = (int)(w % roles);
+  const int isv = role >= p.groups ? 1 : 0;
+  const int lane8 = lane_id() & 7;
+  const long long t = (w / roles) * 4 + (lane_id() >> 3);
+  if (t >= p.tokens) return;
+  const int P = p.c.page_size;
+  const int pos = p.positions[t];
+  int tier = 0;
+  const uint8_t *page = pos < 0 ? nullptr : kv4_page(p.c, p.seq_index ? p.seq_index[t] : (int)t, pos / P, &tier);
+  if (!page && lane8 == 0) atomicCAS(p.c.status, 0, DAK_ERR_INVALID_ARG);
+  const int half = kv4_half_bytes(P, NG);
+  for (int h = role - isv * p.groups; h < p.c.kv_heads; h += p.groups) {
+    uint2 w2 = make_uint2(0u, 0u);
+    float s = 0.f, z = 0.f;
+    if (page) {
+      const uint8_t *slab = page + (long long)h * p.c.slab_bytes + isv * half;
+      w2 = *reinterpret_cast<const uint2 *>(slab + (pos % P) * 64 + lane8 * 8);
+      const uint32_t sz = *reinterpret_cast<const uint32_t *>(slab + P * 64 + ((pos % P) * NG + lane8 / (8 / NG)) * 4);
+      s = __half2float(__ushort_as_half((unsigned short)(sz & 0xffffu)));
+      z = __half2float(__ushort_as_half((unsigned short)(sz >> 16)));
+    }
+    uint4 *dst = reinterpret_cast<uint4 *>(p.out[isv] + (t * p.c.kv_heads + h) * kKv4Dim) + lane8 * 2;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t word = k ? w2.y : w2.x;
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = fmaf(s, (float)((word >> (4 * i)) & 15u), z);
+      dst[k] = pack8<T>(x);
+    }
+  }
+}
+
+template <typename T>
+cudaError_t launch_append(const AppendParams &p, unsigned grid, cudaStream_t s) {
+  switch (p.c.ng) {
+    case 1: return launch_ex(kv4_append_kernel<T, 1>, dim3(grid), dim3(kKv4Threads), 0, s, 1, p.pdl != 0, p);
+    case 2: return launch_ex(kv4_append_kernel<T, 2>, dim3(grid), dim3(kKv4Threads), 0, s, 1, p.pdl != 0, p);
+    default: return launch_ex(kv4_append_kernel<T, 4>, dim3(grid), dim3(kKv4Threads), 0, s, 1, p.pdl != 0, p);
+  }
+}
+
+template <typename T>
+cudaError_t launch_read(const ReadParams &p, unsigned grid, cudaStream_t s) {
+  switch (p.c.ng) {
+    case 1: return launch_ex(kv4_read_kernel<T, 1>, dim3(grid), dim3(kKv4Threads), 0, s, 1, p.pdl != 0, p);
+    case 2: return launch_ex(kv4_read_kernel<T, 2>, dim3(grid), dim3(kKv4Threads), 0, s, 1, p.pdl != 0, p);
+    default: return launch_ex(kv4_read_kernel<T, 4>, dim3(grid), dim3(kKv4Threads), 0, s, 1, p.pdl != 0, p);
+  }
+}
+
+// Warps for the heads of `quads` token quads: one head per warp until the GPU
+// is full, then more heads per warp.
+int head_groups(long long quads, int heads) {
+  return (int)std::min<long long>(heads, std::max<long long>(1, 9472 / std::max(1ll, quads)));
+}
+
+int check_tokens(int tokens, const int32_t *positions, const int32_t *seq_index, int batch) {
+  if (tokens < 0) return fail(DAK_ERR_INVALID_ARG, "tokens must not be negative");
+  if (!positions) return fail(DAK_ERR_INVALID_ARG, "positions is required");
+  if (!seq_index && tokens != batch)
+    return fail(DAK_ERR_INVALID_ARG, "without seq_index there is one token per sequence (%d tokens, %d sequences)", tokens,
+                batch);
+  return DAK_OK;
+}
+
+}  // namespace
+}  // namespace dak
+
+extern "C" int dak_rope_kv_append_q4(const dak_kv4_cache *cache, const dak_kv4_append_args *a, void *stream) {
+  using namespace dak;
+  if (!a) return fail(DAK_ERR_INVALID_ARG, "args is null");
+  int st = kv4_check(cache);
+  if (st) return st;
+  if (a->dtype != DAK_DTYPE_F16 && a->dtype != DAK_DTYPE_BF16)
+    return fail(DAK_ERR_UNSUPPORTED, "the 4-bit append takes float16 and bfloat16");
+  if ((st = check_tokens(a->tokens, a->positions, a->seq_index, cache->batch))) return st;
+  if (a->q_heads < 0 || !a->qkv || (a->q_heads > 0 && !a->q_out))
+    return fail(DAK_ERR_INVALID_ARG, "qkv and, with q heads, q_out are required");
+  if (a->ld < ((int64_t)a->q_heads + 2ll * cache->kv_heads) * kKv4Dim)
+    return fail(DAK_ERR_INVALID_ARG, "qkv row stride below (q_heads + 2 kv_heads) x 128");
+  if (a->ld % 8 || ((reinterpret_cast<uintptr_t>(a->qkv) | reinterpret_cast<uintptr_t>(a->q_out)) & 15u))
+    return fail(DAK_ERR_ALIGNMENT, "qkv and q_out must be 16-byte aligned, the row stride a multiple of 8 elements");
+  if ((st = check_rotary_dim(a->rotary_dim, kKv4Dim, a->interleaved))) return st;
+  if (a->rotary_dim > 0 && !a->inv_freq) return fail(DAK_ERR_INVALID_ARG, "inv_freq is required to rotate");
+  const void *ptrs[5] = {a->qkv, a->q_heads > 0 ? a->q_out : nullptr, a->rotary_dim > 0 ? a->inv_freq : nullptr,
+                         a->positions, a->seq_index};
+  for (const void *q : ptrs)
+    if (q && (st = check_gpu_accessible(q, "append buffer"))) return st;
+  AppendParams p;
+  std::memset(&p, 0, sizeof(p));
+  if ((st = kv4_view(cache, &p.c))) return st;
+  if (a->tokens == 0) return DAK_OK;
+  p.qkv = static_cast<const uint16_t *>(a->qkv);
+  p.ld = a->ld;
+  p.positions = a->positions;
+  p.seq_index = a->seq_index;
+  p.inv_freq = a->inv_freq;
+  p.scale = a->rope_scale;
+  p.q_out = static_cast<uint16_t *>(a->q_out);
+  p.tokens = a->tokens;
+  p.q_heads = a->q_heads;
+  p.rotary_dim = a->rotary_dim;
+  p.interleaved = a->interleaved != 0;
+  p.units = rope_units(kKv4Dim, a->rotary_dim, p.interleaved);
+  const long long quads = (a->tokens + 3ll) / 4;
+  p.q_groups = a->q_heads > 0 ? head_groups(quads, a->q_heads) : 0;
+  p.kv_groups = head_groups(quads, cache->kv_heads);
+  p.pdl = decode_pdl_enabled() ? 1 : 0;
+  const long long grid = (quads * (p.q_groups + 2 * p.kv_groups) + kKv4Warps - 1) / kKv4Warps;
+  if (grid > 0x7fffffffll) return fail(DAK_ERR_UNSUPPORTED, "too many tokens for one launch");
+  auto s = static_cast<cudaStream_t>(stream);
+  return cuda_status(a->dtype == DAK_DTYPE_F16 ? launch_append<__half>(p, (unsigned)grid, s)
+                                               : launch_append<__nv_bfloat16>(p, (unsigned)grid, s),
+                     "4-bit append launch");
+}
+
+extern "C" int dak_kv_read_q4(const dak_kv4_cache *cache, const int32_t *positions, const int32_t *seq_index, void *k_out,
+                              void *v_out, int tokens, int dtype, void *stream) {
+  using namespace dak;
+  int st = kv4_check(cache);
+  if (st) return st;
+  if (dtype != DAK_DTYPE_F16 && dtype != DAK_DTYPE_BF16)
+    return fail(DAK_ERR_UNSUPPORTED, "the 4-bit cache is read to float16 and bfloat16");
+  if ((st = check_tokens(tokens, positions, seq_index, cache->batch))) return st;
+  if (!k_out || !v_out) return fail(DAK_ERR_INVALID_ARG, "k_out and v_out are required");
+  if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15u)
+    return fail(DAK_ERR_ALIGNMENT, "k_out and v_out must be 16-byte aligned");
+  const void *ptrs[4] = {k_out, v_out, positions, seq_index};
+  for (const void *q : ptrs)
+    if (q && (st = check_gpu_accessible(q, "read buffer"))) return st;
+  ReadParams p;
+  std::memset(&p, 0, sizeof(p));
+  if ((st = kv4_view(cache, &p.c))) return st;
+  if (tokens == 0) return DAK_OK;
+  p.positions = positions;
+  p.seq_index = seq_index;
+  p.out[0] = static_cast<uint16_t *>(k_out);
+  p.out[1] = static_cast<uint16_t *>(v_out);
+  p.tokens = tokens;
+  const long long quads = (tokens + 3ll) / 4;
+  p.groups = head_groups(quads, cache->kv_heads);
+  p.pdl = decode_pdl_enabled() ? 1 : 0;
+  const long long grid = (quads * 2 * p.groups + kKv4Warps - 1) / kKv4Warps;
+  if (grid > 0x7fffffffll) return fail(DAK_ERR_UNSUPPORTED, "too many tokens for one launch");
+  auto s = static_cast<cudaStream_t>(stream);
+  return cuda_status(dtype == DAK_DTYPE_F16 ? launch_read<__half>(p, (unsigned)grid, s)
+                                            : launch_read<__nv_bfloat16>(p, (unsigned)grid, s),
+                     "4-bit read launch");
+}

@@ -4,6 +4,8 @@ transformers' Llama arithmetic op by op (app/python/llama/vanila_llama.py:
 227-400 runs the same ops as separate torch kernels)."""
 from __future__ import annotations
 
+import math
+
 import torch
 
 from ._lib import LIB, check
@@ -70,3 +72,94 @@ def silu_mul(gate_up: torch.Tensor, out: torch.Tensor | None = None) -> torch.Te
     check(LIB.dak_silu_mul(gate_up.data_ptr(), gate_up.stride(0), out.data_ptr(), rows, cols,
                            dak_dtype(gate_up.dtype), _stream()), "silu_mul")
     return out
+
+
+def rope_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | None = None,
+                     max_position: int | None = None, device="cuda") -> tuple[torch.Tensor, float]:
+    """(inv_freq [rotary_dim / 2] float32, attention factor) of a rotary embedding.
+
+    ``scaling`` is a model configuration's rope dictionary: ``rope_type``
+    "default", "linear" (positions divided by ``factor``), "llama3" (long
+    wavelengths divided by ``factor``, with a smooth transition between
+    ``low_freq_factor`` and ``high_freq_factor``) or "yarn" (interpolation ramped
+    over the number of turns within the original context, and an attention
+    factor of 0.1 ln(factor) + 1 unless given).  ``max_position`` is the context
+    that "yarn" extends when the dictionary does not name
+    ``original_max_position_embeddings``."""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise RuntimeError("rotary_dim must be positive and even")
+    scaling = scaling or {}
+    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    inv = 1.0 / (theta ** (torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim))
+    attention = 1.0
+    if kind == "linear":
+        inv = inv / float(scaling["factor"])
+    elif kind == "llama3":
+        factor, low, high = (float(scaling[k]) for k in ("factor", "low_freq_factor", "high_freq_factor"))
+        turns = float(scaling["original_max_position_embeddings"]) * inv / (2 * math.pi)
+        smooth = ((turns - low) / (high - low)).clamp(0.0, 1.0)  # 0: divided by factor, 1: as it is
+        inv = (1 - smooth) * inv / factor + smooth * inv
+    elif kind == "yarn":
+        factor = float(scaling["factor"])
+        context = scaling.get("original_max_position_embeddings") or max_position
+        if context is None:
+            raise RuntimeError("yarn scaling needs original_max_position_embeddings or max_position")
+
+        def dim_of(turns: float) -> float:  # the (fractional) pair that makes this many turns in the context
+            return rotary_dim * math.log(context / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+        lo, hi = dim_of(float(scaling.get("beta_fast") or 32)), dim_of(float(scaling.get("beta_slow") or 1))
+        if scaling.get("truncate", True):
+            lo, hi = math.floor(lo), math.ceil(hi)
+        lo, hi = max(lo, 0), min(hi, rotary_dim - 1)
+        ramp = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - lo) / max(hi - lo, 0.001)).clamp(0.0, 1.0)
+        inv = inv / factor * ramp + inv * (1 - ramp)
+        attention = scaling.get("attention_factor")
+        if attention is None:
+            def mscale(m: float) -> float:
+                return 0.1 * m * math.log(factor) + 1.0 if factor > 1 else 1.0
+
+            m, m_all = scaling.get("mscale"), scaling.get("mscale_all_dim")
+            attention = mscale(m) / mscale(m_all) if m and m_all else mscale(1.0)
+    elif kind != "default":
+        raise RuntimeError(f"rope_type {kind!r} is not supported (default, linear, llama3 or yarn)")
+    return inv.to(torch.float32).to(device), float(attention)
+
+
+@traced
+def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, interleaved: bool = False,
+           rope_scale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions of x [tokens, heads, head_dim]: the first
+    2 * inv_freq.numel() dims rotated by positions [tokens] (int32) times
+    inv_freq, in pairs (i, i + R/2) or, ``interleaved``, (2i, 2i + 1), scaled by
+    ``rope_scale`` (the attention factor of ``rope_frequencies``); the other dims
+    copied.  FP32 arithmetic, one rounding, angles exact at any position.  Token
+    and head strides are free (multiples of 8), so x may be the q and k heads of
+    a fused projection; ``out`` may be x itself, else must not overlap it."""
+    _check16(x)
+    if x.dim() != 3:
+        raise RuntimeError("x must be [tokens, heads, head_dim]")
+    T, H, D = x.shape
+    _check_rope(positions, inv_freq, T, D)
+    if out is None:
+        out = torch.empty(T, H, D, dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or (D > 1 and out.stride(2) != 1):
+        raise RuntimeError("out must match x in shape, dtype and device, with a contiguous last dimension")
+    if T and H:
+        xt, xh, _ = x.stride()
+        ot, oh, _ = out.stride()
+        # A dimension of one entry has no stride to speak of.
+        check(LIB.dak_rotary(x.data_ptr(), xt if T > 1 else 0, xh if H > 1 else 0, positions.data_ptr(),
+                             inv_freq.data_ptr(), float(rope_scale), int(interleaved), out.data_ptr(),
+                             ot if T > 1 else 0, oh if H > 1 else 0, T, H, D, 2 * inv_freq.numel(),
+                             dak_dtype(x.dtype), _stream()), "rotary")
+    return out
+
+
+def _check_rope(positions: torch.Tensor, inv_freq: torch.Tensor | None, tokens: int, head_dim: int) -> None:
+    if positions.dtype != torch.int32 or not positions.is_cuda or positions.numel() != tokens \
+            or not positions.is_contiguous():
+        raise RuntimeError("positions must be a contiguous int32 CUDA tensor with one entry per token")
+    if inv_freq is not None and (inv_freq.dtype != torch.float32 or not inv_freq.is_cuda
+                                 or not inv_freq.is_contiguous() or 2 * inv_freq.numel() > head_dim):
+        raise RuntimeError("inv_freq must be a contiguous float32 CUDA tensor of at most head_dim / 2 entries")

@@ -405,6 +405,107 @@ DAK_API int dak_rope_qk(const void *qkv, int64_t ld, const int32_t *positions, c
  * row stride ld (>= 2 cols), out is [rows, cols] contiguous. */
 DAK_API int dak_silu_mul(const void *gate_up, int64_t ld, void *out, int rows, int cols, int dtype, void *stream);
 
+/* ------------------------------------------------------- rotary positions */
+/* out[t, h, :] = x[t, h, :] with its first rotary_dim dims rotated in pairs by
+ * the angle positions[t] * inv_freq[i] (rotary_dim / 2 FP32 frequencies) and
+ * scaled by rope_scale (the attention factor of a scaled rotary, else 1): pairs
+ * (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when interleaved is not 0.  Angles
+ * are exact to about 1e-7 rad at any position, the rotation is FP32 with one
+ * rounding; the other dims are copied.  Strides are in elements, multiples of 8;
+ * head_dim is a multiple of 8 up to 1024; rotary_dim is even, and a multiple of
+ * 16 in the half layout.  out may be x itself (same strides).  No reference
+ * counterpart as a kernel: the reference rotates in torch, whole heads in the
+ * half layout (app/python/llama/vanila_llama.py:212-246). */
+DAK_API int dak_rotary(const void *x, int64_t x_stride_t, int64_t x_stride_h, const int32_t *positions,
+                       const float *inv_freq, float rope_scale, int interleaved, void *out, int64_t o_stride_t,
+                       int64_t o_stride_h, int tokens, int heads, int head_dim, int rotary_dim, int dtype,
+                       void *stream);
+
+/* ------------------------------------------------- 4-bit tiered, paged KV */
+/* A pool is [pages, kv_heads, slab] bytes; the slab of one (page, head) of
+ * page_size (16, 32 or 64) tokens of head_dim 128 holds K codes [page_size][64]
+ * (dim 2i in the low half of byte i), K (scale, zero) float16 pairs
+ * [page_size][128 / group][2], V codes and V pairs: the value of code n is
+ * scale * n + zero.  group is 32, 64 or 128 dims.  block_table[b * table_stride
+ * + j] names page j of sequence b (0 <= b < batch) as in dak_attn_paged_args;
+ * entries outside their pool are recorded in the device error word
+ * (DAK_ERR_INVALID_ARG), skipped by the append and read as zeros.  No reference
+ * counterpart: the reference's cache is 16-bit. */
+typedef struct dak_kv4_cache {
+  void *pool_dev;             /* device pool (or NULL)                          */
+  int64_t dev_pages;
+  void *pool_host;            /* pinned host pool (or NULL)                     */
+  int64_t host_pages;
+  const int32_t *block_table; /* [batch, table_stride]                          */
+  int64_t table_stride;
+  int max_pages;              /* valid entries per table row                    */
+  int batch, kv_heads, page_size, group;
+} dak_kv4_cache;
+
+/* Rotary embedding, 4-bit quantisation and append of `tokens` tokens: a decode
+ * step's one per sequence (seq_index NULL, tokens == batch) or any tokens of
+ * any sequences (seq_index[t]).  qkv is [tokens, (q_heads + 2 kv_heads) * 128]
+ * with row stride ld; q heads go to q_out [tokens, q_heads, 128], rotated as by
+ * dak_rotary; k heads are rotated in FP32 and quantised, v heads quantised,
+ * into slot positions[t] of their sequence.  Per token, head and group:
+ *   zero = fp16(min), scale = fp16((max - min) / 15), both within +-65504,
+ *   code = clamp(round((x - zero) * (1 / scale)), 0, 15), 0 when scale is 0;
+ * a NaN is stored as code 0.  rotary_dim 0 rotates nothing.  The (sequence,
+ * position) pairs of one call must differ. */
+typedef struct dak_kv4_append_args {
+  const void *qkv;
+  int64_t ld;
+  const int32_t *positions;   /* [tokens]                                       */
+  const int32_t *seq_index;   /* [tokens] or NULL                               */
+  const float *inv_freq;      /* [rotary_dim / 2]                               */
+  float rope_scale;
+  void *q_out;                /* [tokens, q_heads, 128]; NULL with q_heads 0    */
+  int tokens, q_heads, rotary_dim, interleaved, dtype;
+} dak_kv4_append_args;
+DAK_API int dak_rope_kv_append_q4(const dak_kv4_cache *cache, const dak_kv4_append_args *args, void *stream);
+
+/* The cache's values at (seq_index[t] or t, positions[t]) in 16 bits: k_out and
+ * v_out are [tokens, kv_heads, 128]. */
+DAK_API int dak_kv_read_q4(const dak_kv4_cache *cache, const int32_t *positions, const int32_t *seq_index,
+                           void *k_out, void *v_out, int tokens, int dtype, void *stream);
+
+/* Decode attention over the 4-bit cache: one query token per sequence, any
+ * number of query heads per KV head.  Sequences longer than max_seq_len are cut
+ * to it; one of no tokens gives zeros.  partial_o holds batch * num_q_heads *
+ * splits * 128 floats and partial_ml twice batch * num_q_heads * splits, splits =
+ * ceil(max_seq_len / split_size); neither is used with one split.
+ * merge_counters (optional): batch * kv_heads * ceil(num_q_heads / kv_heads / 8)
+ * int32 in device memory, zero before the first call and left zero by every
+ * call; with them the last split merges, without them a second kernel does.
+ * Calls that share scratch or counters must not overlap. */
+typedef struct dak_attn_q4_args {
+  const void *query;          /* [batch, num_q_heads, 128]                      */
+  int64_t q_stride_b, q_stride_h;
+  const int32_t *seq_lens;    /* [batch]                                        */
+  void *out;                  /* [batch, num_q_heads, 128]                      */
+  int64_t o_stride_b, o_stride_h;
+  float *partial_o, *partial_ml;
+  int32_t *merge_counters;
+  int num_q_heads, max_seq_len;
+  int split_size;             /* tokens per split, multiple of 64               */
+  float scaling;
+  int dtype;
+} dak_attn_q4_args;
+DAK_API int dak_attn_decode_paged_q4(const dak_kv4_cache *cache, const dak_attn_q4_args *args, void *stream);
+
+/* ------------------------------------------------------------ cache pages */
+/* Copies page src[i] to page dst[i] (host arrays; v >= 0 names device page v,
+ * v < 0 host page -1 - v) for i < n <= 3584 in each of `slabs` slabs, which lie
+ * *_slab_stride bytes apart and hold their pool's pages one after the other.
+ * Any page format: page_bytes is a multiple of 16.  The copies of one call run
+ * at the same time, so a destination named twice, or also named as a source, is
+ * refused.  One launch; the list travels with it and may be reused at once.
+ * Replaces no reference function: the reference's cache has no pages
+ * (app/python/pinned_static_cache.py:8-115). */
+DAK_API int dak_copy_pages(void *pool_dev, int64_t dev_pages, void *pool_host, int64_t host_pages, int64_t page_bytes,
+                           int slabs, int64_t dev_slab_stride, int64_t host_slab_stride, const int32_t *src,
+                           const int32_t *dst, int n, void *stream);
+
 /* ------------------------------------------------------------ diagnostics */
 /* Reads (and with clear != 0 resets) the device-side error word that kernels
  * set when a bounded wait times out (DAK_ERR_TIMEOUT) or a block-table entry
