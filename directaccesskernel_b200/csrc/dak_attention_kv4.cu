@@ -6,8 +6,11 @@
 // (sequence, KV head, block of up to 8 query heads, split of the tokens); the
 // splits' (o, m, l) are merged with log-sum-exp.  Scores are kept in base 2.
 // A sequence of no tokens gives zeros.
+#include <cudaTypedefs.h>
+
 #include <cfloat>
 #include <cstring>
+#include <type_traits>
 
 #include "dak_common.cuh"
 #include "dak_host.h"
@@ -18,9 +21,12 @@ namespace {
 
 constexpr int kQ4Warps = 4;
 constexpr int kQ4Threads = kQ4Warps * 32;
-constexpr int kQ4Heads = 8;  // query heads per CTA
+constexpr int kQ4Heads = 8;    // query heads per CTA: the MMA's N
+constexpr int kQ4Chunk = 64;   // tokens a warp takes at a time
+constexpr int kQ4Stages = 2;   // chunks in flight per warp
 
-struct AttnQ4Params {
+struct alignas(64) AttnQ4Params {
+  CUtensorMap map[2];  // device, host pool: dims {64 bytes, slab rows, pages x heads}
   Kv4Cache c;
   const uint16_t *query;
   long long q_stride_b, q_stride_h;
@@ -35,27 +41,145 @@ struct AttnQ4Params {
   int pdl;
 };
 
-// Sum of the splits' partials of one query head at dim d, in split order.
-template <typename T>
-__device__ __forceinline__ void merge_q4(const AttnQ4Params &p, int b, int hq, int d) {
-  const long long base = ((long long)b * p.num_q_heads + hq) * p.num_splits;
-  float gm = -FLT_MAX;
-  for (int s = 0; s < p.num_splits; ++s) gm = fmaxf(gm, __ldcg(p.partial_ml + (base + s) * 2));
-  float den = 0.f, acc = 0.f;
-  for (int s = 0; s < p.num_splits; ++s) {
-    const float c = exp2f(__ldcg(p.partial_ml + (base + s) * 2) - gm);  // an empty split has l = 0 and o = 0
-    den = fmaf(__ldcg(p.partial_ml + (base + s) * 2 + 1), c, den);
-    acc = fmaf(__ldcg(p.partial_o + (base + s) * kKv4Dim + d), c, acc);
+// Shared memory of a CTA: per warp a ring of chunks, then barriers and the
+// warps' softmax statistics.  After the last chunk a warp's ring holds its
+// partial outputs.
+template <int NG>
+struct Q4Smem {
+  static constexpr uint32_t stage = 2 * kQ4Chunk * (64 + 4 * NG);
+  static constexpr uint32_t bar_off = kQ4Warps * kQ4Stages * stage;
+  static constexpr uint32_t m_off = bar_off + kQ4Warps * kQ4Stages * 8;  // [warps][heads]
+  static constexpr uint32_t l_off = m_off + kQ4Warps * kQ4Heads * 4;
+  static constexpr uint32_t flag_off = l_off + kQ4Warps * kQ4Heads * 4;
+  static constexpr uint32_t bytes = flag_off + 16 + 512;  // 512: alignment
+  static_assert(stage % 512 == 0 && kQ4Stages * stage >= kQ4Heads * kKv4Dim * 4, "a ring must hold a partial output");
+};
+
+__device__ __forceinline__ void tma_load_slab(uint32_t dst, const CUtensorMap *map, int slab, uint32_t bar,
+                                              uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      ".L2::cache_hint [%0], [%1, {%2, %2, %3}], [%4], %5;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(slab), "r"(bar), "l"(policy)
+      : "memory");
+}
+
+// Address of byte x of shared memory as the 64-byte TMA swizzle stored it.
+__device__ __forceinline__ uint32_t swz(uint32_t x) { return x ^ ((x >> 3) & 0x30u); }
+
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+
+// The (scale, zero) words of one token, one per group.
+template <int NG> __device__ __forceinline__ void lds_pairs(uint32_t a, uint32_t (&w)[NG]) {
+  if constexpr (NG == 1) {
+    w[0] = lds32(a);
+  } else if constexpr (NG == 2) {
+    const uint2 v = lds64(a);
+    w[0] = v.x;
+    w[1] = v.y;
+  } else {
+    const uint4 v = lds128(a);
+    w[0] = v.x;
+    w[1] = v.y;
+    w[2] = v.z;
+    w[3] = v.w;
   }
-  p.out[b * p.o_stride_b + hq * p.o_stride_h + d] = Elem<T>::from_float(den == 0.f ? 0.f : acc / den);
+}
+
+__device__ __forceinline__ float2 half2_of(uint32_t w) { return __half22float2(*reinterpret_cast<__half2 *>(&w)); }
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// D += A (16x16, row) * B (16x8, col), float16 in, FP32 accumulators.
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+               "{%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The transpose of an 8x8 matrix of 16-bit elements spread over the warp.
+__device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+// floor(log2 s) of a non-negative float16 value held in FP32, at least -24.
+__device__ __forceinline__ float exponent_of(float s) {
+  const float e = __uint_as_float(0x4B000000u | (__float_as_uint(s) >> 23)) - (8388608.f + 127.f);
+  return fmaxf(e, -24.f);
+}
+
+// Splits that hold tokens of a sequence (at least one, which writes the zeros of
+// an empty sequence).
+__device__ __forceinline__ int live_splits(const AttnQ4Params &p, int seq) {
+  return max(1, (seq + p.split_size - 1) / p.split_size);
+}
+
+// Log-sum-exp merge of a block of heads' split partials by 128 threads, in split
+// order: first each warp forms the maximum and denominator of two heads, then
+// thread d sums dim d of every head.
+template <typename T>
+__device__ __forceinline__ void merge_q4(const AttnQ4Params &p, int b, int h0, int nh, int splits, float *sm) {
+  const long long base = ((long long)b * p.num_q_heads + h0) * p.num_splits;
+  for (int h = warp_id(); h < nh; h += kQ4Warps) {
+    const float2 *ml = reinterpret_cast<const float2 *>(p.partial_ml) + base + (long long)h * p.num_splits;
+    float gm = -FLT_MAX, den = 0.f;
+    for (int s = lane_id(); s < splits; s += 32) gm = fmaxf(gm, __ldcg(ml + s).x);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, x));
+    for (int s = lane_id(); s < splits; s += 32) {
+      const float2 v = __ldcg(ml + s);
+      den = fmaf(v.y, exp2f(v.x - gm), den);
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) den += __shfl_xor_sync(0xffffffffu, den, x);
+    if (lane_id() == 0) {
+      sm[h] = gm;
+      sm[kQ4Heads + h] = den;
+    }
+  }
+  __syncthreads();
+  const int d = threadIdx.x;
+  for (int h = 0; h < nh; ++h) {
+    const long long at = base + (long long)h * p.num_splits;
+    const float gm = sm[h], den = sm[kQ4Heads + h];
+    float acc = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s)
+      acc = fmaf(__ldcg(p.partial_o + (at + s) * kKv4Dim + d), exp2f(__ldcg(p.partial_ml + (at + s) * 2) - gm), acc);
+    p.out[b * p.o_stride_b + (h0 + h) * p.o_stride_h + d] = Elem<T>::from_float(den == 0.f ? 0.f : acc / den);
+  }
 }
 
 template <typename T, int NG>
-__global__ void __launch_bounds__(kQ4Threads) attn_q4_kernel(const __grid_constant__ AttnQ4Params p) {
-  __shared__ float sm_m[kQ4Warps][kQ4Heads], sm_l[kQ4Warps][kQ4Heads], sm_o[kQ4Warps][kQ4Heads][kKv4Dim];
-  __shared__ int last;
+__global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_constant__ AttnQ4Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  using S = Q4Smem<NG>;
+  // The weights of a float16 output are split into two float16 terms.
+  constexpr bool kTwoTerms = std::is_same<T, __half>::value;
+  uint8_t *smem = smem_raw + ((512u - (smem_u32(smem_raw) & 511u)) & 511u);
+  const uint32_t sbase = smem_u32(smem);
   pdl_enter(p.pdl);
   const int warp = warp_id(), lane = lane_id();
+  const int g = lane >> 2, cq = lane & 3;  // fragment row, column pair
   int i = blockIdx.x;
   const int split = i % p.num_splits;
   i /= p.num_splits;
@@ -63,77 +187,395 @@ __global__ void __launch_bounds__(kQ4Threads) attn_q4_kernel(const __grid_consta
   i /= p.head_blocks;
   const int kvh = i % p.c.kv_heads;
   const int b = i / p.c.kv_heads;
+  const int seq = max(0, min(p.seq_lens[b], p.max_seq_len));
+  const int splits = live_splits(p, seq);
+  if (split >= splits) return;
   const int h0 = kvh * p.group + hb * p.block_heads;
   const int nh = min(p.block_heads, p.group - hb * p.block_heads);
-  const int seq = min(p.seq_lens[b], p.max_seq_len);
   const int t0 = split * p.split_size, t1 = min(seq, t0 + p.split_size);
-  const int P = p.c.page_size, half = kv4_half_bytes(P, NG);
+  const int chunks = (t1 - t0 + kQ4Chunk - 1) / kQ4Chunk;
+  const int mine = chunks > warp ? (chunks - warp + kQ4Warps - 1) / kQ4Warps : 0;  // this warp's chunks
+  const int P = p.c.page_size, lp = 31 - __clz(P), ppc = kQ4Chunk >> lp;  // pages per chunk
+  const uint32_t slab = (uint32_t)p.c.slab_bytes, half = slab / 2;
 
-  // Lane owns dims 4 lane .. +3, in group lane / (32 / NG).
-  float q[kQ4Heads][4], o[kQ4Heads][4], m[kQ4Heads], l[kQ4Heads];
+  const uint32_t ring = sbase + warp * kQ4Stages * S::stage;
+  const uint32_t bar0 = sbase + S::bar_off + warp * kQ4Stages * 8;
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + S::flag_off);
+  const WaitCtx wc{abort_flag, p.c.status};
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kQ4Warps * kQ4Stages; ++s) mbar_init(sbase + S::bar_off + 8 * s, 1);
+    abort_flag[0] = abort_flag[1] = 0;  // [1]: of the wait for copies in flight
+    fence_mbar_init();
+  }
+  __syncthreads();
+
+  // Block-table entries: lane l holds entry l of a window of 32 / ppc chunks, and
+  // the window after it is already on its way.
+  const int per_win = 32 / ppc;
+  const int32_t *row = p.c.table + (long long)b * p.c.table_stride;
+  const int last_page = (t1 - 1) / P;
+  auto window = [&](int first) {  // entries of chunks first .. of this warp
+    const int j = first + lane / ppc;
+    const int page = (t0 + (warp + j * kQ4Warps) * kQ4Chunk) / P + lane % ppc;
+    return j < mine && page <= last_page ? row[page] : 0;
+  };
+  int cur = window(0), nxt = window(per_win);
+  const uint64_t pol = l2_policy_evict_first();
+  auto issue = [&](int j) {  // chunk j of this warp into its stage
+    if (j % per_win == 0 && j > 0) {
+      cur = nxt;
+      nxt = window(j + per_win);
+    }
+    const int entry = __shfl_sync(0xffffffffu, cur, (j % per_win) * ppc + lane % ppc);
+    const int first = t0 + (warp + j * kQ4Warps) * kQ4Chunk;
+    const int pages = min(ppc, last_page - first / P + 1);
+    const int s = j % kQ4Stages;
+    if (lane == 0) mbar_arrive_expect_tx(bar0 + 8 * s, pages * slab);
+    __syncwarp();
+    if (lane < pages) {
+      const int tier = entry < 0 ? 1 : 0;
+      long long page = entry < 0 ? -1ll - entry : entry;
+      if (page >= p.c.pages[tier]) {  // the copy starts past the map's end and reads zeros
+        atomicCAS(p.c.status, 0, DAK_ERR_INVALID_ARG);
+        page = max(1ll, p.c.pages[tier]);
+      }
+      tma_load_slab(ring + s * S::stage + lane * slab, &p.map[tier], (int)(page * p.c.kv_heads + kvh), bar0 + 8 * s, pol);
+    }
+    __syncwarp();
+  };
+  const int ahead = min(mine, kQ4Stages);
+  for (int j = 0; j < ahead; ++j) issue(j);
+
+  // Word w (0..3) of a K row that this lane multiplies, 8 dims each: all the
+  // words of one group meet in the same MMA steps.
+  auto k_word = [&](int w) {
+    return NG == 1 ? 4 * cq + w : NG == 2 ? 8 * (w >> 1) + 2 * cq + (w & 1) : 4 * w + cq;
+  };
+  // Query of head g: scaled by a power of two to below 2^14 and to float16 (the
+  // values that float16 cannot hold are 2^-38 of the largest), and summed
+  // over each group for the zeros' share.
+  uint32_t qf[8][2];
+  float qs[2][NG], f[2];
+  {
+    float x[4][8], mx = 0.f, sum[NG];
 #pragma unroll
-  for (int h = 0; h < kQ4Heads; ++h) {
-    m[h] = -FLT_MAX;
-    l[h] = 0.f;
+    for (int n = 0; n < NG; ++n) sum[n] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      o[h][e] = 0.f;
-      q[h][e] = h < nh ? Elem<T>::to_float(p.query[b * p.q_stride_b + (h0 + h) * p.q_stride_h + 4 * lane + e]) : 0.f;
+    for (int w = 0; w < 4; ++w) {
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (g < nh)
+        v = *reinterpret_cast<const uint4 *>(p.query + b * p.q_stride_b + (h0 + g) * p.q_stride_h + 8 * k_word(w));
+      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 y = Elem<T>::to_float2(u[e]);
+        x[w][2 * e] = y.x;
+        x[w][2 * e + 1] = y.y;
+        mx = fmaxf(mx, fmaxf(fabsf(y.x), fabsf(y.y)));
+      }
+    }
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    const int k = mx > 0.f ? max(-100, min(100, 13 - ((int)(__float_as_uint(mx) >> 23) - 127))) : 0;
+    const float up = __uint_as_float((uint32_t)(127 + k) << 23);
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float a = x[w][2 * h] * up, c = x[w][2 * h + 4] * up;
+        const float d = x[w][2 * h + 1] * up, e = x[w][2 * h + 5] * up;
+        qf[2 * w + h][0] = pack_half2(a, c);
+        qf[2 * w + h][1] = pack_half2(d * 0.0625f, e * 0.0625f);
+        sum[w * NG / 4] += (a + c) + (d + e);
+      }
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 1);
+      sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 2);
+    }
+    const float fh = p.scale_log2 * __uint_as_float((uint32_t)(127 + 24 - k) << 23);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {  // lane 4h holds head h
+      const int src = 4 * (2 * cq + e);
+      f[e] = __shfl_sync(0xffffffffu, fh, src);
+#pragma unroll
+      for (int n = 0; n < NG; ++n) qs[e][n] = __shfl_sync(0xffffffffu, sum[n], src) * 0x1p-24f;
     }
   }
-  for (int t = t0 + warp; t < t1; t += kQ4Warps) {
-    int tier = 0;
-    const uint8_t *slab = kv4_page(p.c, b, t / P, &tier);
-    float k[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (!slab) {
-      if (lane == 0) atomicCAS(p.c.status, 0, DAK_ERR_INVALID_ARG);  // reads zeros
-    } else {
-      slab += (long long)kvh * p.c.slab_bytes;
+
+  // V: this lane takes 4 dims at a time (piece x) of tokens 2 cq, 2 cq + 1 (and 8
+  // on).  Odd columns read the second token first, which spreads a warp's reads
+  // over all banks; the byte selectors put the pair back in order.
+  const uint32_t flip = cq & 1;
+  const uint32_t sel_lo = flip ? 0x1054u : 0x5410u, sel_hi = flip ? 0x3276u : 0x7632u;
+  const uint32_t sel_g = (g & 1) ? sel_hi : sel_lo;
+
+  float o[8][4], m[2] = {-FLT_MAX, -FLT_MAX}, l[2] = {0.f, 0.f};
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const uint8_t *part = slab + kv * half;
-        const uint32_t w = *reinterpret_cast<const uint16_t *>(part + (t % P) * 64 + 2 * lane);
-        const __half2 sz = *reinterpret_cast<const __half2 *>(part + P * 64 + ((t % P) * NG + lane / (32 / NG)) * 4);
+  for (int t = 0; t < 8; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          (kv ? v : k)[e] = fmaf(__low2float(sz), (float)((w >> (4 * e)) & 15u), __high2float(sz));
+    for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
+
+  // One chunk: tokens first .. first + valid - 1 in stage `st`.
+  auto chunk = [&](uint32_t st, int valid, auto full_c) {
+    constexpr bool kFull = decltype(full_c)::value;
+    float y[4][4];  // scores in base 2: tile, {token g, g + 8} x {head 2 cq, 2 cq + 1}
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int page = (t * 16) >> lp, r0 = (t * 16) & (P - 1);
+      const uint32_t kb = st + page * slab;
+      if (!kFull && t * 16 >= valid) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[t][e] = -INFINITY;
+        continue;
+      }
+      // S^T = K Q^T with the codes as they are: a nibble at bits 0-3 of a half word
+      // is the subnormal code * 2^-24, at bits 4-7 code * 2^-20 (its q is / 16).
+      const uint32_t ka = kb + (r0 + g) * 64;
+      uint32_t w0[4], w1[4];  // tokens g and g + 8
+      if constexpr (NG == 1) {
+        const uint32_t a = swz(ka + 16 * cq);
+        const uint4 u = lds128(a), v = lds128(a + 512);
+        w0[0] = u.x, w0[1] = u.y, w0[2] = u.z, w0[3] = u.w;
+        w1[0] = v.x, w1[1] = v.y, w1[2] = v.z, w1[3] = v.w;
+      } else if constexpr (NG == 2) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const uint32_t a = swz(ka + 32 * n + 8 * cq);
+          const uint2 u = lds64(a), v = lds64(a + 512);
+          w0[2 * n] = u.x, w0[2 * n + 1] = u.y;
+          w1[2 * n] = v.x, w1[2 * n + 1] = v.y;
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const uint32_t a = swz(ka + 16 * n + 4 * cq);
+          w0[n] = lds32(a);
+          w1[n] = lds32(a + 512);
+        }
+      }
+      uint32_t kp[2][NG], vp[2][NG];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t at = kb + P * 64 + (r0 + g + 8 * r) * (4 * NG);
+        lds_pairs<NG>(swz(at), kp[r]);
+        lds_pairs<NG>(swz(at + half), vp[r]);
+      }
+      float sc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = n * 4 / NG; w < (n + 1) * 4 / NG; ++w) {
+          mma_f16(acc, w0[w] & 0x000F000Fu, w1[w] & 0x000F000Fu, w0[w] & 0x00F000F0u, w1[w] & 0x00F000F0u, qf[2 * w][0],
+                  qf[2 * w][1]);
+          const uint32_t s0 = w0[w] >> 8, s1 = w1[w] >> 8;
+          mma_f16(acc, s0 & 0x000F000Fu, s1 & 0x000F000Fu, s0 & 0x00F000F0u, s1 & 0x00F000F0u, qf[2 * w + 1][0],
+                  qf[2 * w + 1][1]);
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float2 sz = half2_of(kp[r][n]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            sc[2 * r + e] = fmaf(sz.x, acc[2 * r + e], sc[2 * r + e]);
+            sc[2 * r + e] = fmaf(sz.y, qs[e][n], sc[2 * r + e]);
+          }
+        }
+      }
+      // The maximum is taken over score + log2(V scale), so that the weight times
+      // the scale is below 2 and float16 keeps it whatever V's magnitude.
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float s = half2_of(vp[r][0]).x;
+#pragma unroll
+        for (int n = 1; n < NG; ++n) s = fmaxf(s, half2_of(vp[r][n]).x);
+        const bool in = kFull || t * 16 + 8 * r + g < valid;
+        const float ex = exponent_of(s);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float v = sc[2 * r + e] * f[e];
+          y[t][2 * r + e] = in ? v : -INFINITY;
+          mx[e] = in ? fmaxf(mx[e], v + ex) : mx[e];
+        }
+      }
+    }
+    float alpha[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int x = 4; x <= 16; x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
+      const float mn = fmaxf(m[e], mx[e]);
+      alpha[e] = exp2f(m[e] - mn);
+      m[e] = mn;
+      l[e] *= alpha[e];
+    }
+    // Weights, and the zeros' share of the output: sum_t p_t zero_t per group.
+    float zs[2][NG];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int n = 0; n < NG; ++n) zs[e][n] = 0.f;
+    uint32_t vp[4][2][NG];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int page = (t * 16) >> lp, r0 = (t * 16) & (P - 1);
+      if (!kFull && t * 16 >= valid) continue;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        lds_pairs<NG>(swz(st + page * slab + half + P * 64 + (r0 + g + 8 * r) * (4 * NG)), vp[t][r]);
+        const bool in = kFull || t * 16 + 8 * r + g < valid;
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+          if (!in) vp[t][r][n] = 0u;  // anything may lie behind the last token
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float w = exp2f(y[t][2 * r + e] - m[e]);
+          y[t][2 * r + e] = w;
+          l[e] += w;
+#pragma unroll
+          for (int n = 0; n < NG; ++n) zs[e][n] = fmaf(w, half2_of(vp[t][r][n]).y, zs[e][n]);
+        }
       }
     }
 #pragma unroll
-    for (int h = 0; h < kQ4Heads; ++h) {
-      float s = q[h][0] * k[0] + q[h][1] * k[1] + q[h][2] * k[2] + q[h][3] * k[3];
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
-      for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      s *= p.scale_log2;
-      const float mn = fmaxf(m[h], s);
-      const float a = exp2f(m[h] - mn), w = exp2f(s - mn);
-      m[h] = mn;
-      l[h] = l[h] * a + w;
+      for (int n = 0; n < NG; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[h][e] = fmaf(w, v[e], o[h][e] * a);
+        for (int x = 4; x <= 16; x <<= 1) zs[e][n] += __shfl_xor_sync(0xffffffffu, zs[e][n], x);
+    // O rows: even dims count codes * 2^-24, odd dims * 2^-20.  Adding the zeros'
+    // share chunk by chunk keeps O centred, so nothing cancels at the end.
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        o[t][e] = fmaf(o[t][e], alpha[e & 1], zs[e & 1][(t >> 1) * NG / 4] * (e < 2 ? 0x1p-24f : 0x1p-20f));
+    // O^T += V^T P^T
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int page = (t * 16) >> lp, r0 = (t * 16) & (P - 1);
+      if (!kFull && t * 16 >= valid) continue;
+      const uint32_t vb = st + page * slab + half + r0 * 64;
+      uint32_t bf[NG][2];
+      [[maybe_unused]] uint32_t bl[NG][2];
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float s = half2_of(vp[t][r][n]).x;
+          const float a = y[t][2 * r] * s, c = y[t][2 * r + 1] * s;
+          const uint32_t hi = pack_half2(a, c);
+          bf[n][r] = movmatrix(hi);
+          if constexpr (kTwoTerms) {
+            const float2 back = half2_of(hi);
+            bl[n][r] = movmatrix(pack_half2(a - back.x, c - back.y));
+          }
+        }
+      uint32_t x[2][4];  // token pairs (2 cq, +1) and (2 cq + 8, +9): 4 pieces of 4 dims
+      const uint32_t row0 = vb + (2 * cq + flip) * 64, row1 = vb + (2 * cq + 1 - flip) * 64;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        if constexpr (NG == 1) {
+          const uint2 u = lds64(swz(row0 + 8 * g) + 512 * r), v = lds64(swz(row1 + 8 * g) + 512 * r);
+          x[r][0] = __byte_perm(u.x, v.x, sel_lo);
+          x[r][1] = __byte_perm(u.x, v.x, sel_hi);
+          x[r][2] = __byte_perm(u.y, v.y, sel_lo);
+          x[r][3] = __byte_perm(u.y, v.y, sel_hi);
+        } else if constexpr (NG == 2) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const uint32_t u = lds32(swz(row0 + 32 * n + 4 * g) + 512 * r), v = lds32(swz(row1 + 32 * n + 4 * g) + 512 * r);
+            x[r][2 * n] = __byte_perm(u, v, sel_lo);
+            x[r][2 * n + 1] = __byte_perm(u, v, sel_hi);
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const uint32_t u = lds32(swz(row0 + 16 * n + 4 * (g >> 1)) + 512 * r);
+            const uint32_t v = lds32(swz(row1 + 16 * n + 4 * (g >> 1)) + 512 * r);
+            x[r][n] = __byte_perm(u, v, sel_g);
+          }
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = q * NG / 4;
+        const uint32_t s0 = x[0][q] >> 8, s1 = x[1][q] >> 8;
+        mma_f16(o[2 * q], x[0][q] & 0x000F000Fu, x[0][q] & 0x00F000F0u, x[1][q] & 0x000F000Fu, x[1][q] & 0x00F000F0u,
+                bf[n][0], bf[n][1]);
+        mma_f16(o[2 * q + 1], s0 & 0x000F000Fu, s0 & 0x00F000F0u, s1 & 0x000F000Fu, s1 & 0x00F000F0u, bf[n][0], bf[n][1]);
+        if constexpr (kTwoTerms) {
+          mma_f16(o[2 * q], x[0][q] & 0x000F000Fu, x[0][q] & 0x00F000F0u, x[1][q] & 0x000F000Fu, x[1][q] & 0x00F000F0u,
+                  bl[n][0], bl[n][1]);
+          mma_f16(o[2 * q + 1], s0 & 0x000F000Fu, s0 & 0x00F000F0u, s1 & 0x000F000Fu, s1 & 0x00F000F0u, bl[n][0],
+                  bl[n][1]);
+        }
+      }
     }
+  };
+
+  bool ok = true;
+  for (int j = 0; j < mine; ++j) {
+    const int s = j % kQ4Stages;
+    ok = mbar_wait<false>(bar0 + 8 * s, (j / kQ4Stages) & 1, wc);
+    if (!__all_sync(0xffffffffu, ok)) {
+      // Gave up: let this warp's copies land (bounded again), then leave.
+      if (lane == 0) {
+        const WaitCtx drain{reinterpret_cast<volatile int *>(smem + S::flag_off + 4), p.c.status};
+        for (int k = j; k < min(mine, j + kQ4Stages); ++k)
+          mbar_wait<false>(bar0 + 8 * (k % kQ4Stages), (k / kQ4Stages) & 1, drain);
+      }
+      __syncwarp();
+      break;
+    }
+    const uint32_t st = ring + s * S::stage;
+    const int valid = min(kQ4Chunk, t1 - (t0 + (warp + j * kQ4Warps) * kQ4Chunk));
+    if (valid == kQ4Chunk)
+      chunk(st, valid, std::true_type{});
+    else
+      chunk(st, valid, std::false_type{});
+    __syncwarp();
+    if (j + kQ4Stages < mine) issue(j + kQ4Stages);
   }
+
+  // Merge the warps: each leaves (m, l, o) of its heads, o in its own ring.
+  float *sm_m = reinterpret_cast<float *>(smem + S::m_off), *sm_l = reinterpret_cast<float *>(smem + S::l_off);
 #pragma unroll
-  for (int h = 0; h < kQ4Heads; ++h) {
-    if (lane == 0) {
-      sm_m[warp][h] = m[h];
-      sm_l[warp][h] = l[h];
+  for (int e = 0; e < 2; ++e)
+#pragma unroll
+    for (int x = 4; x <= 16; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
+  float *ring_f = reinterpret_cast<float *>(smem + warp * kQ4Stages * S::stage);  // [head][dim]
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int h = 2 * cq + e;
+    if (h >= nh) continue;
+    if (g == 0) {
+      sm_m[warp * kQ4Heads + h] = m[e];
+      sm_l[warp * kQ4Heads + h] = l[e];
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sm_o[warp][h][4 * lane + e] = o[h][e];
+    for (int t = 0; t < 8; ++t) {
+      const int q = t >> 1;
+      const int d = (NG == 1 ? 16 * g + 4 * q : NG == 2 ? 64 * (q >> 1) + 8 * g + 4 * (q & 1) : 32 * q + 4 * g) + 2 * (t & 1);
+      *reinterpret_cast<float2 *>(ring_f + h * kKv4Dim + d) = make_float2(o[t][e] * 0x1p24f, o[t][2 + e] * 0x1p20f);
+    }
   }
   __syncthreads();
   const int d = threadIdx.x;
   for (int h = 0; h < nh; ++h) {
     float gm = -FLT_MAX;
-    for (int w = 0; w < kQ4Warps; ++w) gm = fmaxf(gm, sm_m[w][h]);
+#pragma unroll
+    for (int w = 0; w < kQ4Warps; ++w) gm = fmaxf(gm, sm_m[w * kQ4Heads + h]);
     float den = 0.f, acc = 0.f;
+#pragma unroll
     for (int w = 0; w < kQ4Warps; ++w) {
-      const float c = exp2f(sm_m[w][h] - gm);
-      den = fmaf(sm_l[w][h], c, den);
-      acc = fmaf(sm_o[w][h][d], c, acc);
+      const float c = exp2f(sm_m[w * kQ4Heads + h] - gm);
+      den = fmaf(sm_l[w * kQ4Heads + h], c, den);
+      acc = fmaf(reinterpret_cast<const float *>(smem + w * kQ4Stages * S::stage)[h * kKv4Dim + d], c, acc);
     }
-    if (p.num_splits == 1) {
+    if (splits == 1) {
       p.out[b * p.o_stride_b + (h0 + h) * p.o_stride_h + d] = Elem<T>::from_float(den == 0.f ? 0.f : acc / den);
     } else {
       const long long at = ((long long)b * p.num_q_heads + h0 + h) * p.num_splits + split;
@@ -144,35 +586,47 @@ __global__ void __launch_bounds__(kQ4Threads) attn_q4_kernel(const __grid_consta
       }
     }
   }
-  if (p.num_splits > 1 && p.counters) {
+  if (splits > 1 && p.counters) {
     // The split that finishes last merges all of them and resets the counter.
+    int *last = reinterpret_cast<int *>(smem + S::flag_off + 8);
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
       int32_t *counter = p.counters + blockIdx.x / p.num_splits;
-      last = atomicAdd(counter, 1) == p.num_splits - 1;
-      if (last) *counter = 0;
+      *last = atomicAdd(counter, 1) == splits - 1;
+      if (*last) *counter = 0;
     }
     __syncthreads();
-    if (last) {
+    if (*last) {
       __threadfence();
-      for (int h = 0; h < nh; ++h) merge_q4<T>(p, b, h0 + h, d);
+      merge_q4<T>(p, b, h0, nh, splits, sm_m);
     }
   }
 }
 
+// The merge as a launch of its own, one CTA per block of heads.
 template <typename T>
-__global__ void __launch_bounds__(kKv4Dim) attn_q4_merge_kernel(const __grid_constant__ AttnQ4Params p) {
+__global__ void __launch_bounds__(kQ4Threads) attn_q4_merge_kernel(const __grid_constant__ AttnQ4Params p) {
+  __shared__ float sm[2 * kQ4Heads];
   pdl_enter(p.pdl);
-  merge_q4<T>(p, blockIdx.x / p.num_q_heads, blockIdx.x % p.num_q_heads, threadIdx.x);
+  int i = blockIdx.x;
+  const int hb = i % p.head_blocks;
+  i /= p.head_blocks;
+  const int kvh = i % p.c.kv_heads;
+  const int b = i / p.c.kv_heads;
+  const int splits = live_splits(p, max(0, min(p.seq_lens[b], p.max_seq_len)));
+  if (splits == 1) return;  // written already
+  merge_q4<T>(p, b, kvh * p.group + hb * p.block_heads, min(p.block_heads, p.group - hb * p.block_heads), splits, sm);
 }
 
 template <typename T, int NG>
 cudaError_t launch_attn(const AttnQ4Params &p, long long grid, cudaStream_t s) {
-  cudaError_t e = launch_ex(attn_q4_kernel<T, NG>, dim3((unsigned)grid), dim3(kQ4Threads), 0, s, 1, p.pdl != 0, p);
+  auto kern = attn_q4_kernel<T, NG>;
+  cudaError_t e = prepare_kernel_attributes(reinterpret_cast<const void *>(kern));
+  if (e != cudaSuccess) return e;
+  e = launch_ex(kern, dim3((unsigned)grid), dim3(kQ4Threads), Q4Smem<NG>::bytes, s, 1, p.pdl != 0, p);
   if (e != cudaSuccess || p.num_splits == 1 || p.counters) return e;
-  return launch_ex(attn_q4_merge_kernel<T>, dim3((unsigned)(p.c.rows * p.num_q_heads)), dim3(kKv4Dim), 0, s, 1, p.pdl != 0,
-                   p);
+  return launch_ex(attn_q4_merge_kernel<T>, dim3((unsigned)(grid / p.num_splits)), dim3(kQ4Threads), 0, s, 1, p.pdl != 0, p);
 }
 
 template <typename T>
@@ -182,6 +636,38 @@ cudaError_t launch_attn_t(const AttnQ4Params &p, long long grid, cudaStream_t s)
     case 2: return launch_attn<T, 2>(p, grid, s);
     default: return launch_attn<T, 4>(p, grid, s);
   }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void *ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool ok = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault, &q) ==
+                        cudaSuccess &&
+                    q == cudaDriverEntryPointSuccess;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ok ? ptr : nullptr);
+  }();
+  return fn;
+}
+
+// Map of a pool as slabs of 64-byte rows, one box per slab, stored with the
+// 64-byte swizzle.
+int slab_map(CUtensorMap *out, const Kv4Cache &c, int tier) {
+  const int from = c.pool[tier] ? tier : 1 - tier;  // an absent tier: one page that no entry reaches
+  const long long pages = c.pool[tier] ? c.pages[tier] : 1;
+  const long long slabs = pages * c.kv_heads;
+  if (slabs + c.kv_heads > 0x7fffffffll) return fail(DAK_ERR_UNSUPPORTED, "pages x kv_heads of a pool must stay below 2^31");
+  auto fn = tensor_map_encoder();
+  if (!fn) return fail(DAK_ERR_DRIVER, "cuTensorMapEncodeTiled entry point unavailable");
+  const cuuint64_t dims[3] = {64, (cuuint64_t)c.slab_bytes / 64, (cuuint64_t)slabs};
+  const cuuint64_t strides[2] = {64, (cuuint64_t)c.slab_bytes};
+  const cuuint32_t box[3] = {64, (cuuint32_t)c.slab_bytes / 64, 1};
+  const cuuint32_t es[3] = {1, 1, 1};
+  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, c.pool[from], dims, strides, box, es,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(DAK_ERR_DRIVER, "cuTensorMapEncodeTiled (4-bit KV) failed with %d", (int)r);
+  return DAK_OK;
 }
 
 }  // namespace
@@ -213,6 +699,8 @@ extern "C" int dak_attn_decode_paged_q4(const dak_kv4_cache *cache, const dak_at
   AttnQ4Params p;
   std::memset(&p, 0, sizeof(p));
   if ((st = kv4_view(cache, &p.c))) return st;
+  for (int tier = 0; tier < 2; ++tier)
+    if ((st = slab_map(&p.map[tier], p.c, tier))) return st;
   p.query = static_cast<const uint16_t *>(a->query);
   p.q_stride_b = a->q_stride_b;
   p.q_stride_h = a->q_stride_h;
