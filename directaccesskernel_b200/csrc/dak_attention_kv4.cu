@@ -64,35 +64,24 @@ __device__ __forceinline__ void tma_load_slab(uint32_t dst, const CUtensorMap *m
       : "memory");
 }
 
-// Address of byte x of shared memory as the 64-byte TMA swizzle stored it.
-__device__ __forceinline__ uint32_t swz(uint32_t x) { return x ^ ((x >> 3) & 0x30u); }
-
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
+// Where the 64-byte TMA swizzle put byte `lb` (below 64) of the row `row` rows
+// after offset C of a stage (C a multiple of 64, the stage 512-byte aligned):
+// bits 4-5 are xored with bits 7-8.  C is a constant at every call, so what
+// depends on the lane is the same few values for all tiles.
+__device__ __forceinline__ uint32_t swz(uint32_t C, uint32_t row, uint32_t lb) {
+  return C + row * 64 + (lb ^ ((((C >> 7) + ((row + ((C >> 6) & 1u)) >> 1)) & 3u) << 4));
 }
 
 // The (scale, zero) words of one token, one per group.
-template <int NG> __device__ __forceinline__ void lds_pairs(uint32_t a, uint32_t (&w)[NG]) {
+template <int NG> __device__ __forceinline__ void load_pairs(const uint8_t *a, uint32_t (&w)[NG]) {
   if constexpr (NG == 1) {
-    w[0] = lds32(a);
+    w[0] = *reinterpret_cast<const uint32_t *>(a);
   } else if constexpr (NG == 2) {
-    const uint2 v = lds64(a);
+    const uint2 v = *reinterpret_cast<const uint2 *>(a);
     w[0] = v.x;
     w[1] = v.y;
   } else {
-    const uint4 v = lds128(a);
+    const uint4 v = *reinterpret_cast<const uint4 *>(a);
     w[0] = v.x;
     w[1] = v.y;
     w[2] = v.z;
@@ -100,6 +89,11 @@ template <int NG> __device__ __forceinline__ void lds_pairs(uint32_t a, uint32_t
   }
 }
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float2 half2_of(uint32_t w) { return __half22float2(*reinterpret_cast<__half2 *>(&w)); }
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -109,22 +103,23 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
 // D += A (16x16, row) * B (16x8, col), float16 in, FP32 accumulators.
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-               "{%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // The transpose of an 8x8 matrix of 16-bit elements spread over the warp.
 __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 
-// floor(log2 s) of a non-negative float16 value held in FP32, at least -24.
-__device__ __forceinline__ float exponent_of(float s) {
-  const float e = __uint_as_float(0x4B000000u | (__float_as_uint(s) >> 23)) - (8388608.f + 127.f);
-  return fmaxf(e, -24.f);
+// floor(log2 s) of a float16 s >= 0 given by its bits; -24 (its smallest
+// exponent) for 0.
+__device__ __forceinline__ float exponent_of(uint32_t bits) {
+  const float s = __half2float(__ushort_as_half((unsigned short)bits));
+  return fmaxf((float)((int)(__float_as_uint(s) >> 23) - 127), -24.f);
 }
 
 // Splits that hold tokens of a sequence (at least one, which writes the zeros of
@@ -147,7 +142,7 @@ __device__ __forceinline__ void merge_q4(const AttnQ4Params &p, int b, int h0, i
     for (int x = 16; x > 0; x >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, x));
     for (int s = lane_id(); s < splits; s += 32) {
       const float2 v = __ldcg(ml + s);
-      den = fmaf(v.y, exp2f(v.x - gm), den);
+      den = fmaf(v.y, ex2(v.x - gm), den);
     }
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) den += __shfl_xor_sync(0xffffffffu, den, x);
@@ -164,13 +159,13 @@ __device__ __forceinline__ void merge_q4(const AttnQ4Params &p, int b, int h0, i
     float acc = 0.f;
 #pragma unroll 4
     for (int s = 0; s < splits; ++s)
-      acc = fmaf(__ldcg(p.partial_o + (at + s) * kKv4Dim + d), exp2f(__ldcg(p.partial_ml + (at + s) * 2) - gm), acc);
+      acc = fmaf(__ldcg(p.partial_o + (at + s) * kKv4Dim + d), ex2(__ldcg(p.partial_ml + (at + s) * 2) - gm), acc);
     p.out[b * p.o_stride_b + (h0 + h) * p.o_stride_h + d] = Elem<T>::from_float(den == 0.f ? 0.f : acc / den);
   }
 }
 
-template <typename T, int NG>
-__global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_constant__ AttnQ4Params p) {
+template <typename T, int NG, int P>
+__global__ void __launch_bounds__(kQ4Threads, NG == 4 ? 2 : 3) attn_q4_kernel(const __grid_constant__ AttnQ4Params p) {
   extern __shared__ uint8_t smem_raw[];
   using S = Q4Smem<NG>;
   // The weights of a float16 output are split into two float16 terms.
@@ -195,8 +190,8 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
   const int t0 = split * p.split_size, t1 = min(seq, t0 + p.split_size);
   const int chunks = (t1 - t0 + kQ4Chunk - 1) / kQ4Chunk;
   const int mine = chunks > warp ? (chunks - warp + kQ4Warps - 1) / kQ4Warps : 0;  // this warp's chunks
-  const int P = p.c.page_size, lp = 31 - __clz(P), ppc = kQ4Chunk >> lp;  // pages per chunk
-  const uint32_t slab = (uint32_t)p.c.slab_bytes, half = slab / 2;
+  constexpr int ppc = kQ4Chunk / P;  // pages per chunk
+  constexpr uint32_t half = kv4_half_bytes(P, NG), slab = 2 * half;
 
   const uint32_t ring = sbase + warp * kQ4Stages * S::stage;
   const uint32_t bar0 = sbase + S::bar_off + warp * kQ4Stages * 8;
@@ -211,7 +206,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
 
   // Block-table entries: lane l holds entry l of a window of 32 / ppc chunks, and
   // the window after it is already on its way.
-  const int per_win = 32 / ppc;
+  constexpr int per_win = 32 / ppc;
   const int32_t *row = p.c.table + (long long)b * p.c.table_stride;
   const int last_page = (t1 - 1) / P;
   auto window = [&](int first) {  // entries of chunks first .. of this warp
@@ -277,7 +272,9 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     const int k = mx > 0.f ? max(-100, min(100, 13 - ((int)(__float_as_uint(mx) >> 23) - 127))) : 0;
-    const float up = __uint_as_float((uint32_t)(127 + k) << 23);
+    // A negative scaling turns the query over, so that a larger raw score is
+    // always a larger score.
+    const float up = copysignf(__uint_as_float((uint32_t)(127 + k) << 23), p.scale_log2);
 #pragma unroll
     for (int w = 0; w < 4; ++w)
 #pragma unroll
@@ -293,7 +290,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
       sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 1);
       sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 2);
     }
-    const float fh = p.scale_log2 * __uint_as_float((uint32_t)(127 + 24 - k) << 23);
+    const float fh = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 + 24 - k) << 23);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {  // lane 4h holds head h
       const int src = 4 * (2 * cq + e);
@@ -310,59 +307,71 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
   const uint32_t sel_lo = flip ? 0x1054u : 0x5410u, sel_hi = flip ? 0x3276u : 0x7632u;
   const uint32_t sel_g = (g & 1) ? sel_hi : sel_lo;
 
-  float o[8][4], m[2] = {-FLT_MAX, -FLT_MAX}, l[2] = {0.f, 0.f};
+  // Statistics: weights are 2^(score - m).  m is the largest score so far plus E,
+  // the exponent of the warp's largest V scale so far, so that weight x scale is
+  // below 2 and float16 holds it whatever V's magnitude.
+  float o[8][4], m[2] = {-FLT_MAX, -FLT_MAX}, l[2] = {0.f, 0.f}, E = -24.f;
+  uint32_t s_max = 0u;
 #pragma unroll
   for (int t = 0; t < 8; ++t)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
 
-  // One chunk: tokens first .. first + valid - 1 in stage `st`.
-  auto chunk = [&](uint32_t st, int valid, auto full_c) {
+  // One chunk of `valid` tokens in the stage at `st`.
+  auto chunk = [&](const uint8_t *st, int valid, auto full_c) {
     constexpr bool kFull = decltype(full_c)::value;
-    float y[4][4];  // scores in base 2: tile, {token g, g + 8} x {head 2 cq, 2 cq + 1}
+    // Offset of tile t's first code row (V: + half) and of its pairs of token g + 8r.
+    auto rows_at = [](int t) { return (uint32_t)((16 * t) / P * slab + (16 * t) % P * 64); };
+    auto pairs_at = [&](int t, int r) {
+      const uint32_t c = (16 * t) / P * slab + P * 64 + (16 * t) % P * (4 * NG);
+      return NG == 4 ? swz(c + 128 * r, g >> 2, 16 * (g & 3)) : NG == 2 ? swz(c + 64 * r, 0, 8 * g) : swz(c, 0, 4 * g + 32 * r);
+    };
+    auto vpairs_at = [&](int t, int r) {
+      const uint32_t c = (16 * t) / P * slab + half + P * 64 + (16 * t) % P * (4 * NG);
+      return NG == 4 ? swz(c + 128 * r, g >> 2, 16 * (g & 3)) : NG == 2 ? swz(c + 64 * r, 0, 8 * g) : swz(c, 0, 4 * g + 32 * r);
+    };
+    float y[4][4];  // raw scores: tile, {token g, g + 8} x {head 2 cq, 2 cq + 1}
     float mx[2] = {-INFINITY, -INFINITY};
+    uint32_t vp[4][2][NG];
+    __half2 vmax = __float2half2_rn(0.f);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const int page = (t * 16) >> lp, r0 = (t * 16) & (P - 1);
-      const uint32_t kb = st + page * slab;
-      if (!kFull && t * 16 >= valid) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[t][e] = -INFINITY;
-        continue;
-      }
+      if (!kFull && t * 16 >= valid) continue;
       // S^T = K Q^T with the codes as they are: a nibble at bits 0-3 of a half word
       // is the subnormal code * 2^-24, at bits 4-7 code * 2^-20 (its q is / 16).
-      const uint32_t ka = kb + (r0 + g) * 64;
       uint32_t w0[4], w1[4];  // tokens g and g + 8
       if constexpr (NG == 1) {
-        const uint32_t a = swz(ka + 16 * cq);
-        const uint4 u = lds128(a), v = lds128(a + 512);
+        const uint8_t *a = st + swz(rows_at(t), g, 16 * cq);
+        const uint4 u = *reinterpret_cast<const uint4 *>(a), v = *reinterpret_cast<const uint4 *>(a + 512);
         w0[0] = u.x, w0[1] = u.y, w0[2] = u.z, w0[3] = u.w;
         w1[0] = v.x, w1[1] = v.y, w1[2] = v.z, w1[3] = v.w;
       } else if constexpr (NG == 2) {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          const uint32_t a = swz(ka + 32 * n + 8 * cq);
-          const uint2 u = lds64(a), v = lds64(a + 512);
+          const uint8_t *a = st + swz(rows_at(t), g, 32 * n + 8 * cq);
+          const uint2 u = *reinterpret_cast<const uint2 *>(a), v = *reinterpret_cast<const uint2 *>(a + 512);
           w0[2 * n] = u.x, w0[2 * n + 1] = u.y;
           w1[2 * n] = v.x, w1[2 * n + 1] = v.y;
         }
       } else {
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-          const uint32_t a = swz(ka + 16 * n + 4 * cq);
-          w0[n] = lds32(a);
-          w1[n] = lds32(a + 512);
+          const uint8_t *a = st + swz(rows_at(t), g, 16 * n + 4 * cq);
+          w0[n] = *reinterpret_cast<const uint32_t *>(a);
+          w1[n] = *reinterpret_cast<const uint32_t *>(a + 512);
         }
       }
-      uint32_t kp[2][NG], vp[2][NG];
+      uint32_t kp[2][NG];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const uint32_t at = kb + P * 64 + (r0 + g + 8 * r) * (4 * NG);
-        lds_pairs<NG>(swz(at), kp[r]);
-        lds_pairs<NG>(swz(at + half), vp[r]);
+        load_pairs<NG>(st + pairs_at(t, r), kp[r]);
+        load_pairs<NG>(st + vpairs_at(t, r), vp[t][r]);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          if (!kFull && t * 16 + 8 * r + g >= valid) vp[t][r][n] = 0u;  // anything may lie behind the last token
+          vmax = __hmax2(vmax, *reinterpret_cast<const __half2 *>(&vp[t][r][n]));
+        }
       }
-      float sc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -379,65 +388,53 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
           const float2 sz = half2_of(kp[r][n]);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            sc[2 * r + e] = fmaf(sz.x, acc[2 * r + e], sc[2 * r + e]);
-            sc[2 * r + e] = fmaf(sz.y, qs[e][n], sc[2 * r + e]);
+            const float zq = n == 0 ? sz.y * qs[e][n] : fmaf(sz.y, qs[e][n], y[t][2 * r + e]);
+            y[t][2 * r + e] = fmaf(sz.x, acc[2 * r + e], zq);
           }
         }
       }
-      // The maximum is taken over score + log2(V scale), so that the weight times
-      // the scale is below 2 and float16 keeps it whatever V's magnitude.
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float s = half2_of(vp[r][0]).x;
+      for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int n = 1; n < NG; ++n) s = fmaxf(s, half2_of(vp[r][n]).x);
-        const bool in = kFull || t * 16 + 8 * r + g < valid;
-        const float ex = exponent_of(s);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float v = sc[2 * r + e] * f[e];
-          y[t][2 * r + e] = in ? v : -INFINITY;
-          mx[e] = in ? fmaxf(mx[e], v + ex) : mx[e];
-        }
-      }
+        for (int e = 0; e < 2; ++e)
+          if (kFull || t * 16 + 8 * r + g < valid) mx[e] = fmaxf(mx[e], y[t][2 * r + e]);
     }
-    float alpha[2];
+    // A larger V scale than any before raises E (rarely, after the first chunks).
+    const uint32_t sm = __reduce_max_sync(0xffffffffu, *reinterpret_cast<const uint32_t *>(&vmax) & 0xffffu);
+    float rise = 0.f;
+    if (sm > s_max) {
+      s_max = sm;
+      const float en = fmaxf(E, exponent_of(sm));
+      rise = en - E;
+      E = en;
+    }
+    float alpha[2], zs[2][NG];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
 #pragma unroll
       for (int x = 4; x <= 16; x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
-      const float mn = fmaxf(m[e], mx[e]);
-      alpha[e] = exp2f(m[e] - mn);
+      const float mn = fmaxf(m[e] + rise, fmaf(mx[e], f[e], E));
+      alpha[e] = ex2(m[e] - mn);
       m[e] = mn;
       l[e] *= alpha[e];
-    }
-    // Weights, and the zeros' share of the output: sum_t p_t zero_t per group.
-    float zs[2][NG];
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int n = 0; n < NG; ++n) zs[e][n] = 0.f;
-    uint32_t vp[4][2][NG];
+    }
+    // Weights, and the zeros' share of the output: sum_t p_t zero_t per group.
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const int page = (t * 16) >> lp, r0 = (t * 16) & (P - 1);
       if (!kFull && t * 16 >= valid) continue;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        lds_pairs<NG>(swz(st + page * slab + half + P * 64 + (r0 + g + 8 * r) * (4 * NG)), vp[t][r]);
-        const bool in = kFull || t * 16 + 8 * r + g < valid;
-#pragma unroll
-        for (int n = 0; n < NG; ++n)
-          if (!in) vp[t][r][n] = 0u;  // anything may lie behind the last token
+      for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float w = exp2f(y[t][2 * r + e] - m[e]);
+          float w = ex2(fmaf(y[t][2 * r + e], f[e], -m[e]));
+          if (!kFull && t * 16 + 8 * r + g >= valid) w = 0.f;
           y[t][2 * r + e] = w;
           l[e] += w;
 #pragma unroll
           for (int n = 0; n < NG; ++n) zs[e][n] = fmaf(w, half2_of(vp[t][r][n]).y, zs[e][n]);
         }
-      }
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e)
@@ -448,16 +445,20 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
     // O rows: even dims count codes * 2^-24, odd dims * 2^-20.  Adding the zeros'
     // share chunk by chunk keeps O centred, so nothing cancels at the end.
 #pragma unroll
-    for (int t = 0; t < 8; ++t)
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        o[t][e] = fmaf(o[t][e], alpha[e & 1], zs[e & 1][(t >> 1) * NG / 4] * (e < 2 ? 0x1p-24f : 0x1p-20f));
+      for (int n = 0; n < NG; ++n) {
+        const float even = zs[e][n] * 0x1p-24f, odd = zs[e][n] * 0x1p-20f;
+#pragma unroll
+        for (int t = 8 * n / NG; t < 8 * (n + 1) / NG; ++t) {
+          o[t][e] = fmaf(o[t][e], alpha[e], even);
+          o[t][2 + e] = fmaf(o[t][2 + e], alpha[e], odd);
+        }
+      }
     // O^T += V^T P^T
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const int page = (t * 16) >> lp, r0 = (t * 16) & (P - 1);
       if (!kFull && t * 16 >= valid) continue;
-      const uint32_t vb = st + page * slab + half + r0 * 64;
       uint32_t bf[NG][2];
       [[maybe_unused]] uint32_t bl[NG][2];
 #pragma unroll
@@ -474,29 +475,38 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
           }
         }
       uint32_t x[2][4];  // token pairs (2 cq, +1) and (2 cq + 8, +9): 4 pieces of 4 dims
-      const uint32_t row0 = vb + (2 * cq + flip) * 64, row1 = vb + (2 * cq + 1 - flip) * 64;
+      const uint32_t row0 = 2 * cq + flip, row1 = 2 * cq + 1 - flip;
+      const uint32_t vc = rows_at(t) + half;
+      if constexpr (NG == 1) {
+        const uint8_t *a = st + swz(vc, row0, 8 * g), *c = st + swz(vc, row1, 8 * g);
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        if constexpr (NG == 1) {
-          const uint2 u = lds64(swz(row0 + 8 * g) + 512 * r), v = lds64(swz(row1 + 8 * g) + 512 * r);
+        for (int r = 0; r < 2; ++r) {
+          const uint2 u = *reinterpret_cast<const uint2 *>(a + 512 * r), v = *reinterpret_cast<const uint2 *>(c + 512 * r);
           x[r][0] = __byte_perm(u.x, v.x, sel_lo);
           x[r][1] = __byte_perm(u.x, v.x, sel_hi);
           x[r][2] = __byte_perm(u.y, v.y, sel_lo);
           x[r][3] = __byte_perm(u.y, v.y, sel_hi);
-        } else if constexpr (NG == 2) {
+        }
+      } else if constexpr (NG == 2) {
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const uint32_t u = lds32(swz(row0 + 32 * n + 4 * g) + 512 * r), v = lds32(swz(row1 + 32 * n + 4 * g) + 512 * r);
+        for (int n = 0; n < 2; ++n) {
+          const uint8_t *a = st + swz(vc, row0, 32 * n + 4 * g), *c = st + swz(vc, row1, 32 * n + 4 * g);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t u = *reinterpret_cast<const uint32_t *>(a + 512 * r);
+            const uint32_t v = *reinterpret_cast<const uint32_t *>(c + 512 * r);
             x[r][2 * n] = __byte_perm(u, v, sel_lo);
             x[r][2 * n + 1] = __byte_perm(u, v, sel_hi);
           }
-        } else {
+        }
+      } else {
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const uint32_t u = lds32(swz(row0 + 16 * n + 4 * (g >> 1)) + 512 * r);
-            const uint32_t v = lds32(swz(row1 + 16 * n + 4 * (g >> 1)) + 512 * r);
-            x[r][n] = __byte_perm(u, v, sel_g);
-          }
+        for (int n = 0; n < 4; ++n) {
+          const uint8_t *a = st + swz(vc, row0, 16 * n + 4 * (g >> 1)), *c = st + swz(vc, row1, 16 * n + 4 * (g >> 1));
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            x[r][n] = __byte_perm(*reinterpret_cast<const uint32_t *>(a + 512 * r),
+                                  *reinterpret_cast<const uint32_t *>(c + 512 * r), sel_g);
         }
       }
 #pragma unroll
@@ -530,7 +540,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
       __syncwarp();
       break;
     }
-    const uint32_t st = ring + s * S::stage;
+    const uint8_t *st = smem + (warp * kQ4Stages + s) * S::stage;
     const int valid = min(kQ4Chunk, t1 - (t0 + (warp + j * kQ4Warps) * kQ4Chunk));
     if (valid == kQ4Chunk)
       chunk(st, valid, std::true_type{});
@@ -571,7 +581,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2) attn_q4_kernel(const __grid_con
     float den = 0.f, acc = 0.f;
 #pragma unroll
     for (int w = 0; w < kQ4Warps; ++w) {
-      const float c = exp2f(sm_m[w * kQ4Heads + h] - gm);
+      const float c = ex2(sm_m[w * kQ4Heads + h] - gm);
       den = fmaf(sm_l[w * kQ4Heads + h], c, den);
       acc = fmaf(reinterpret_cast<const float *>(smem + w * kQ4Stages * S::stage)[h * kKv4Dim + d], c, acc);
     }
@@ -619,9 +629,9 @@ __global__ void __launch_bounds__(kQ4Threads) attn_q4_merge_kernel(const __grid_
   merge_q4<T>(p, b, kvh * p.group + hb * p.block_heads, min(p.block_heads, p.group - hb * p.block_heads), splits, sm);
 }
 
-template <typename T, int NG>
+template <typename T, int NG, int P>
 cudaError_t launch_attn(const AttnQ4Params &p, long long grid, cudaStream_t s) {
-  auto kern = attn_q4_kernel<T, NG>;
+  auto kern = attn_q4_kernel<T, NG, P>;
   cudaError_t e = prepare_kernel_attributes(reinterpret_cast<const void *>(kern));
   if (e != cudaSuccess) return e;
   e = launch_ex(kern, dim3((unsigned)grid), dim3(kQ4Threads), Q4Smem<NG>::bytes, s, 1, p.pdl != 0, p);
@@ -629,12 +639,21 @@ cudaError_t launch_attn(const AttnQ4Params &p, long long grid, cudaStream_t s) {
   return launch_ex(attn_q4_merge_kernel<T>, dim3((unsigned)(grid / p.num_splits)), dim3(kQ4Threads), 0, s, 1, p.pdl != 0, p);
 }
 
+template <typename T, int NG>
+cudaError_t launch_attn_g(const AttnQ4Params &p, long long grid, cudaStream_t s) {
+  switch (p.c.page_size) {
+    case 16: return launch_attn<T, NG, 16>(p, grid, s);
+    case 32: return launch_attn<T, NG, 32>(p, grid, s);
+    default: return launch_attn<T, NG, 64>(p, grid, s);
+  }
+}
+
 template <typename T>
 cudaError_t launch_attn_t(const AttnQ4Params &p, long long grid, cudaStream_t s) {
   switch (p.c.ng) {
-    case 1: return launch_attn<T, 1>(p, grid, s);
-    case 2: return launch_attn<T, 2>(p, grid, s);
-    default: return launch_attn<T, 4>(p, grid, s);
+    case 1: return launch_attn_g<T, 1>(p, grid, s);
+    case 2: return launch_attn_g<T, 2>(p, grid, s);
+    default: return launch_attn_g<T, 4>(p, grid, s);
   }
 }
 

@@ -17,6 +17,20 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def stream_of(device: int) -> int:
+    """The current stream's handle on the current device, without building a
+    ``torch.cuda.Stream`` (3 us of a call's host time)."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def current_device_of(t: torch.Tensor, name: str) -> int:
+    """The index of t's device, which must be the current CUDA device."""
+    device = t.get_device()
+    if device < 0 or device != torch.cuda.current_device():
+        raise RuntimeError(f"{name} must be on the current CUDA device")
+    return device
+
+
 def _check16(*ts):
     for t in ts:
         if t.dtype not in (torch.float16, torch.bfloat16) or not t.is_cuda:
@@ -136,11 +150,12 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
     copied.  FP32 arithmetic, one rounding, angles exact at any position.  Token
     and head strides are free (multiples of 8), so x may be the q and k heads of
     a fused projection; ``out`` may be x itself, else must not overlap it."""
+    device = current_device_of(x, "x")
     _check16(x)
     if x.dim() != 3:
         raise RuntimeError("x must be [tokens, heads, head_dim]")
     T, H, D = x.shape
-    _check_rope(positions, inv_freq, T, D)
+    _check_rope(positions, inv_freq, T, D, device)
     if out is None:
         out = torch.empty(T, H, D, dtype=x.dtype, device=x.device)
     elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or (D > 1 and out.stride(2) != 1):
@@ -152,14 +167,14 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
         check(LIB.dak_rotary(x.data_ptr(), xt if T > 1 else 0, xh if H > 1 else 0, positions.data_ptr(),
                              inv_freq.data_ptr(), float(rope_scale), int(interleaved), out.data_ptr(),
                              ot if T > 1 else 0, oh if H > 1 else 0, T, H, D, 2 * inv_freq.numel(),
-                             dak_dtype(x.dtype), _stream()), "rotary")
+                             dak_dtype(x.dtype), stream_of(device)), "rotary")
     return out
 
 
-def _check_rope(positions: torch.Tensor, inv_freq: torch.Tensor | None, tokens: int, head_dim: int) -> None:
-    if positions.dtype != torch.int32 or not positions.is_cuda or positions.numel() != tokens \
+def _check_rope(positions: torch.Tensor, inv_freq: torch.Tensor | None, tokens: int, head_dim: int, device: int) -> None:
+    if positions.dtype != torch.int32 or positions.get_device() != device or positions.numel() != tokens \
             or not positions.is_contiguous():
         raise RuntimeError("positions must be a contiguous int32 CUDA tensor with one entry per token")
-    if inv_freq is not None and (inv_freq.dtype != torch.float32 or not inv_freq.is_cuda
+    if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.get_device() != device
                                  or not inv_freq.is_contiguous() or 2 * inv_freq.numel() > head_dim):
         raise RuntimeError("inv_freq must be a contiguous float32 CUDA tensor of at most head_dim / 2 entries")

@@ -27,8 +27,8 @@ import torch
 
 from . import _lib
 from ._lib import LIB, check
-from .attention import HEAD_DIM, _stream_ptr, auto_split_size
-from .decode_ops import _check_rope
+from .attention import HEAD_DIM
+from .decode_ops import _check_rope, current_device_of, stream_of
 from .runtime import dak_dtype
 from .trace import traced
 
@@ -49,59 +49,62 @@ _FORMATS = {page_bytes(p, g): (p, g) for p in PAGE_SIZES for g in GROUPS}
 
 def page_format(pool: torch.Tensor) -> tuple[int, int]:
     """(page_size, group) of a pool [pages, kv_heads, page_bytes]."""
-    fmt = _FORMATS.get(pool.shape[-1])
-    if fmt is None:
+    if pool.shape[-1] not in _FORMATS:
         raise RuntimeError(f"{pool.shape[-1]} bytes per (page, head) is no page_bytes(page_size, group)")
-    return fmt
+    return _FORMATS[pool.shape[-1]]
 
 
-def _cache(device: torch.device, pool_dev, pool_host, block_table: torch.Tensor) -> _lib.Kv4Cache:
+def _cache(device: int, pool_dev, pool_host, block_table: torch.Tensor) -> _lib.Kv4Cache:
     """The checked pools and table as the C ABI takes them."""
-    pool = pool_dev if pool_dev is not None else pool_host
-    if pool is None:
-        raise RuntimeError("no KV pool given")
-    for t, nm in ((pool_dev, "pool_dev"), (pool_host, "pool_host")):
-        if t is None:
-            continue
-        if t.dtype != torch.uint8 or t.dim() != 3 or not t.is_contiguous():
-            raise RuntimeError(f"{nm} must be a contiguous uint8 [pages, kv_heads, page_bytes] tensor")
-        if t.shape[1:] != pool.shape[1:]:
-            raise RuntimeError("the pools must share kv_heads and page_bytes")
-    if pool_dev is not None and pool_dev.device != device:
-        raise RuntimeError("pool_dev is on the wrong device")
-    if pool_host is not None and (pool_host.is_cuda or not pool_host.is_pinned()):
-        raise RuntimeError("pool_host must be pinned host memory")
-    if block_table.dtype != torch.int32 or block_table.device != device or block_table.dim() != 2 \
-            or (block_table.size(1) > 1 and block_table.stride(1) != 1):
-        raise RuntimeError("block_table must be an int32 CUDA tensor [B, max_pages]")
     c = _lib.Kv4Cache()
-    c.page_size, c.group = page_format(pool)
-    c.kv_heads = pool.shape[1]
-    if pool_dev is not None and pool_dev.shape[0]:
-        c.pool_dev, c.dev_pages = pool_dev.data_ptr(), pool_dev.shape[0]
-    if pool_host is not None and pool_host.shape[0]:
-        c.pool_host, c.host_pages = pool_host.data_ptr(), pool_host.shape[0]
-    c.batch, c.max_pages = block_table.shape
-    c.block_table = block_table.data_ptr()
-    c.table_stride = block_table.stride(0) if c.batch > 1 else c.max_pages
+    shape = None
+    if pool_dev is not None:
+        if pool_dev.get_device() != device:
+            raise RuntimeError("pool_dev is on the wrong device")
+        shape = _pool_shape(pool_dev, "pool_dev")
+        if shape[0]:
+            c.pool_dev, c.dev_pages = pool_dev.data_ptr(), shape[0]
+    if pool_host is not None:
+        if pool_host.is_cuda or not pool_host.is_pinned():
+            raise RuntimeError("pool_host must be pinned host memory")
+        host = _pool_shape(pool_host, "pool_host")
+        if shape is not None and host[1:] != shape[1:]:
+            raise RuntimeError("the pools must share kv_heads and page_bytes")
+        shape = host
+        if shape[0]:
+            c.pool_host, c.host_pages = pool_host.data_ptr(), shape[0]
+    if shape is None:
+        raise RuntimeError("no KV pool given")
+    if block_table.dtype != torch.int32 or block_table.get_device() != device or block_table.dim() != 2:
+        raise RuntimeError("block_table must be an int32 CUDA tensor [B, max_pages]")
+    (rows, pages), (row_stride, stride) = block_table.shape, block_table.stride()
+    if pages > 1 and stride != 1:
+        raise RuntimeError("block_table must have contiguous rows")
+    fmt = _FORMATS.get(shape[2])
+    if fmt is None:
+        raise RuntimeError(f"{shape[2]} bytes per (page, head) is no page_bytes(page_size, group)")
+    c.page_size, c.group = fmt
+    c.kv_heads, c.batch, c.max_pages = shape[1], rows, pages
+    c.block_table, c.table_stride = block_table.data_ptr(), row_stride if rows > 1 else pages
     return c
 
 
-def _on_current(device: torch.device) -> None:
-    if device.type != "cuda" or device.index != torch.cuda.current_device():
-        raise RuntimeError(f"tensors must be on the current CUDA device, got {device}")
+def _pool_shape(t: torch.Tensor, name: str):
+    if t.dtype != torch.uint8 or t.dim() != 3 or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous uint8 [pages, kv_heads, page_bytes] tensor")
+    return t.shape
 
 
-def _check_tokens(positions: torch.Tensor, seq_index: torch.Tensor | None, device, batch: int) -> int:
-    if positions.dtype != torch.int32 or positions.device != device or positions.dim() != 1 \
+def _check_tokens(positions: torch.Tensor, seq_index: torch.Tensor | None, device: int, batch: int) -> int:
+    if positions.dtype != torch.int32 or positions.get_device() != device or positions.dim() != 1 \
             or not positions.is_contiguous():
         raise RuntimeError("positions must be a contiguous int32 CUDA tensor [tokens]")
     T = positions.numel()
     if seq_index is None:
         if T != batch:
             raise RuntimeError("without seq_index there is one token per sequence of the block table")
-    elif seq_index.dtype != torch.int32 or seq_index.device != device or seq_index.shape != positions.shape \
-            or not seq_index.is_contiguous():
+    elif seq_index.dtype != torch.int32 or seq_index.get_device() != device or seq_index.dim() != 1 \
+            or seq_index.numel() != T or not seq_index.is_contiguous():
         raise RuntimeError("seq_index must be a contiguous int32 CUDA tensor [tokens]")
     return T
 
@@ -122,16 +125,15 @@ def rope_kv_append_q4(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torc
     rotates nothing.  Two tokens of one call must not share a sequence and
     position.  A NaN is stored as code 0 and values beyond float16 saturate: the
     cache holds finite numbers only."""
-    device = qkv.device
-    _on_current(device)
+    device = current_device_of(qkv, "qkv")
     if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("qkv must be a 16-bit [tokens, (q_heads + 2 kv_heads) * 128] tensor, last dim contiguous")
     c = _cache(device, pool_dev, pool_host, block_table)
     T = _check_tokens(positions, seq_index, device, c.batch)
-    _check_rope(positions, inv_freq, T, HEAD_DIM)
+    _check_rope(positions, inv_freq, T, HEAD_DIM, device)
     if qkv.shape[0] != T or qkv.shape[1] != (q_heads + 2 * c.kv_heads) * HEAD_DIM:
         raise RuntimeError(f"qkv must be [{T}, {(q_heads + 2 * c.kv_heads) * HEAD_DIM}]")
-    if q_heads and (q_out is None or not q_out.is_contiguous() or q_out.dtype != qkv.dtype or q_out.device != device
+    if q_heads and (q_out is None or not q_out.is_contiguous() or q_out.dtype != qkv.dtype or q_out.get_device() != device
                     or q_out.numel() != T * q_heads * HEAD_DIM):
         raise RuntimeError("q_out must be a contiguous [tokens, q_heads, 128] tensor of the qkv dtype")
     if T == 0:
@@ -144,7 +146,7 @@ def rope_kv_append_q4(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torc
     a.rope_scale, a.interleaved = rope_scale, int(interleaved)
     a.q_out = q_out.data_ptr() if q_heads else None
     a.tokens, a.q_heads, a.dtype = T, q_heads, dak_dtype(qkv.dtype)
-    check(LIB.dak_rope_kv_append_q4(ctypes.byref(c), ctypes.byref(a), _stream_ptr()), "rope_kv_append_q4")
+    check(LIB.dak_rope_kv_append_q4(ctypes.byref(c), ctypes.byref(a), stream_of(device)), "rope_kv_append_q4")
 
 
 @traced
@@ -154,25 +156,33 @@ def kv_read_q4(pool_dev: torch.Tensor | None, pool_host: torch.Tensor | None, bl
     """(k, v) [tokens, kv_heads, 128] that the cache holds for the given tokens, in
     16 bits: what attention over the cache sees, for a prompt whose prefix is
     already cached."""
-    device = block_table.device
-    _on_current(device)
+    device = current_device_of(block_table, "block_table")
     if dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("dtype must be float16 or bfloat16")
     c = _cache(device, pool_dev, pool_host, block_table)
     T = _check_tokens(positions, seq_index, device, c.batch)
     shape = (T, c.kv_heads, HEAD_DIM)
-    outs = []
     for t, nm in ((k_out, "k_out"), (v_out, "v_out")):
-        if t is None:
-            t = torch.empty(shape, dtype=dtype, device=device)
-        elif t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
+        if t is not None and (t.shape != shape or t.dtype != dtype or t.get_device() != device or not t.is_contiguous()):
             raise RuntimeError(f"{nm} must be a contiguous [tokens, kv_heads, 128] tensor of dtype")
-        outs.append(t)
+    if k_out is None and v_out is None:  # one allocation for both
+        k_out, v_out = torch.empty((2, *shape), dtype=dtype, device=block_table.device)
+    elif k_out is None:
+        k_out = torch.empty_like(v_out)
+    elif v_out is None:
+        v_out = torch.empty_like(k_out)
     if T:
         check(LIB.dak_kv_read_q4(ctypes.byref(c), positions.data_ptr(),
-                                 seq_index.data_ptr() if seq_index is not None else None, outs[0].data_ptr(),
-                                 outs[1].data_ptr(), T, dak_dtype(dtype), _stream_ptr()), "kv_read_q4")
-    return outs[0], outs[1]
+                                 seq_index.data_ptr() if seq_index is not None else None, k_out.data_ptr(),
+                                 v_out.data_ptr(), T, dak_dtype(dtype), stream_of(device)), "kv_read_q4")
+    return k_out, v_out
+
+
+def auto_split_size_q4(rows: int, max_seq_len: int) -> int:
+    """Tokens per split (a multiple of 64) for ``rows`` = sequences x KV heads x head
+    blocks."""
+    splits = max(1, min(444 // rows if rows <= 444 else 2000 // rows, max_seq_len // 256))
+    return -(-max_seq_len // (splits * 64)) * 64
 
 
 def merge_counter_count(batch: int, q_heads: int, kv_heads: int) -> int:
@@ -197,55 +207,63 @@ def decode_paged_q4(query: torch.Tensor, pool_dev: torch.Tensor | None, pool_hos
     every call) the last split merges the splits inside the attention kernel
     instead of a second launch; the result is the same.  Calls that may overlap
     on the GPU need scratch and counters of their own."""
-    device = query.device
-    _on_current(device)
-    if query.dim() != 3 or query.size(2) != HEAD_DIM or query.stride(2) != 1:
+    device = current_device_of(query, "query")
+    dtype = query.dtype
+    if query.dim() != 3 or query.shape[2] != HEAD_DIM or query.stride(2) != 1:
         raise RuntimeError("query must be [B, Hq, 128] with a contiguous last dimension")
-    if query.dtype not in (torch.float16, torch.bfloat16):
+    if dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("query must be float16 or bfloat16")
     c = _cache(device, pool_dev, pool_host, block_table)
-    B, Hq = query.size(0), query.size(1)
-    if block_table.size(0) != B:
+    B, Hq, _ = query.shape
+    if c.batch != B:
         raise RuntimeError("block_table must have one row per sequence")
-    if seq_lens.dtype != torch.int32 or seq_lens.device != device or seq_lens.numel() != B \
+    if seq_lens.dtype != torch.int32 or seq_lens.get_device() != device or seq_lens.numel() != B \
             or not seq_lens.is_contiguous():
         raise RuntimeError("seq_lens must be a contiguous int32 CUDA tensor [B]")
-    if Hq % c.kv_heads:
+    kv_heads = c.kv_heads
+    if Hq % kv_heads:
         raise RuntimeError("the KV heads must divide the query heads")
     if max_seq_len is None:
         max_seq_len = c.max_pages * c.page_size
-    blocks = -(-(Hq // c.kv_heads) // MAX_BLOCK_HEADS)
+    blocks = -(-(Hq // kv_heads) // MAX_BLOCK_HEADS)
     if split_size is None:
-        split_size = auto_split_size(B * blocks, c.kv_heads, max_seq_len)
+        split_size = auto_split_size_q4(B * kv_heads * blocks, max_seq_len)
     if split_size <= 0:
         raise RuntimeError("split_size must be positive")
     splits = -(-max_seq_len // split_size)
     if out is None:
-        out = torch.empty((B, Hq, HEAD_DIM), dtype=query.dtype, device=device)
-    elif out.shape != query.shape or out.dtype != query.dtype or out.device != device or out.stride(2) != 1:
+        out = torch.empty((B, Hq, HEAD_DIM), dtype=dtype, device=query.device)
+    elif out.shape != query.shape or out.dtype != dtype or out.get_device() != device or out.stride(2) != 1:
         raise RuntimeError("out must be [B, Hq, 128] of the query dtype with a contiguous last dimension")
     a = _lib.AttnQ4Args()
     if splits > 1:
-        for t, n, nm in ((partial_o, HEAD_DIM, "partial_o"), (partial_ml, 2, "partial_ml")):
-            if t is not None and (t.dtype != torch.float32 or t.device != device or not t.is_contiguous()
-                                  or t.numel() < B * Hq * splits * n):
-                raise RuntimeError(f"{nm} must be a contiguous float32 CUDA tensor of B * Hq * {splits} * {n} entries")
-        if partial_o is None:
-            partial_o = torch.empty(B * Hq * splits * HEAD_DIM, dtype=torch.float32, device=device)
-        if partial_ml is None:
-            partial_ml = torch.empty(B * Hq * splits * 2, dtype=torch.float32, device=device)
-        a.partial_o, a.partial_ml = partial_o.data_ptr(), partial_ml.data_ptr()
+        n = B * Hq * splits
+        for t, per, nm in ((partial_o, HEAD_DIM, "partial_o"), (partial_ml, 2, "partial_ml")):
+            if t is not None and (t.dtype != torch.float32 or t.get_device() != device or not t.is_contiguous()
+                                  or t.numel() < n * per):
+                raise RuntimeError(f"{nm} must be a contiguous float32 CUDA tensor of B * Hq * {splits} * {per} entries")
+        if partial_o is None and partial_ml is None:  # one allocation for both
+            partial_o = torch.empty(n * (HEAD_DIM + 2), dtype=torch.float32, device=query.device)
+            a.partial_o = partial_o.data_ptr()
+            a.partial_ml = a.partial_o + 4 * n * HEAD_DIM
+        else:
+            if partial_o is None:
+                partial_o = torch.empty(n * HEAD_DIM, dtype=torch.float32, device=query.device)
+            if partial_ml is None:
+                partial_ml = torch.empty(n * 2, dtype=torch.float32, device=query.device)
+            a.partial_o, a.partial_ml = partial_o.data_ptr(), partial_ml.data_ptr()
         if merge_counters is not None:
-            if merge_counters.dtype != torch.int32 or merge_counters.device != device \
-                    or merge_counters.numel() < B * c.kv_heads * blocks or not merge_counters.is_contiguous():
+            if merge_counters.dtype != torch.int32 or merge_counters.get_device() != device \
+                    or merge_counters.numel() < B * kv_heads * blocks or not merge_counters.is_contiguous():
                 raise RuntimeError("merge_counters must be a contiguous int32 CUDA tensor of merge_counter_count entries")
             a.merge_counters = merge_counters.data_ptr()
-    a.query = query.data_ptr()
-    a.q_stride_b, a.q_stride_h = query.stride(0) if B > 1 else 0, query.stride(1) if Hq > 1 else 0
-    a.seq_lens = seq_lens.data_ptr()
-    a.out = out.data_ptr()
-    a.o_stride_b, a.o_stride_h = out.stride(0) if B > 1 else 0, out.stride(1) if Hq > 1 else 0
+    a.query, a.seq_lens, a.out = query.data_ptr(), seq_lens.data_ptr(), out.data_ptr()
+    # A dimension of one entry has no stride to speak of.
+    qb, qh, _ = query.stride()
+    ob, oh, _ = out.stride()
+    a.q_stride_b, a.q_stride_h = qb if B > 1 else 0, qh if Hq > 1 else 0
+    a.o_stride_b, a.o_stride_h = ob if B > 1 else 0, oh if Hq > 1 else 0
     a.num_q_heads, a.max_seq_len, a.split_size = Hq, max_seq_len, split_size
-    a.scaling, a.dtype = scaling, dak_dtype(query.dtype)
-    check(LIB.dak_attn_decode_paged_q4(ctypes.byref(c), ctypes.byref(a), _stream_ptr()), "decode_paged_q4")
+    a.scaling, a.dtype = scaling, dak_dtype(dtype)
+    check(LIB.dak_attn_decode_paged_q4(ctypes.byref(c), ctypes.byref(a), stream_of(device)), "decode_paged_q4")
     return out

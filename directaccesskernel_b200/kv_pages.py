@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from ._lib import LIB, check
-from .attention import _stream_ptr
+from .decode_ops import current_device_of, stream_of
 from .trace import traced
 
 MAX_MOVES = 3584  # pages per launch
@@ -45,8 +45,7 @@ def copy_pages(pool_dev: torch.Tensor | None, pool_host: torch.Tensor | None, sr
         raise RuntimeError("no KV pool given")
     if not 0 <= page_dim < pool.dim():
         raise RuntimeError("page_dim is outside the pool's dimensions")
-    if pool_dev is not None and (not pool_dev.is_cuda or pool_dev.device.index != torch.cuda.current_device()):
-        raise RuntimeError("pool_dev must be on the current CUDA device")
+    device = current_device_of(pool_dev, "pool_dev") if pool_dev is not None else torch.cuda.current_device()
     if pool_host is not None and (pool_host.is_cuda or not pool_host.is_pinned()):
         raise RuntimeError("pool_host must be pinned host memory")
     for t in (pool_dev, pool_host):
@@ -80,7 +79,7 @@ def copy_pages(pool_dev: torch.Tensor | None, pool_host: torch.Tensor | None, sr
     for i in range(0, n, MAX_MOVES):
         s, d = src[i:i + MAX_MOVES], dst[i:i + MAX_MOVES]
         check(LIB.dak_copy_pages(pool_dev.data_ptr() if nd else None, nd, pool_host.data_ptr() if nh else None, nh, page,
-                                 slabs, nd * page, nh * page, s.data_ptr(), d.data_ptr(), s.numel(), _stream_ptr()),
+                                 slabs, nd * page, nh * page, s.data_ptr(), d.data_ptr(), s.numel(), stream_of(device)),
               "copy_pages")
 
 
