@@ -125,8 +125,8 @@ class Kv4AppendArgs(ctypes.Structure):
 class AttnQ4Args(ctypes.Structure):
     _fields_ = [
         ("query", c_vp), ("q_stride_b", c_i64), ("q_stride_h", c_i64), ("seq_lens", c_vp),
-        ("out", c_vp), ("o_stride_b", c_i64), ("o_stride_h", c_i64), ("partial_o", c_vp), ("partial_ml", c_vp),
-        ("merge_counters", c_vp), ("num_q_heads", c_int), ("max_seq_len", c_int), ("split_size", c_int),
+        ("out", c_vp), ("o_stride_b", c_i64), ("o_stride_h", c_i64), ("scratch", c_vp), ("scratch_floats", c_i64),
+        ("merge_counters", c_vp), ("num_q_heads", c_int), ("max_seq_len", c_int),
         ("scaling", ctypes.c_float), ("dtype", c_int),
     ]
 
@@ -167,6 +167,7 @@ SIGNATURES = {
     "dak_rope_kv_append_q4": (c_int, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4AppendArgs), c_vp]),
     "dak_kv_read_q4": (c_int, [ctypes.POINTER(Kv4Cache), c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_vp]),
     "dak_attn_decode_paged_q4": (c_int, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(AttnQ4Args), c_vp]),
+    "dak_attn_q4_scratch": (c_i64, [ctypes.POINTER(Kv4Cache), c_int, c_int]),
     "dak_copy_pages": (c_int, [c_vp, c_i64, c_vp, c_i64, c_i64, c_int, c_i64, c_i64, c_vp, c_vp, c_int, c_vp]),
     "dak_device_status": (c_int, [c_int, ctypes.POINTER(c_int)]),
     "dak_selftest_wait_timeout": (c_int, [ctypes.c_uint, c_vp]),

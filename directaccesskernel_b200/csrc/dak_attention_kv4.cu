@@ -2,10 +2,14 @@
 // (dak_kv4.cuh), whose pages lie in HBM or in pinned host memory.
 //
 // One query token per sequence: o = softmax(scaling q K^T) V over the first
-// seq_lens[b] tokens, K and V being scale * code + zero.  One CTA per
-// (sequence, KV head, block of up to 8 query heads, split of the tokens); the
-// splits' (o, m, l) are merged with log-sum-exp.  Scores are kept in base 2.
-// A sequence of no tokens gives zeros.
+// seq_lens[b] tokens, K and V being scale * code + zero.  A row is one
+// (sequence, KV head, block of up to 8 query heads); its tokens are cut into
+// chunks of 64.  The chunks of all rows, laid end to end, are dealt out in equal
+// contiguous ranges, one to each CTA that the GPU holds at once, whatever the
+// lengths: a CTA walks over its range row by row, its four warps taking every
+// fourth chunk, with copies running ahead across rows.  A row that spans CTAs is
+// merged by log-sum-exp.  Scores are kept in base 2; a sequence of no tokens
+// gives zeros.
 #include <cudaTypedefs.h>
 
 #include <cfloat>
@@ -19,11 +23,12 @@
 namespace dak {
 namespace {
 
-constexpr int kQ4Warps = 4;
-constexpr int kQ4Threads = kQ4Warps * 32;
 constexpr int kQ4Heads = 8;    // query heads per CTA: the MMA's N
 constexpr int kQ4Chunk = 64;   // tokens a warp takes at a time
 constexpr int kQ4Stages = 2;   // chunks in flight per warp
+constexpr int kQ4PerSm = 2;    // CTAs per SM
+constexpr int kQ4MergeWarps = 4;
+constexpr int kQ4RowChunks = 8;  // rows up to this long are not split while the GPU holds them all
 
 struct alignas(64) AttnQ4Params {
   CUtensorMap map[2];  // device, host pool: dims {64 bytes, slab rows, pages x heads}
@@ -33,26 +38,31 @@ struct alignas(64) AttnQ4Params {
   uint16_t *out;
   long long o_stride_b, o_stride_h;
   const int32_t *seq_lens;
-  float *partial_o, *partial_ml;
-  int32_t *counters;
+  float *scratch;     // 2 slots per CTA of [heads][128] outputs, then of [heads][2] (m, l)
+  int32_t *counters;  // [rows]: the CTA that finishes a split row last merges it (nullptr: merge kernel)
   int num_q_heads, group, block_heads, head_blocks;  // group: query heads per KV head
-  int max_seq_len, split_size, num_splits;
+  int max_seq_len;
+  int ctas, warps, by_row;  // by_row: CTA i takes row i, and no row is split
   float scale_log2;                                  // scaling * log2(e)
   int pdl;
 };
 
-// Shared memory of a CTA: per warp a ring of chunks, then barriers and the
-// warps' softmax statistics.  After the last chunk a warp's ring holds its
-// partial outputs.
+// Shared memory of a CTA: per warp a ring of chunks; the warps' statistics and
+// one block of outputs that they add up in turn; barriers.  Two CTAs share an SM,
+// and have as many warps as their rings leave room for.
 template <int NG>
 struct Q4Smem {
+  static constexpr int warps = NG == 4 ? 5 : 6;
+  static constexpr int threads = 32 * warps;
   static constexpr uint32_t stage = 2 * kQ4Chunk * (64 + 4 * NG);
-  static constexpr uint32_t bar_off = kQ4Warps * kQ4Stages * stage;
-  static constexpr uint32_t m_off = bar_off + kQ4Warps * kQ4Stages * 8;  // [warps][heads]
-  static constexpr uint32_t l_off = m_off + kQ4Warps * kQ4Heads * 4;
-  static constexpr uint32_t flag_off = l_off + kQ4Warps * kQ4Heads * 4;
-  static constexpr uint32_t bytes = flag_off + 16 + 512;  // 512: alignment
-  static_assert(stage % 512 == 0 && kQ4Stages * stage >= kQ4Heads * kKv4Dim * 4, "a ring must hold a partial output");
+  static constexpr uint32_t o_off = warps * kQ4Stages * stage;            // [heads][128]
+  static constexpr uint32_t m_off = o_off + kQ4Heads * kKv4Dim * 4;       // [warps][heads]
+  static constexpr uint32_t l_off = m_off + warps * kQ4Heads * 4;
+  static constexpr uint32_t bar_off = l_off + warps * kQ4Heads * 4;
+  static constexpr uint32_t flag_off = bar_off + warps * kQ4Stages * 8;   // abort, abort of the drain, last
+  static constexpr uint32_t bytes = flag_off + 16 + 496;                  // 496: alignment to 512
+  static_assert(stage % 512 == 0, "the swizzle is computed from the offset in a stage");
+  static_assert(kQ4PerSm * (bytes + 1024) <= 228 * 1024, "CTAs per SM");
 };
 
 __device__ __forceinline__ void tma_load_slab(uint32_t dst, const CUtensorMap *map, int slab, uint32_t bar,
@@ -122,109 +132,172 @@ __device__ __forceinline__ float exponent_of(uint32_t bits) {
   return fmaxf((float)((int)(__float_as_uint(s) >> 23) - 127), -24.f);
 }
 
-// Splits that hold tokens of a sequence (at least one, which writes the zeros of
-// an empty sequence).
-__device__ __forceinline__ int live_splits(const AttnQ4Params &p, int seq) {
-  return max(1, (seq + p.split_size - 1) / p.split_size);
+// Dims 4 lane .. + 3 of a head's output; zeros where no weight was summed.
+template <typename T>
+__device__ __forceinline__ void store_out(const AttnQ4Params &p, int b, int h, int lane, float4 v, float den) {
+  const float r = den == 0.f ? 0.f : 1.f / den;
+  *reinterpret_cast<uint2 *>(p.out + b * p.o_stride_b + h * p.o_stride_h + 4 * lane) =
+      make_uint2(Elem<T>::pack2(v.x * r, v.y * r), Elem<T>::pack2(v.z * r, v.w * r));
 }
 
-// Log-sum-exp merge of a block of heads' split partials by 128 threads, in split
-// order: first each warp forms the maximum and denominator of two heads, then
-// thread d sums dim d of every head.
+__device__ __forceinline__ int seq_of(const AttnQ4Params &p, int b) {
+  return max(0, min(p.seq_lens[b], p.max_seq_len));
+}
+__device__ __forceinline__ int chunks_of(int seq) { return (seq + kQ4Chunk - 1) / kQ4Chunk; }
+
+// Chunks of a CTA's range, given those of all rows: every CTA the same, at least
+// one for each warp.
+__device__ __forceinline__ int range_of(const AttnQ4Params &p, int total) {
+  return max((total + p.ctas - 1) / p.ctas, p.warps);
+}
+
+// Sum of the batch's chunks per (KV head, head block), by one warp.
+__device__ __forceinline__ int batch_chunks(const AttnQ4Params &p) {
+  int n = 0;
+  for (int b = lane_id(); b < p.c.rows; b += 32) n += chunks_of(seq_of(p, b));
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) n += __shfl_xor_sync(0xffffffffu, n, x);
+  return n;
+}
+
+// Where row (b, r) ended up in the scratch: its chunks are [begin, end) of all, in
+// ranges of `per`.  Piece i is CTA i's first segment (slot 2 i), or, if the row
+// begins within CTA i's range, its last (slot 2 i + 1).  One warp per head sums
+// the pieces in order, 4 dims per lane.
 template <typename T>
-__device__ __forceinline__ void merge_q4(const AttnQ4Params &p, int b, int h0, int nh, int splits, float *sm) {
-  const long long base = ((long long)b * p.num_q_heads + h0) * p.num_splits;
-  for (int h = warp_id(); h < nh; h += kQ4Warps) {
-    const float2 *ml = reinterpret_cast<const float2 *>(p.partial_ml) + base + (long long)h * p.num_splits;
-    float gm = -FLT_MAX, den = 0.f;
-    for (int s = lane_id(); s < splits; s += 32) gm = fmaxf(gm, __ldcg(ml + s).x);
+__device__ __forceinline__ void merge_row(const AttnQ4Params &p, int b, int h0, int nh, int begin, int end, int per, int warps) {
+  const int first = begin / per, pieces = (end - 1) / per - first + 1, lane = lane_id();
+  const float *po = p.scratch;
+  const float2 *pm = reinterpret_cast<const float2 *>(p.scratch + 2ll * p.ctas * kQ4Heads * kKv4Dim);
+  auto slot = [&](int i) { return 2 * (first + i) + ((first + i) * per < begin ? 1 : 0); };
+  for (int h = warp_id(); h < nh; h += warps) {
+    float2 mine = make_float2(-FLT_MAX, 0.f);
+    float gm = -FLT_MAX;
+    for (int i = lane; i < pieces; i += 32) {
+      const float2 v = __ldcg(pm + (long long)slot(i) * kQ4Heads + h);
+      if (i == lane) mine = v;
+      gm = fmaxf(gm, v.x);
+    }
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, x));
-    for (int s = lane_id(); s < splits; s += 32) {
-      const float2 v = __ldcg(ml + s);
-      den = fmaf(v.y, ex2(v.x - gm), den);
+    float den = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < pieces; i0 += 32) {
+      if (i0 > 0 && i0 + lane < pieces) mine = __ldcg(pm + (long long)slot(i0 + lane) * kQ4Heads + h);
+      const float c = i0 + lane < pieces ? ex2(mine.x - gm) : 0.f;
+      const float lc = i0 + lane < pieces ? mine.y * c : 0.f;
+      const int n = min(32, pieces - i0);
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const float ci = __shfl_sync(0xffffffffu, c, i);
+        den += __shfl_sync(0xffffffffu, lc, i);
+        const float4 v = __ldcg(reinterpret_cast<const float4 *>(po + ((long long)slot(i0 + i) * kQ4Heads + h) * kKv4Dim) + lane);
+        acc.x = fmaf(v.x, ci, acc.x);
+        acc.y = fmaf(v.y, ci, acc.y);
+        acc.z = fmaf(v.z, ci, acc.z);
+        acc.w = fmaf(v.w, ci, acc.w);
+      }
     }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) den += __shfl_xor_sync(0xffffffffu, den, x);
-    if (lane_id() == 0) {
-      sm[h] = gm;
-      sm[kQ4Heads + h] = den;
-    }
-  }
-  __syncthreads();
-  const int d = threadIdx.x;
-  for (int h = 0; h < nh; ++h) {
-    const long long at = base + (long long)h * p.num_splits;
-    const float gm = sm[h], den = sm[kQ4Heads + h];
-    float acc = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s)
-      acc = fmaf(__ldcg(p.partial_o + (at + s) * kKv4Dim + d), ex2(__ldcg(p.partial_ml + (at + s) * 2) - gm), acc);
-    p.out[b * p.o_stride_b + (h0 + h) * p.o_stride_h + d] = Elem<T>::from_float(den == 0.f ? 0.f : acc / den);
+    store_out<T>(p, b, h0 + h, lane, acc, den);
   }
 }
 
 template <typename T, int NG, int P>
-__global__ void __launch_bounds__(kQ4Threads, NG == 4 ? 2 : 3) attn_q4_kernel(const __grid_constant__ AttnQ4Params p) {
+__global__ void __launch_bounds__(Q4Smem<NG>::threads, kQ4PerSm) attn_q4_kernel(const __grid_constant__ AttnQ4Params p) {
   extern __shared__ uint8_t smem_raw[];
   using S = Q4Smem<NG>;
+  constexpr int W = S::warps;
   // The weights of a float16 output are split into two float16 terms.
   constexpr bool kTwoTerms = std::is_same<T, __half>::value;
   uint8_t *smem = smem_raw + ((512u - (smem_u32(smem_raw) & 511u)) & 511u);
   const uint32_t sbase = smem_u32(smem);
-  pdl_enter(p.pdl);
   const int warp = warp_id(), lane = lane_id();
   const int g = lane >> 2, cq = lane & 3;  // fragment row, column pair
-  int i = blockIdx.x;
-  const int split = i % p.num_splits;
-  i /= p.num_splits;
-  const int hb = i % p.head_blocks;
-  i /= p.head_blocks;
-  const int kvh = i % p.c.kv_heads;
-  const int b = i / p.c.kv_heads;
-  const int seq = max(0, min(p.seq_lens[b], p.max_seq_len));
-  const int splits = live_splits(p, seq);
-  if (split >= splits) return;
-  const int h0 = kvh * p.group + hb * p.block_heads;
-  const int nh = min(p.block_heads, p.group - hb * p.block_heads);
-  const int t0 = split * p.split_size, t1 = min(seq, t0 + p.split_size);
-  const int chunks = (t1 - t0 + kQ4Chunk - 1) / kQ4Chunk;
-  const int mine = chunks > warp ? (chunks - warp + kQ4Warps - 1) / kQ4Warps : 0;  // this warp's chunks
-  constexpr int ppc = kQ4Chunk / P;  // pages per chunk
+  constexpr int ppc = kQ4Chunk / P;        // pages per chunk
   constexpr uint32_t half = kv4_half_bytes(P, NG), slab = 2 * half;
-
-  const uint32_t ring = sbase + warp * kQ4Stages * S::stage;
   const uint32_t bar0 = sbase + S::bar_off + warp * kQ4Stages * 8;
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + S::flag_off);
   const WaitCtx wc{abort_flag, p.c.status};
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kQ4Warps * kQ4Stages; ++s) mbar_init(sbase + S::bar_off + 8 * s, 1);
+    for (int s = 0; s < W * kQ4Stages; ++s) mbar_init(sbase + S::bar_off + 8 * s, 1);
     abort_flag[0] = abort_flag[1] = 0;  // [1]: of the wait for copies in flight
     fence_mbar_init();
+    prefetch_tensormap(&p.map[0]);
+    prefetch_tensormap(&p.map[1]);
   }
+  pdl_enter(p.pdl);
   __syncthreads();
 
-  // Block-table entries: lane l holds entry l of a window of 32 / ppc chunks, and
-  // the window after it is already on its way.
-  constexpr int per_win = 32 / ppc;
-  const int32_t *row = p.c.table + (long long)b * p.c.table_stride;
-  const int last_page = (t1 - 1) / P;
-  auto window = [&](int first) {  // entries of chunks first .. of this warp
-    const int j = first + lane / ppc;
-    const int page = (t0 + (warp + j * kQ4Warps) * kQ4Chunk) / P + lane % ppc;
-    return j < mine && page <= last_page ? row[page] : 0;
-  };
-  int cur = window(0), nxt = window(per_win);
-  const uint64_t pol = l2_policy_evict_first();
-  auto issue = [&](int j) {  // chunk j of this warp into its stage
-    if (j % per_win == 0 && j > 0) {
-      cur = nxt;
-      nxt = window(j + per_win);
+  // This CTA's range of chunks [lo, hi) and the row (b0, r0) that it begins in,
+  // whose chunks begin at `begin`.
+  const int R = p.c.kv_heads * p.head_blocks;
+  int lo, hi, begin, b0, r0, per = 0;
+  if (p.by_row) {
+    b0 = blockIdx.x / R;
+    r0 = blockIdx.x - b0 * R;
+    lo = begin = 0;
+    hi = chunks_of(seq_of(p, b0));
+    if (hi == 0) {  // threads 0..nh-1 x 32 lanes would do; the block is small
+      const int h0 = r0 / p.head_blocks * p.group + r0 % p.head_blocks * p.block_heads;
+      const int nh = min(p.block_heads, p.group - r0 % p.head_blocks * p.block_heads);
+      for (int h = warp; h < nh; h += W) store_out<T>(p, b0, h0 + h, lane, make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
+      return;
     }
-    const int entry = __shfl_sync(0xffffffffu, cur, (j % per_win) * ppc + lane % ppc);
-    const int first = t0 + (warp + j * kQ4Warps) * kQ4Chunk;
-    const int pages = min(ppc, last_page - first / P + 1);
-    const int s = j % kQ4Stages;
+  } else {
+    for (int b = blockIdx.x; b < p.c.rows; b += p.ctas)  // sequences of no tokens belong to no range
+      if (seq_of(p, b) == 0)
+        for (int h = warp; h < p.num_q_heads; h += W) store_out<T>(p, b, h, lane, make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
+    const int total = batch_chunks(p) * R;
+    per = range_of(p, total);
+    if ((long long)blockIdx.x * per >= total) return;
+    lo = blockIdx.x * per;
+    hi = min(total, lo + per);
+    int before = 0;  // chunks of the sequences before this block of 32
+    b0 = r0 = begin = 0;
+    for (int base = 0;; base += 32) {
+      const int n = base + lane < p.c.rows ? chunks_of(seq_of(p, base + lane)) * R : 0;
+      int incl = n;
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, x);
+        if (lane >= x) incl += v;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, before + incl > lo);
+      if (past) {
+        const int at = __ffs(past) - 1;
+        const int seq_n = __shfl_sync(0xffffffffu, n, at);
+        const int seq_begin = before + __shfl_sync(0xffffffffu, incl, at) - seq_n;
+        b0 = base + at;
+        r0 = (lo - seq_begin) / (seq_n / R);
+        begin = seq_begin + r0 * (seq_n / R);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+  }
+
+  // Copies, ahead of the arithmetic: this warp takes chunks lo + warp, + 4, ...
+  // The position (row, table entries) of the copy after next is worked out while
+  // the chunks in flight are multiplied.
+  const uint64_t pol = l2_policy_evict_first();
+  int at = lo + warp, at_b = b0, at_r = r0, at_begin = begin, at_seq = seq_of(p, b0), at_n = chunks_of(at_seq);
+  int entry = 0, pages = 0, issued = 0;
+  auto locate = [&]() {
+    if (at >= hi) return;
+    while (at >= at_begin + at_n) {
+      at_begin += at_n;
+      if (at_n == 0 || ++at_r == R) {
+        at_r = 0;
+        at_seq = seq_of(p, ++at_b);
+        at_n = chunks_of(at_seq);
+      }
+    }
+    const int first = (at - at_begin) * ppc;
+    pages = min(ppc, (at_seq + P - 1) / P - first);
+    entry = lane < pages ? p.c.table[at_b * p.c.table_stride + first + lane] : 0;
+  };
+  auto issue = [&]() {
+    const int s = issued % kQ4Stages;
     if (lane == 0) mbar_arrive_expect_tx(bar0 + 8 * s, pages * slab);
     __syncwarp();
     if (lane < pages) {
@@ -234,12 +307,17 @@ __global__ void __launch_bounds__(kQ4Threads, NG == 4 ? 2 : 3) attn_q4_kernel(co
         atomicCAS(p.c.status, 0, DAK_ERR_INVALID_ARG);
         page = max(1ll, p.c.pages[tier]);
       }
-      tma_load_slab(ring + s * S::stage + lane * slab, &p.map[tier], (int)(page * p.c.kv_heads + kvh), bar0 + 8 * s, pol);
+      tma_load_slab(sbase + (warp * kQ4Stages + s) * S::stage + lane * slab, &p.map[tier],
+                    (int)(page * p.c.kv_heads + at_r / p.head_blocks), bar0 + 8 * s, pol);
     }
     __syncwarp();
+    ++issued;
+    at += W;
+    locate();
   };
-  const int ahead = min(mine, kQ4Stages);
-  for (int j = 0; j < ahead; ++j) issue(j);
+  locate();
+  for (int j = 0; j < kQ4Stages; ++j)
+    if (at < hi) issue();
 
   // Word w (0..3) of a K row that this lane multiplies, 8 dims each: all the
   // words of one group meet in the same MMA steps.
@@ -251,7 +329,7 @@ __global__ void __launch_bounds__(kQ4Threads, NG == 4 ? 2 : 3) attn_q4_kernel(co
   // over each group for the zeros' share.
   uint32_t qf[8][2];
   float qs[2][NG], f[2];
-  {
+  auto load_query = [&](int b, int h0, int nh) {
     float x[4][8], mx = 0.f, sum[NG];
 #pragma unroll
     for (int n = 0; n < NG; ++n) sum[n] = 0.f;
@@ -298,7 +376,7 @@ __global__ void __launch_bounds__(kQ4Threads, NG == 4 ? 2 : 3) attn_q4_kernel(co
 #pragma unroll
       for (int n = 0; n < NG; ++n) qs[e][n] = __shfl_sync(0xffffffffu, sum[n], src) * 0x1p-24f;
     }
-  }
+  };
 
   // V: this lane takes 4 dims at a time (piece x) of tokens 2 cq, 2 cq + 1 (and 8
   // on).  Odd columns read the second token first, which spreads a warp's reads
@@ -310,12 +388,8 @@ __global__ void __launch_bounds__(kQ4Threads, NG == 4 ? 2 : 3) attn_q4_kernel(co
   // Statistics: weights are 2^(score - m).  m is the largest score so far plus E,
   // the exponent of the warp's largest V scale so far, so that weight x scale is
   // below 2 and float16 holds it whatever V's magnitude.
-  float o[8][4], m[2] = {-FLT_MAX, -FLT_MAX}, l[2] = {0.f, 0.f}, E = -24.f;
-  uint32_t s_max = 0u;
-#pragma unroll
-  for (int t = 0; t < 8; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
+  float o[8][4], m[2], l[2], E;
+  uint32_t s_max;
 
   // One chunk of `valid` tokens in the stage at `st`.
   auto chunk = [&](const uint8_t *st, int valid, auto full_c) {
@@ -332,7 +406,20 @@ __global__ void __launch_bounds__(kQ4Threads, NG == 4 ? 2 : 3) attn_q4_kernel(co
     };
     float y[4][4];  // raw scores: tile, {token g, g + 8} x {head 2 cq, 2 cq + 1}
     float mx[2] = {-INFINITY, -INFINITY};
+    // V's (scale, zero) words of tile t, token g + 8r.  With one group they stay in
+    // registers; more of them are read again where they are needed, which costs
+    // less than the registers would.
     uint32_t vp[4][2][NG];
+    auto load_vp = [&](int t, int r, bool again) {
+      if (again && NG == 1) return;
+      load_pairs<NG>(st + vpairs_at(t, r), vp[t][r]);
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+        if (!kFull && t * 16 + 8 * r + g >= valid) vp[t][r][n] = 0u;  // anything may lie behind the last token
+    };
+    auto forget = [] {
+      if (NG > 1) asm volatile("" ::: "memory");
+    };
     __half2 vmax = __float2half2_rn(0.f);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -365,12 +452,9 @@ __global__ void __launch_bounds__(kQ4Threads, NG == 4 ? 2 : 3) attn_q4_kernel(co
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         load_pairs<NG>(st + pairs_at(t, r), kp[r]);
-        load_pairs<NG>(st + vpairs_at(t, r), vp[t][r]);
+        load_vp(t, r, false);
 #pragma unroll
-        for (int n = 0; n < NG; ++n) {
-          if (!kFull && t * 16 + 8 * r + g >= valid) vp[t][r][n] = 0u;  // anything may lie behind the last token
-          vmax = __hmax2(vmax, *reinterpret_cast<const __half2 *>(&vp[t][r][n]));
-        }
+        for (int n = 0; n < NG; ++n) vmax = __hmax2(vmax, *reinterpret_cast<const __half2 *>(&vp[t][r][n]));
       }
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
@@ -421,11 +505,13 @@ __global__ void __launch_bounds__(kQ4Threads, NG == 4 ? 2 : 3) attn_q4_kernel(co
       for (int n = 0; n < NG; ++n) zs[e][n] = 0.f;
     }
     // Weights, and the zeros' share of the output: sum_t p_t zero_t per group.
+    forget();
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       if (!kFull && t * 16 >= valid) continue;
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
+      for (int r = 0; r < 2; ++r) {
+        load_vp(t, r, true);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float w = ex2(fmaf(y[t][2 * r + e], f[e], -m[e]));
@@ -435,7 +521,9 @@ __global__ void __launch_bounds__(kQ4Threads, NG == 4 ? 2 : 3) attn_q4_kernel(co
 #pragma unroll
           for (int n = 0; n < NG; ++n) zs[e][n] = fmaf(w, half2_of(vp[t][r][n]).y, zs[e][n]);
         }
+      }
     }
+    forget();
 #pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -462,9 +550,10 @@ __global__ void __launch_bounds__(kQ4Threads, NG == 4 ? 2 : 3) attn_q4_kernel(co
       uint32_t bf[NG][2];
       [[maybe_unused]] uint32_t bl[NG][2];
 #pragma unroll
-      for (int n = 0; n < NG; ++n)
+      for (int r = 0; r < 2; ++r) {
+        load_vp(t, r, true);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+        for (int n = 0; n < NG; ++n) {
           const float s = half2_of(vp[t][r][n]).x;
           const float a = y[t][2 * r] * s, c = y[t][2 * r + 1] * s;
           const uint32_t hi = pack_half2(a, c);
@@ -474,6 +563,7 @@ __global__ void __launch_bounds__(kQ4Threads, NG == 4 ? 2 : 3) attn_q4_kernel(co
             bl[n][r] = movmatrix(pack_half2(a - back.x, c - back.y));
           }
         }
+      }
       uint32_t x[2][4];  // token pairs (2 cq, +1) and (2 cq + 8, +9): 4 pieces of 4 dims
       const uint32_t row0 = 2 * cq + flip, row1 = 2 * cq + 1 - flip;
       const uint32_t vc = rows_at(t) + half;
@@ -526,135 +616,210 @@ __global__ void __launch_bounds__(kQ4Threads, NG == 4 ? 2 : 3) attn_q4_kernel(co
     }
   };
 
-  bool ok = true;
-  for (int j = 0; j < mine; ++j) {
-    const int s = j % kQ4Stages;
-    ok = mbar_wait<false>(bar0 + 8 * s, (j / kQ4Stages) & 1, wc);
-    if (!__all_sync(0xffffffffu, ok)) {
-      // Gave up: let this warp's copies land (bounded again), then leave.
-      if (lane == 0) {
-        const WaitCtx drain{reinterpret_cast<volatile int *>(smem + S::flag_off + 4), p.c.status};
-        for (int k = j; k < min(mine, j + kQ4Stages); ++k)
-          mbar_wait<false>(bar0 + 8 * (k % kQ4Stages), (k / kQ4Stages) & 1, drain);
-      }
-      __syncwarp();
-      break;
-    }
-    const uint8_t *st = smem + (warp * kQ4Stages + s) * S::stage;
-    const int valid = min(kQ4Chunk, t1 - (t0 + (warp + j * kQ4Warps) * kQ4Chunk));
-    if (valid == kQ4Chunk)
-      chunk(st, valid, std::true_type{});
-    else
-      chunk(st, valid, std::false_type{});
-    __syncwarp();
-    if (j + kQ4Stages < mine) issue(j + kQ4Stages);
-  }
-
-  // Merge the warps: each leaves (m, l, o) of its heads, o in its own ring.
   float *sm_m = reinterpret_cast<float *>(smem + S::m_off), *sm_l = reinterpret_cast<float *>(smem + S::l_off);
-#pragma unroll
-  for (int e = 0; e < 2; ++e)
-#pragma unroll
-    for (int x = 4; x <= 16; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
-  float *ring_f = reinterpret_cast<float *>(smem + warp * kQ4Stages * S::stage);  // [head][dim]
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int h = 2 * cq + e;
-    if (h >= nh) continue;
-    if (g == 0) {
-      sm_m[warp * kQ4Heads + h] = m[e];
-      sm_l[warp * kQ4Heads + h] = l[e];
-    }
-#pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      const int q = t >> 1;
-      const int d = (NG == 1 ? 16 * g + 4 * q : NG == 2 ? 64 * (q >> 1) + 8 * g + 4 * (q & 1) : 32 * q + 4 * g) + 2 * (t & 1);
-      *reinterpret_cast<float2 *>(ring_f + h * kKv4Dim + d) = make_float2(o[t][e] * 0x1p24f, o[t][2 + e] * 0x1p20f);
-    }
-  }
-  __syncthreads();
-  const int d = threadIdx.x;
-  for (int h = 0; h < nh; ++h) {
-    float gm = -FLT_MAX;
-#pragma unroll
-    for (int w = 0; w < kQ4Warps; ++w) gm = fmaxf(gm, sm_m[w * kQ4Heads + h]);
-    float den = 0.f, acc = 0.f;
-#pragma unroll
-    for (int w = 0; w < kQ4Warps; ++w) {
-      const float c = ex2(sm_m[w * kQ4Heads + h] - gm);
-      den = fmaf(sm_l[w * kQ4Heads + h], c, den);
-      acc = fmaf(reinterpret_cast<const float *>(smem + w * kQ4Stages * S::stage)[h * kKv4Dim + d], c, acc);
-    }
-    if (splits == 1) {
-      p.out[b * p.o_stride_b + (h0 + h) * p.o_stride_h + d] = Elem<T>::from_float(den == 0.f ? 0.f : acc / den);
-    } else {
-      const long long at = ((long long)b * p.num_q_heads + h0 + h) * p.num_splits + split;
-      p.partial_o[at * kKv4Dim + d] = acc;
-      if (d == 0) {
-        p.partial_ml[at * 2] = gm;
-        p.partial_ml[at * 2 + 1] = den;
+  float *sm_o = reinterpret_cast<float *>(smem + S::o_off);
+  int done = 0, dead_at = -1;  // chunks taken; the chunk whose copy never came
+  int b = b0, r = r0, seq = seq_of(p, b0), n = chunks_of(seq);
+  for (int s0 = lo; s0 < hi;) {
+    // The segment [s0, s1) of row (b, r), whose chunks begin at `begin`.
+    while (s0 >= begin + n) {
+      begin += n;
+      if (n == 0 || ++r == R) {
+        r = 0;
+        seq = seq_of(p, ++b);
+        n = chunks_of(seq);
       }
     }
-  }
-  if (splits > 1 && p.counters) {
-    // The split that finishes last merges all of them and resets the counter.
-    int *last = reinterpret_cast<int *>(smem + S::flag_off + 8);
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      int32_t *counter = p.counters + blockIdx.x / p.num_splits;
-      *last = atomicAdd(counter, 1) == splits - 1;
-      if (*last) *counter = 0;
+    const int s1 = min(hi, begin + n);
+    const int hb = r % p.head_blocks, h0 = r / p.head_blocks * p.group + hb * p.block_heads;
+    const int nh = min(p.block_heads, p.group - hb * p.block_heads);
+    load_query(b, h0, nh);
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
+    m[0] = m[1] = -FLT_MAX;
+    l[0] = l[1] = 0.f;
+    E = -24.f;
+    s_max = 0u;
+    for (; lo + warp + W * done < s1; ++done) {
+      const int id = lo + warp + W * done, s = done % kQ4Stages;
+      const bool ok = dead_at < 0 && mbar_wait<false>(bar0 + 8 * s, (done / kQ4Stages) & 1, wc);
+      if (!__all_sync(0xffffffffu, ok)) {  // give up, but keep to the barriers below
+        if (dead_at < 0) dead_at = done;
+        continue;
+      }
+      const uint8_t *st = smem + (warp * kQ4Stages + s) * S::stage;
+      const int valid = min(kQ4Chunk, seq - (id - begin) * kQ4Chunk);
+      if (valid == kQ4Chunk)
+        chunk(st, valid, std::true_type{});
+      else
+        chunk(st, valid, std::false_type{});
+      __syncwarp();
+      if (at < hi) issue();
+    }
+
+    // Add up the warps: statistics first, then each warp its share in turn.
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int x = 4; x <= 16; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
+      if (g == 0) {
+        sm_m[warp * kQ4Heads + 2 * cq + e] = m[e];
+        sm_l[warp * kQ4Heads + 2 * cq + e] = l[e];
+      }
     }
     __syncthreads();
-    if (*last) {
+    float c[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int h = 2 * cq + e;
+      float gm = sm_m[h];
+#pragma unroll
+      for (int w = 1; w < W; ++w) gm = fmaxf(gm, sm_m[w * kQ4Heads + h]);
+      c[e] = ex2(m[e] - gm);
+    }
+    const int live = min(W, s1 - s0);  // warps that had a chunk of this segment
+    for (int turn = 0; turn < live; ++turn) {
+      // Chunk s0 + turn is this warp's.
+      if ((s0 - lo + turn) % W == warp) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int h = 2 * cq + e;
+          if (h >= nh) continue;
+#pragma unroll
+          for (int t = 0; t < 8; ++t) {
+            const int q = t >> 1;
+            const int d =
+                (NG == 1 ? 16 * g + 4 * q : NG == 2 ? 64 * (q >> 1) + 8 * g + 4 * (q & 1) : 32 * q + 4 * g) + 2 * (t & 1);
+            float2 *to = reinterpret_cast<float2 *>(sm_o + h * kKv4Dim + d);
+            float2 v = turn == 0 ? make_float2(0.f, 0.f) : *to;
+            v.x = fmaf(o[t][e] * 0x1p24f, c[e], v.x);
+            v.y = fmaf(o[t][2 + e] * 0x1p20f, c[e], v.y);
+            *to = v;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    // A warp per head: the output, or a piece of it.
+    const bool whole = s0 == begin && s1 == begin + n;
+    for (int h = warp; h < nh; h += W) {
+      float gm = sm_m[h], den = 0.f;
+#pragma unroll
+      for (int w = 1; w < W; ++w) gm = fmaxf(gm, sm_m[w * kQ4Heads + h]);
+#pragma unroll
+      for (int w = 0; w < W; ++w) den = fmaf(sm_l[w * kQ4Heads + h], ex2(sm_m[w * kQ4Heads + h] - gm), den);
+      const float4 v = *reinterpret_cast<const float4 *>(sm_o + h * kKv4Dim + 4 * lane);
+      if (whole) {
+        store_out<T>(p, b, h0 + h, lane, v, den);
+      } else {
+        const long long slot = (2ll * blockIdx.x + (s0 == lo ? 0 : 1)) * kQ4Heads + h;
+        __stcg(reinterpret_cast<float4 *>(p.scratch + slot * kKv4Dim) + lane, v);
+        if (lane == 0)
+          __stcg(reinterpret_cast<float2 *>(p.scratch + 2ll * p.ctas * kQ4Heads * kKv4Dim) + slot, make_float2(gm, den));
+      }
+    }
+    if (!whole && p.counters) {
+      // The CTA that finishes the row last merges it and resets the counter.
+      int *last = reinterpret_cast<int *>(smem + S::flag_off + 8);
       __threadfence();
-      merge_q4<T>(p, b, h0, nh, splits, sm_m);
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        int32_t *counter = p.counters + (long long)b * R + r;
+        *last = atomicAdd(counter, 1) == (begin + n - 1) / per - begin / per;
+        if (*last) *counter = 0;
+      }
+      __syncthreads();
+      if (*last) {
+        __threadfence();
+        merge_row<T>(p, b, h0, nh, begin, begin + n, per, W);
+      }
     }
+    __syncthreads();  // the statistics are free again
+    s0 = s1;
+  }
+  if (dead_at >= 0 && lane == 0) {
+    // Copies still in flight land before the CTA leaves (bounded again).
+    const WaitCtx drain{reinterpret_cast<volatile int *>(smem + S::flag_off + 4), p.c.status};
+    for (int k = dead_at; k < issued; ++k) mbar_wait<false>(bar0 + 8 * (k % kQ4Stages), (k / kQ4Stages) & 1, drain);
   }
 }
 
-// The merge as a launch of its own, one CTA per block of heads.
+// The merge as a launch of its own, one CTA per row.
 template <typename T>
-__global__ void __launch_bounds__(kQ4Threads) attn_q4_merge_kernel(const __grid_constant__ AttnQ4Params p) {
-  __shared__ float sm[2 * kQ4Heads];
+__global__ void __launch_bounds__(kQ4MergeWarps * 32) attn_q4_merge_kernel(const __grid_constant__ AttnQ4Params p) {
   pdl_enter(p.pdl);
-  int i = blockIdx.x;
-  const int hb = i % p.head_blocks;
-  i /= p.head_blocks;
-  const int kvh = i % p.c.kv_heads;
-  const int b = i / p.c.kv_heads;
-  const int splits = live_splits(p, max(0, min(p.seq_lens[b], p.max_seq_len)));
-  if (splits == 1) return;  // written already
-  merge_q4<T>(p, b, kvh * p.group + hb * p.block_heads, min(p.block_heads, p.group - hb * p.block_heads), splits, sm);
+  const int R = p.c.kv_heads * p.head_blocks;
+  const int b = blockIdx.x / R, r = blockIdx.x - b * R;
+  const int n = chunks_of(seq_of(p, b));
+  int before = 0, total = 0;
+  for (int i = lane_id(); i < p.c.rows; i += 32) {
+    const int v = chunks_of(seq_of(p, i));
+    total += v;
+    before += i < b ? v : 0;
+  }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, x);
+    before += __shfl_xor_sync(0xffffffffu, before, x);
+  }
+  const int per = range_of(p, total * R), begin = before * R + r * n;
+  if (n == 0 || begin / per == (begin + n - 1) / per) return;  // written already
+  const int hb = r % p.head_blocks;
+  merge_row<T>(p, b, r / p.head_blocks * p.group + hb * p.block_heads, min(p.block_heads, p.group - hb * p.block_heads), begin,
+               begin + n, per, kQ4MergeWarps);
 }
 
 template <typename T, int NG, int P>
-cudaError_t launch_attn(const AttnQ4Params &p, long long grid, cudaStream_t s) {
+cudaError_t launch_attn(const AttnQ4Params &p, int rows, cudaStream_t s) {
   auto kern = attn_q4_kernel<T, NG, P>;
   cudaError_t e = prepare_kernel_attributes(reinterpret_cast<const void *>(kern));
   if (e != cudaSuccess) return e;
-  e = launch_ex(kern, dim3((unsigned)grid), dim3(kQ4Threads), Q4Smem<NG>::bytes, s, 1, p.pdl != 0, p);
-  if (e != cudaSuccess || p.num_splits == 1 || p.counters) return e;
-  return launch_ex(attn_q4_merge_kernel<T>, dim3((unsigned)(grid / p.num_splits)), dim3(kQ4Threads), 0, s, 1, p.pdl != 0, p);
+  e = launch_ex(kern, dim3(p.ctas), dim3(Q4Smem<NG>::threads), Q4Smem<NG>::bytes, s, 1, p.pdl != 0, p);
+  if (e != cudaSuccess || p.by_row || p.counters) return e;
+  return launch_ex(attn_q4_merge_kernel<T>, dim3(rows), dim3(kQ4MergeWarps * 32), 0, s, 1, p.pdl != 0, p);
 }
 
 template <typename T, int NG>
-cudaError_t launch_attn_g(const AttnQ4Params &p, long long grid, cudaStream_t s) {
+cudaError_t launch_attn_g(const AttnQ4Params &p, int rows, cudaStream_t s) {
   switch (p.c.page_size) {
-    case 16: return launch_attn<T, NG, 16>(p, grid, s);
-    case 32: return launch_attn<T, NG, 32>(p, grid, s);
-    default: return launch_attn<T, NG, 64>(p, grid, s);
+    case 16: return launch_attn<T, NG, 16>(p, rows, s);
+    case 32: return launch_attn<T, NG, 32>(p, rows, s);
+    default: return launch_attn<T, NG, 64>(p, rows, s);
   }
 }
 
 template <typename T>
-cudaError_t launch_attn_t(const AttnQ4Params &p, long long grid, cudaStream_t s) {
+cudaError_t launch_attn_t(const AttnQ4Params &p, int rows, cudaStream_t s) {
   switch (p.c.ng) {
-    case 1: return launch_attn_g<T, 1>(p, grid, s);
-    case 2: return launch_attn_g<T, 2>(p, grid, s);
-    default: return launch_attn_g<T, 4>(p, grid, s);
+    case 1: return launch_attn_g<T, 1>(p, rows, s);
+    case 2: return launch_attn_g<T, 2>(p, rows, s);
+    default: return launch_attn_g<T, 4>(p, rows, s);
   }
+}
+
+// How a call is dealt out.  Rows that fit the GPU at once and are short are not
+// split: a merge would cost more than it gives.  Else there are as many CTAs as
+// the GPU holds at once, or as there can be warps with a chunk.
+struct Q4Plan {
+  long long rows;
+  int ctas, warps, by_row;
+  long long scratch_floats;
+};
+
+Q4Plan q4_plan(const dak_kv4_cache *c, int num_q_heads, int max_seq_len) {
+  Q4Plan plan;
+  const int group = num_q_heads / c->kv_heads;
+  plan.rows = (long long)c->batch * c->kv_heads * ((group + kQ4Heads - 1) / kQ4Heads);
+  const long long chunks = ((long long)max_seq_len + kQ4Chunk - 1) / kQ4Chunk;
+  const int resident = device_sms() * kQ4PerSm;
+  plan.warps = c->group == 32 ? Q4Smem<4>::warps : Q4Smem<1>::warps;
+  plan.by_row = plan.rows <= resident && chunks <= kQ4RowChunks;
+  plan.ctas = plan.by_row ? (int)plan.rows
+                          : (int)std::min<long long>(resident, (plan.rows * chunks + plan.warps - 1) / plan.warps);
+  plan.scratch_floats = plan.by_row ? 0 : 2ll * plan.ctas * kQ4Heads * (kKv4Dim + 2);
+  return plan;
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
@@ -703,16 +868,18 @@ extern "C" int dak_attn_decode_paged_q4(const dak_kv4_cache *cache, const dak_at
     return fail(DAK_ERR_INVALID_ARG, "num_q_heads must be a positive multiple of kv_heads");
   if (a->max_seq_len <= 0 || (int64_t)cache->max_pages * cache->page_size < a->max_seq_len)
     return fail(DAK_ERR_INVALID_ARG, "max_seq_len must be positive and within the block table's pages");
-  if (a->split_size <= 0 || a->split_size % 64)
-    return fail(DAK_ERR_INVALID_ARG, "split_size must be a positive multiple of 64");
   if (!a->query || !a->out || !a->seq_lens) return fail(DAK_ERR_INVALID_ARG, "query, out and seq_lens are required");
-  if (a->q_stride_b % 8 || a->q_stride_h % 8 || (reinterpret_cast<uintptr_t>(a->query) & 15u))
-    return fail(DAK_ERR_ALIGNMENT, "query must be 16-byte aligned, its strides multiples of 8 elements");
-  const int splits = (int)(((long long)a->max_seq_len + a->split_size - 1) / a->split_size);
-  if (splits > 1 && (!a->partial_o || !a->partial_ml))
-    return fail(DAK_ERR_INVALID_ARG, "partial_o and partial_ml scratch are required when max_seq_len > split_size");
-  const void *ptrs[6] = {a->query, a->out, a->seq_lens, splits > 1 ? a->partial_o : nullptr,
-                         splits > 1 ? a->partial_ml : nullptr, splits > 1 ? a->merge_counters : nullptr};
+  if (a->q_stride_b % 8 || a->q_stride_h % 8 || a->o_stride_b % 8 || a->o_stride_h % 8 ||
+      ((reinterpret_cast<uintptr_t>(a->query) | reinterpret_cast<uintptr_t>(a->out) |
+        reinterpret_cast<uintptr_t>(a->scratch)) & 15u))
+    return fail(DAK_ERR_ALIGNMENT, "query, out and scratch must be 16-byte aligned, strides multiples of 8 elements");
+  const Q4Plan plan = q4_plan(cache, a->num_q_heads, a->max_seq_len);
+  if (plan.rows > 0x7fffffffll / (((int64_t)a->max_seq_len + kQ4Chunk - 1) / kQ4Chunk))
+    return fail(DAK_ERR_UNSUPPORTED, "batch x heads x max_seq_len is too large for one launch");
+  if (plan.scratch_floats > 0 && (!a->scratch || a->scratch_floats < plan.scratch_floats))
+    return fail(DAK_ERR_INVALID_ARG, "attention needs %lld floats of scratch", (long long)plan.scratch_floats);
+  const void *ptrs[5] = {a->query, a->out, a->seq_lens, plan.by_row ? nullptr : a->scratch,
+                         plan.by_row ? nullptr : a->merge_counters};
   for (const void *q : ptrs)
     if (q && (st = check_gpu_accessible(q, "attention buffer"))) return st;
   AttnQ4Params p;
@@ -727,21 +894,26 @@ extern "C" int dak_attn_decode_paged_q4(const dak_kv4_cache *cache, const dak_at
   p.o_stride_b = a->o_stride_b;
   p.o_stride_h = a->o_stride_h;
   p.seq_lens = a->seq_lens;
-  p.partial_o = a->partial_o;
-  p.partial_ml = a->partial_ml;
-  p.counters = splits > 1 ? a->merge_counters : nullptr;
+  p.scratch = plan.by_row ? nullptr : a->scratch;
+  p.counters = plan.by_row ? nullptr : a->merge_counters;
   p.num_q_heads = a->num_q_heads;
   p.group = a->num_q_heads / cache->kv_heads;
   p.head_blocks = (p.group + kQ4Heads - 1) / kQ4Heads;
   p.block_heads = (p.group + p.head_blocks - 1) / p.head_blocks;
   p.max_seq_len = a->max_seq_len;
-  p.split_size = a->split_size;
-  p.num_splits = splits;
+  p.ctas = plan.ctas;
+  p.warps = plan.warps;
+  p.by_row = plan.by_row;
   p.scale_log2 = a->scaling * 1.4426950408889634f;
   p.pdl = decode_pdl_enabled() ? 1 : 0;
-  const long long grid = (long long)cache->batch * cache->kv_heads * p.head_blocks * splits;
-  if (grid > 0x7fffffffll) return fail(DAK_ERR_UNSUPPORTED, "too many splits for one launch; raise split_size");
   auto s = static_cast<cudaStream_t>(stream);
-  return cuda_status(a->dtype == DAK_DTYPE_F16 ? launch_attn_t<__half>(p, grid, s) : launch_attn_t<__nv_bfloat16>(p, grid, s),
+  const int rows = (int)plan.rows;
+  return cuda_status(a->dtype == DAK_DTYPE_F16 ? launch_attn_t<__half>(p, rows, s) : launch_attn_t<__nv_bfloat16>(p, rows, s),
                      "4-bit attention launch");
+}
+
+extern "C" int64_t dak_attn_q4_scratch(const dak_kv4_cache *cache, int num_q_heads, int max_seq_len) {
+  using namespace dak;
+  if (kv4_check(cache) || num_q_heads <= 0 || num_q_heads % cache->kv_heads || max_seq_len <= 0) return -1;
+  return q4_plan(cache, num_q_heads, max_seq_len).scratch_floats;
 }

@@ -25,6 +25,8 @@ int cuda_status(cudaError_t e, const char *what);
 uint64_t current_context_id();
 // Device address of the kernels' error word in the current context.
 int *device_status_word();
+// SMs of the current device (a B200's 148 when there is none).
+int device_sms();
 // DAK_OK if `p` is memory of the current device or pinned host memory.
 int check_gpu_accessible(const void *p, const char *what);
 // DAK_OK if the rotary kernels serve this part of a head.

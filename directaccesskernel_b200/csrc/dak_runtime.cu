@@ -119,6 +119,11 @@ int device_info(DeviceInfo **out) {
 }
 }  // namespace
 
+int device_sms() {
+  DeviceInfo *d = nullptr;
+  return device_info(&d) == DAK_OK ? d->num_sms : 148;
+}
+
 int *device_status_word() {
   DeviceInfo *d = nullptr;
   return device_info(&d) == DAK_OK ? d->status : nullptr;

@@ -178,35 +178,40 @@ def kv_read_q4(pool_dev: torch.Tensor | None, pool_host: torch.Tensor | None, bl
     return k_out, v_out
 
 
-def auto_split_size_q4(rows: int, max_seq_len: int) -> int:
-    """Tokens per split (a multiple of 64) for ``rows`` = sequences x KV heads x head
-    blocks."""
-    splits = max(1, min(444 // rows if rows <= 444 else 2000 // rows, max_seq_len // 256))
-    return -(-max_seq_len // (splits * 64)) * 64
-
-
 def merge_counter_count(batch: int, q_heads: int, kv_heads: int) -> int:
     """Entries of ``decode_paged_q4``'s merge_counters."""
     return batch * kv_heads * -(-(q_heads // kv_heads) // MAX_BLOCK_HEADS)
 
 
+def scratch_floats(batch: int, q_heads: int, kv_heads: int, page_size: int, group: int, max_seq_len: int) -> int:
+    """Entries of ``decode_paged_q4``'s scratch on the current device."""
+    c = _lib.Kv4Cache()
+    c.pool_dev, c.dev_pages, c.block_table = 16, 1, 16  # checked for presence only
+    c.table_stride = c.max_pages = -(-max_seq_len // page_size)
+    c.batch, c.kv_heads, c.page_size, c.group = batch, kv_heads, page_size, group
+    n = LIB.dak_attn_q4_scratch(ctypes.byref(c), q_heads, max_seq_len)
+    if n < 0:
+        raise RuntimeError("decode_paged_q4 does not serve these sizes")
+    return n
+
+
 @traced
 def decode_paged_q4(query: torch.Tensor, pool_dev: torch.Tensor | None, pool_host: torch.Tensor | None,
-                    block_table: torch.Tensor, seq_lens: torch.Tensor, scaling: float, split_size: int | None = None, *,
-                    out: torch.Tensor | None = None, partial_o: torch.Tensor | None = None,
-                    partial_ml: torch.Tensor | None = None, max_seq_len: int | None = None,
-                    merge_counters: torch.Tensor | None = None) -> torch.Tensor:
+                    block_table: torch.Tensor, seq_lens: torch.Tensor, scaling: float, *,
+                    out: torch.Tensor | None = None, scratch: torch.Tensor | None = None,
+                    max_seq_len: int | None = None, merge_counters: torch.Tensor | None = None) -> torch.Tensor:
     """Decode attention over the 4-bit cache; returns [B, Hq, 128].
 
     ``query`` [B, Hq, 128], any number of query heads per KV head; ``seq_lens``
     [B] int32 on the GPU (0: the row is zeros; longer than ``max_seq_len``: cut to
-    it).  ``max_seq_len`` defaults to what the block table can name.  Scratch:
-    partial_o [B, Hq, splits, 128] and partial_ml [B, Hq, splits, 2] float32,
-    allocated when not given.  With ``merge_counters`` (int32 CUDA,
-    ``merge_counter_count`` entries, zero before the first call and left zero by
-    every call) the last split merges the splits inside the attention kernel
-    instead of a second launch; the result is the same.  Calls that may overlap
-    on the GPU need scratch and counters of their own."""
+    it).  ``max_seq_len`` defaults to what the block table can name; the work is
+    spread over the GPU by the lengths themselves.  ``scratch``: float32,
+    ``scratch_floats`` entries, allocated when not given and needed.  With
+    ``merge_counters`` (int32 CUDA, ``merge_counter_count`` entries, zero before
+    the first call and left zero by every call) rows that were split are merged
+    inside the attention kernel instead of by a second launch; the result is the
+    same.  Calls that may overlap on the GPU need scratch and counters of their
+    own."""
     device = current_device_of(query, "query")
     dtype = query.dtype
     if query.dim() != 3 or query.shape[2] != HEAD_DIM or query.stride(2) != 1:
@@ -220,41 +225,28 @@ def decode_paged_q4(query: torch.Tensor, pool_dev: torch.Tensor | None, pool_hos
     if seq_lens.dtype != torch.int32 or seq_lens.get_device() != device or seq_lens.numel() != B \
             or not seq_lens.is_contiguous():
         raise RuntimeError("seq_lens must be a contiguous int32 CUDA tensor [B]")
-    kv_heads = c.kv_heads
-    if Hq % kv_heads:
+    if Hq % c.kv_heads:
         raise RuntimeError("the KV heads must divide the query heads")
     if max_seq_len is None:
         max_seq_len = c.max_pages * c.page_size
-    blocks = -(-(Hq // kv_heads) // MAX_BLOCK_HEADS)
-    if split_size is None:
-        split_size = auto_split_size_q4(B * kv_heads * blocks, max_seq_len)
-    if split_size <= 0:
-        raise RuntimeError("split_size must be positive")
-    splits = -(-max_seq_len // split_size)
+    elif not 0 < max_seq_len <= c.max_pages * c.page_size:
+        raise RuntimeError("max_seq_len must be positive and within the block table's pages")
     if out is None:
         out = torch.empty((B, Hq, HEAD_DIM), dtype=dtype, device=query.device)
     elif out.shape != query.shape or out.dtype != dtype or out.get_device() != device or out.stride(2) != 1:
         raise RuntimeError("out must be [B, Hq, 128] of the query dtype with a contiguous last dimension")
     a = _lib.AttnQ4Args()
-    if splits > 1:
-        n = B * Hq * splits
-        for t, per, nm in ((partial_o, HEAD_DIM, "partial_o"), (partial_ml, 2, "partial_ml")):
-            if t is not None and (t.dtype != torch.float32 or t.get_device() != device or not t.is_contiguous()
-                                  or t.numel() < n * per):
-                raise RuntimeError(f"{nm} must be a contiguous float32 CUDA tensor of B * Hq * {splits} * {per} entries")
-        if partial_o is None and partial_ml is None:  # one allocation for both
-            partial_o = torch.empty(n * (HEAD_DIM + 2), dtype=torch.float32, device=query.device)
-            a.partial_o = partial_o.data_ptr()
-            a.partial_ml = a.partial_o + 4 * n * HEAD_DIM
-        else:
-            if partial_o is None:
-                partial_o = torch.empty(n * HEAD_DIM, dtype=torch.float32, device=query.device)
-            if partial_ml is None:
-                partial_ml = torch.empty(n * 2, dtype=torch.float32, device=query.device)
-            a.partial_o, a.partial_ml = partial_o.data_ptr(), partial_ml.data_ptr()
+    need = LIB.dak_attn_q4_scratch(ctypes.byref(c), Hq, max_seq_len)
+    if need > 0:
+        if scratch is None:
+            scratch = torch.empty(need, dtype=torch.float32, device=query.device)
+        elif scratch.dtype != torch.float32 or scratch.get_device() != device or scratch.numel() < need \
+                or not scratch.is_contiguous():
+            raise RuntimeError(f"scratch must be a contiguous float32 CUDA tensor of {need} entries")
+        a.scratch, a.scratch_floats = scratch.data_ptr(), need
         if merge_counters is not None:
             if merge_counters.dtype != torch.int32 or merge_counters.get_device() != device \
-                    or merge_counters.numel() < B * kv_heads * blocks or not merge_counters.is_contiguous():
+                    or merge_counters.numel() < merge_counter_count(B, Hq, c.kv_heads) or not merge_counters.is_contiguous():
                 raise RuntimeError("merge_counters must be a contiguous int32 CUDA tensor of merge_counter_count entries")
             a.merge_counters = merge_counters.data_ptr()
     a.query, a.seq_lens, a.out = query.data_ptr(), seq_lens.data_ptr(), out.data_ptr()
@@ -263,7 +255,6 @@ def decode_paged_q4(query: torch.Tensor, pool_dev: torch.Tensor | None, pool_hos
     ob, oh, _ = out.stride()
     a.q_stride_b, a.q_stride_h = qb if B > 1 else 0, qh if Hq > 1 else 0
     a.o_stride_b, a.o_stride_h = ob if B > 1 else 0, oh if Hq > 1 else 0
-    a.num_q_heads, a.max_seq_len, a.split_size = Hq, max_seq_len, split_size
-    a.scaling, a.dtype = scaling, dak_dtype(dtype)
+    a.num_q_heads, a.max_seq_len, a.scaling, a.dtype = Hq, max_seq_len, scaling, dak_dtype(dtype)
     check(LIB.dak_attn_decode_paged_q4(ctypes.byref(c), ctypes.byref(a), stream_of(device)), "decode_paged_q4")
     return out

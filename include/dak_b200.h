@@ -471,27 +471,32 @@ DAK_API int dak_kv_read_q4(const dak_kv4_cache *cache, const int32_t *positions,
 
 /* Decode attention over the 4-bit cache: one query token per sequence, any
  * number of query heads per KV head.  Sequences longer than max_seq_len are cut
- * to it; one of no tokens gives zeros.  partial_o holds batch * num_q_heads *
- * splits * 128 floats and partial_ml twice batch * num_q_heads * splits, splits =
- * ceil(max_seq_len / split_size); neither is used with one split.
- * merge_counters (optional): batch * kv_heads * ceil(num_q_heads / kv_heads / 8)
- * int32 in device memory, zero before the first call and left zero by every
- * call; with them the last split merges, without them a second kernel does.
- * Calls that share scratch or counters must not overlap. */
+ * to it; one of no tokens gives zeros.  The work is spread evenly over the GPU
+ * by the sequences' lengths, which are read on the device: a graph captured with
+ * one max_seq_len serves any lengths up to it.  scratch: dak_attn_q4_scratch
+ * floats (0: none needed).  merge_counters (optional): batch * kv_heads *
+ * ceil(num_q_heads / kv_heads / 8) int32 in device memory, zero before the first
+ * call and left zero by every call; with them the CTA that finishes a row last
+ * merges its pieces, without them a second kernel does; the results are the
+ * same bits.  Calls that share scratch or counters must not overlap. */
 typedef struct dak_attn_q4_args {
   const void *query;          /* [batch, num_q_heads, 128]                      */
-  int64_t q_stride_b, q_stride_h;
+  int64_t q_stride_b, q_stride_h;   /* elements, multiples of 8                 */
   const int32_t *seq_lens;    /* [batch]                                        */
   void *out;                  /* [batch, num_q_heads, 128]                      */
-  int64_t o_stride_b, o_stride_h;
-  float *partial_o, *partial_ml;
+  int64_t o_stride_b, o_stride_h;   /* elements, multiples of 8                 */
+  float *scratch;
+  int64_t scratch_floats;
   int32_t *merge_counters;
   int num_q_heads, max_seq_len;
-  int split_size;             /* tokens per split, multiple of 64               */
   float scaling;
   int dtype;
 } dak_attn_q4_args;
 DAK_API int dak_attn_decode_paged_q4(const dak_kv4_cache *cache, const dak_attn_q4_args *args, void *stream);
+/* Floats of scratch that dak_attn_decode_paged_q4 needs for these sizes on the
+ * current device (from the cache only batch, kv_heads and the format count
+ * beside its own checks); negative for sizes that it refuses. */
+DAK_API int64_t dak_attn_q4_scratch(const dak_kv4_cache *cache, int num_q_heads, int max_seq_len);
 
 /* ------------------------------------------------------------ cache pages */
 /* Copies page src[i] to page dst[i] (host arrays; v >= 0 names device page v,

@@ -201,13 +201,13 @@ def _bound(ref, q, k_abs, v_range, scaling, dtype):
     return rounding(ref, dtype) + 2.0**-11 * v_range + 2 * d * (v_range + ref[torch.isfinite(ref)].abs().amax())
 
 
-def _attend(B, Hq, Hkv, page, group, lens, dtype, seed, *, split=None, width=None, host_every=0, q_pad=0, counters=False,
+def _attend(B, Hq, Hkv, page, group, lens, dtype, seed, *, wide=False, width=None, host_every=0, q_pad=0, counters=False,
             max_seq_len=None, spread=1.0, q_scale=1.0, share_out=False):
     kv4 = _kv4()
     g = torch.Generator().manual_seed(seed)
     lens = torch.tensor(lens)
     pages = [-(-max(0, int(n)) // page) for n in lens]
-    width = width or max(1, max(pages))
+    width = max(width or 1, max(pages), 513 // page + 1 if wide else 1)  # beyond 512 tokens rows may be split
     ids = torch.randperm(sum(pages), generator=g).tolist()
     table = torch.full((B, width), 2**30, dtype=torch.int64)  # entries past a sequence are never read
     n_dev = n_host = 0
@@ -225,7 +225,7 @@ def _attend(B, Hq, Hkv, page, group, lens, dtype, seed, *, split=None, width=Non
     limit = max_seq_len or width * page
     cnt = torch.zeros(kv4.merge_counter_count(B, Hq, Hkv), dtype=torch.int32, device="cuda") if counters else None
     got = kv4.decode_paged_q4(q.cuda()[..., :D], pool.cuda(), host.pin_memory() if host is not None else None,
-                              table.int().cuda(), lens.int().cuda(), scaling, split, max_seq_len=max_seq_len,
+                              table.int().cuda(), lens.int().cuda(), scaling, max_seq_len=max_seq_len,
                               merge_counters=cnt)
     if counters:
         assert not cnt.any()
@@ -238,26 +238,28 @@ def _attend(B, Hq, Hkv, page, group, lens, dtype, seed, *, split=None, width=Non
 
 @pytest.mark.parametrize("lens", [[1], [2], [15], [16], [17], [63], [64], [65], [130], [1000]])
 @pytest.mark.parametrize("page,group", [(16, 32), (32, 64), (64, 128)])
-def test_attend_lengths(lens, page, group):
-    got, ref, tol = _attend(1, 4, 1, page, group, lens, torch.float16, lens[0])
+@pytest.mark.parametrize("wide", [False, True])
+def test_attend_lengths(lens, page, group, wide):
+    got, ref, tol = _attend(1, 4, 1, page, group, lens, torch.float16, lens[0], wide=wide)
     assert ((got - ref).abs() <= tol).all()
 
 
 @pytest.mark.parametrize("share", [1, 2, 3, 4, 5, 6, 7, 8, 9, 12, 16, 20])
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_attend_shared_heads(share, dtype):
-    got, ref, tol = _attend(2, 2 * share, 2, 16, 64, [100, 70], dtype, share, split=64)
+@pytest.mark.parametrize("wide", [False, True])
+def test_attend_shared_heads(share, dtype, wide):
+    got, ref, tol = _attend(2, 2 * share, 2, 16, 64, [100, 70], dtype, share, wide=wide)
     assert ((got - ref).abs() <= tol).all()
 
 
 @pytest.mark.parametrize("counters", [False, True])
-@pytest.mark.parametrize("page,group,host_every,split", [
-    (16, 32, 2, 64), (16, 128, 3, 192), (32, 64, 1, 128), (64, 32, 2, 320), (64, 128, 0, 64), (64, 128, 3, 4096)])
+@pytest.mark.parametrize("page,group,host_every", [(16, 32, 2), (16, 64, 0), (16, 128, 3), (32, 64, 1), (32, 128, 2),
+                                                   (32, 32, 0), (64, 32, 2), (64, 64, 3), (64, 128, 0), (64, 128, 3)])
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_attend_ragged_tiers_and_splits(counters, page, group, host_every, split, dtype):
-    """Rows of no tokens, one token, page ends, all pages on the host, many splits."""
+def test_attend_ragged_tiers_and_splits(counters, page, group, host_every, dtype):
+    """Rows of no tokens, one token, page ends, all pages on the host, rows over several CTAs."""
     lens = [0, 1, 777, 64, 500, 2049, 0, 333]
-    got, ref, tol = _attend(8, 8, 2, page, group, lens, dtype, split, split=split, host_every=host_every, counters=counters)
+    got, ref, tol = _attend(8, 8, 2, page, group, lens, dtype, page + group, host_every=host_every, counters=counters)
     assert ((got - ref).abs() <= tol).all()
     assert not got[0].any() and not got[6].any()
 
@@ -267,16 +269,18 @@ def test_attend_long_row_and_strided_query():
     assert ((got - ref).abs() <= tol).all()
 
 
-def test_attend_cuts_rows_at_max_seq_len():
-    got, ref, tol = _attend(2, 4, 2, 16, 32, [300, 90], torch.float16, 8, max_seq_len=100, split=64)
+@pytest.mark.parametrize("max_seq_len", [1, 100, 513, 700])
+def test_attend_cuts_rows_at_max_seq_len(max_seq_len):
+    got, ref, tol = _attend(2, 4, 2, 16, 32, [800, 90], torch.float16, 8, max_seq_len=max_seq_len)
     assert ((got - ref).abs() <= tol).all()
 
 
 @pytest.mark.parametrize("spread,q_scale", [(1e-4, 1.0), (300.0, 1e-3), (1.0, 200.0), (30.0, 30.0), (1e-4, 3e4)])
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_attend_large_and_small_values(spread, q_scale, dtype):
+@pytest.mark.parametrize("wide", [False, True])
+def test_attend_large_and_small_values(spread, q_scale, dtype, wide):
     """Tiny V scales (float16 subnormals after the weights), one-hot softmax, large q."""
-    got, ref, tol = _attend(2, 5, 1, 32, 64, [400, 33], dtype, 11, split=128, spread=spread, q_scale=q_scale)
+    got, ref, tol = _attend(2, 5, 1, 32, 64, [400, 33], dtype, 11, wide=wide, spread=spread, q_scale=q_scale)
     fine = torch.isfinite(ref)  # 3e4 takes some float16 queries to infinity: no reference there
     assert fine.any() and (fine.all() or (dtype == torch.float16 and q_scale == 3e4))
     assert torch.isfinite(got[fine]).all()
@@ -335,10 +339,10 @@ def test_attend_same_bits_with_counters_and_every_time():
     q = torch.randn(2, 16, D, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).cuda()
     table, lens = torch.arange(40, dtype=torch.int32, device="cuda").view(2, 20), _i32([1280, 901])
     cnt = torch.zeros(kv4.merge_counter_count(2, 16, 2), dtype=torch.int32, device="cuda")
-    first = kv4.decode_paged_q4(q, pool, None, table, lens, 0.09, 128)
+    first = kv4.decode_paged_q4(q, pool, None, table, lens, 0.09)
     for _ in range(5):
-        assert torch.equal(kv4.decode_paged_q4(q, pool, None, table, lens, 0.09, 128, merge_counters=cnt), first)
-        assert torch.equal(kv4.decode_paged_q4(q, pool, None, table, lens, 0.09, 128), first)
+        assert torch.equal(kv4.decode_paged_q4(q, pool, None, table, lens, 0.09, merge_counters=cnt), first)
+        assert torch.equal(kv4.decode_paged_q4(q, pool, None, table, lens, 0.09), first)
 
 
 def test_attend_refusals():
@@ -353,19 +357,41 @@ def test_attend_refusals():
                      (dict(pool_host=torch.zeros(1, 1, pool.shape[2], dtype=torch.uint8).pin_memory()), "share"),
                      (dict(block_table=table.long()), "int32"), (dict(block_table=table[:1]), "one row"),
                      (dict(seq_lens=lens.cpu()), "seq_lens"), (dict(seq_lens=lens[:1]), "seq_lens"),
-                     (dict(max_seq_len=33), "max_seq_len"), (dict(split_size=32), "64"), (dict(split_size=0), "positive"),
+                     (dict(max_seq_len=33), "max_seq_len"), (dict(max_seq_len=0), "max_seq_len"),
                      (dict(out=torch.empty(2, 4, D, device="cuda")), "out"),
-                     (dict(split_size=64, max_seq_len=32, merge_counters=None, query=q[:, :, :].transpose(0, 1).contiguous()
-                           .transpose(0, 1)[:, :, :], out=torch.empty(2, 4, 2 * D, dtype=torch.float16, device="cuda")[..., ::2]),
-                      "contiguous")):
+                     (dict(out=torch.empty(2, 4, 2 * D, dtype=torch.float16, device="cuda")[..., ::2]), "contiguous"),
+                     (dict(query=torch.zeros(2, 4, 2 * D + 4, dtype=torch.float16, device="cuda")[..., :D]), "strides"),
+                     (dict(out=torch.empty(8 * D + 4, dtype=torch.float16, device="cuda")[4:].view(2, 4, D)), "aligned")):
         with pytest.raises(RuntimeError, match=msg):
             kv4.decode_paged_q4(**{**ok, **bad})
-    big = dict(ok, block_table=_i32([[0] * 8, [0] * 8]), split_size=64)
-    for bad, msg in ((dict(partial_o=torch.empty(10, device="cuda")), "partial_o"),
-                     (dict(partial_ml=torch.empty(2, 4, 2, 2, device="cuda", dtype=torch.float16)), "partial_ml"),
+    big = dict(ok, block_table=_i32([[0] * 40, [0] * 40]))
+    for bad, msg in ((dict(scratch=torch.empty(10, device="cuda")), "scratch"),
+                     (dict(scratch=torch.empty(10**6, device="cuda", dtype=torch.float16)), "scratch"),
                      (dict(merge_counters=torch.zeros(3, dtype=torch.int32, device="cuda")), "merge_counters")):
         with pytest.raises(RuntimeError, match=msg):
             kv4.decode_paged_q4(**{**big, **bad})
+
+
+def test_attend_many_rows_and_dealt_ranges():
+    """More rows than CTAs, ranges that begin and end within rows, given scratch."""
+    kv4 = _kv4()
+    g = torch.Generator().manual_seed(40)
+    B, Hq, Hkv, page = 150, 24, 4, 16
+    lens = torch.randint(0, 200, (B,), generator=g)
+    lens[::7] = 0
+    lens[5], lens[149] = 1500, 700
+    pages = -(-lens // page)
+    pool = random_pool(97, Hkv, page, 64, 41)
+    table = torch.randint(0, 97, (B, int(pages.max())), generator=g)  # shared pages
+    q = torch.randn(B, Hq, D, generator=g).to(torch.bfloat16)
+    scratch = torch.full((kv4.scratch_floats(B, Hq, Hkv, page, 64, 16 * table.shape[1]),), float("nan"), device="cuda")
+    ref = attend64(q, (pool, None), page, 64, table, lens, 0.088)
+    k_abs, v_range = values(*parts(pool, page, 64)[:2]).abs().amax(), 15 * parts(pool, page, 64)[3][..., 0].double().amax()
+    for cnt in (None, torch.zeros(kv4.merge_counter_count(B, Hq, Hkv), dtype=torch.int32, device="cuda")):
+        got = kv4.decode_paged_q4(q.cuda(), pool.cuda(), None, table.int().cuda(), lens.int().cuda(), 0.088, scratch=scratch,
+                                  merge_counters=cnt)
+        assert ((got.cpu().double() - ref).abs() <= _bound(ref, q, k_abs, v_range, 0.088, torch.bfloat16)).all()
+        assert cnt is None or not cnt.any()
 
 
 # ---------------------------------------------------------------- together
@@ -397,7 +423,7 @@ def test_prompt_then_steps_in_a_graph_on_another_stream(dtype):
 
     def step():
         kv4.rope_kv_append_q4(qkv, where, inv_d, Hq, q_buf, dev, host, tab)
-        kv4.decode_paged_q4(q_buf, dev, host, tab, lens, 0.088, 64, out=out, merge_counters=cnt)
+        kv4.decode_paged_q4(q_buf, dev, host, tab, lens, 0.088, out=out, merge_counters=cnt)
         where.add_(1)
         lens.add_(1)
 

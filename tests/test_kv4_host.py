@@ -71,25 +71,33 @@ def test_cache_refusals(bad, status, msg):
     (dict(num_q_heads=0), _lib.DAK_ERR_INVALID_ARG, "multiple of kv_heads"),
     (dict(max_seq_len=33), _lib.DAK_ERR_INVALID_ARG, "max_seq_len"),
     (dict(max_seq_len=0), _lib.DAK_ERR_INVALID_ARG, "max_seq_len"),
-    (dict(split_size=100), _lib.DAK_ERR_INVALID_ARG, "multiple of 64"),
     (dict(query=None), _lib.DAK_ERR_INVALID_ARG, "query"),
     (dict(q_stride_h=100), _lib.DAK_ERR_ALIGNMENT, "strides"),
+    (dict(o_stride_b=513), _lib.DAK_ERR_ALIGNMENT, "strides"),
+    (dict(out=BUF + 2), _lib.DAK_ERR_ALIGNMENT, "aligned"),
 ])
 def test_attention_refusals(bad, status, msg):
     a = _lib.AttnQ4Args()
     for k, v in {**dict(query=BUF, q_stride_b=512, q_stride_h=128, seq_lens=BUF, out=BUF, o_stride_b=512, o_stride_h=128,
-                        num_q_heads=4, max_seq_len=32, split_size=64, scaling=0.1, dtype=_lib.DTYPE_F16), **bad}.items():
+                        num_q_heads=4, max_seq_len=32, scaling=0.1, dtype=_lib.DTYPE_F16), **bad}.items():
         setattr(a, k, v)
     st, text = _status(_lib.LIB.dak_attn_decode_paged_q4, ctypes.byref(_cache()), ctypes.byref(a), None)
     assert st == status and msg in text, text
 
 
-def test_attention_needs_scratch_for_splits():
+def test_attention_scratch():
+    """None for short rows that fit the GPU at once, else two slots of 8 heads for
+    every CTA; a call with less is refused."""
     c = _cache()
-    c.max_pages = c.table_stride = 8
+    assert _lib.LIB.dak_attn_q4_scratch(ctypes.byref(c), 4, 32) == 0 == kv4.scratch_floats(3, 4, 2, 16, 32, 32)
+    assert _lib.LIB.dak_attn_q4_scratch(ctypes.byref(c), 5, 32) < 0
+    assert kv4.scratch_floats(1, 8, 1, 64, 128, 513) == 2 * 2 * 8 * 130  # 9 chunks: 2 CTAs of 6 warps
+    sms = _lib.constants().num_sms
+    assert kv4.scratch_floats(64, 64, 8, 64, 128, 16384) == 2 * 2 * sms * 8 * 130  # two CTAs per SM
+    c.max_pages = c.table_stride = 64
     a = _lib.AttnQ4Args()
     for k, v in dict(query=BUF, q_stride_b=512, q_stride_h=128, seq_lens=BUF, out=BUF, o_stride_b=512, o_stride_h=128,
-                     num_q_heads=4, max_seq_len=128, split_size=64, scaling=0.1, dtype=_lib.DTYPE_F16).items():
+                     num_q_heads=4, max_seq_len=1000, scaling=0.1, dtype=_lib.DTYPE_F16, scratch=BUF, scratch_floats=100).items():
         setattr(a, k, v)
     st, text = _status(_lib.LIB.dak_attn_decode_paged_q4, ctypes.byref(c), ctypes.byref(a), None)
     assert st == _lib.DAK_ERR_INVALID_ARG and "scratch" in text
