@@ -106,6 +106,14 @@ class KvAppendArgs(ctypes.Structure):
     ]
 
 
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_vp), ("x_stride_t", c_i64), ("x_stride_h", c_i64), ("positions", c_vp), ("inv_freq", c_vp),
+        ("out", c_vp), ("o_stride_t", c_i64), ("o_stride_h", c_i64), ("tokens", c_int), ("heads", c_int),
+        ("head_dim", c_int), ("rotary_dim", c_int), ("interleaved", c_int), ("rope_scale", ctypes.c_float), ("dtype", c_int),
+    ]
+
+
 class Kv4Cache(ctypes.Structure):
     _fields_ = [
         ("pool_dev", c_vp), ("dev_pages", c_i64), ("pool_host", c_vp), ("host_pages", c_i64),
@@ -162,8 +170,7 @@ SIGNATURES = {
     "dak_rope_qk": (c_int, [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_vp]),
     "dak_silu_mul": (c_int, [c_vp, c_i64, c_vp, c_int, c_int, c_int, c_vp]),
     "dak_attn_decode_noalloc": (c_int, [ctypes.POINTER(AttnDecodeArgs), c_vp]),
-    "dak_rotary": (c_int, [c_vp, c_i64, c_i64, c_vp, c_vp, ctypes.c_float, c_int, c_vp, c_i64, c_i64, c_int, c_int,
-                           c_int, c_int, c_int, c_vp]),
+    "dak_rotary": (c_int, [ctypes.POINTER(RotaryArgs), c_vp]),
     "dak_rope_kv_append_q4": (c_int, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4AppendArgs), c_vp]),
     "dak_kv_read_q4": (c_int, [ctypes.POINTER(Kv4Cache), c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_vp]),
     "dak_attn_decode_paged_q4": (c_int, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(AttnQ4Args), c_vp]),

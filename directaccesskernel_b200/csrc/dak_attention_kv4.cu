@@ -27,7 +27,7 @@ constexpr int kQ4Heads = 8;    // query heads per CTA: the MMA's N
 constexpr int kQ4Chunk = 64;   // tokens a warp takes at a time
 constexpr int kQ4Stages = 2;   // chunks in flight per warp
 constexpr int kQ4PerSm = 2;    // CTAs per SM
-constexpr int kQ4MergeWarps = 4;
+constexpr int kQ4MergeBatch = 8;  // pieces of a row read at once
 constexpr int kQ4RowChunks = 8;  // rows up to this long are not split while the GPU holds them all
 
 struct alignas(64) AttnQ4Params {
@@ -38,7 +38,7 @@ struct alignas(64) AttnQ4Params {
   uint16_t *out;
   long long o_stride_b, o_stride_h;
   const int32_t *seq_lens;
-  float *scratch;     // 2 slots per CTA of [heads][128] outputs, then of [heads][2] (m, l)
+  float *scratch;     // 2 slots per CTA: outputs (kQ4Frags float4 each), then (m, l) of the heads
   int32_t *counters;  // [rows]: the CTA that finishes a split row last merges it (nullptr: merge kernel)
   int num_q_heads, group, block_heads, head_blocks;  // group: query heads per KV head
   int max_seq_len;
@@ -132,12 +132,26 @@ __device__ __forceinline__ float exponent_of(uint32_t bits) {
   return fmaxf((float)((int)(__float_as_uint(s) >> 23) - 127), -24.f);
 }
 
-// Dims 4 lane .. + 3 of a head's output; zeros where no weight was summed.
-template <typename T>
-__device__ __forceinline__ void store_out(const AttnQ4Params &p, int b, int h, int lane, float4 v, float den) {
-  const float r = den == 0.f ? 0.f : 1.f / den;
-  *reinterpret_cast<uint2 *>(p.out + b * p.o_stride_b + h * p.o_stride_h + 4 * lane) =
-      make_uint2(Elem<T>::pack2(v.x * r, v.y * r), Elem<T>::pack2(v.z * r, v.w * r));
+// Outputs are added up and kept in scratch in the MMA's own layout, 256 float4 of
+// a row: number i holds, for c = i % 4, g = i / 4 % 8 and t = i / 32, dims d, d + 1
+// of heads 2c and 2c + 1 as (d, 2c), (d, 2c + 1), (d + 1, 2c), (d + 1, 2c + 1), d
+// being frag_dim.  Every step is then linear in the thread.
+constexpr int kQ4Frags = kQ4Heads * kKv4Dim / 4;
+template <int NG> __device__ __forceinline__ int frag_dim(int t, int g) {
+  const int q = t >> 1;
+  return (NG == 1 ? 16 * g + 4 * q : NG == 2 ? 64 * (q >> 1) + 8 * g + 4 * (q & 1) : 32 * q + 4 * g) + 2 * (t & 1);
+}
+
+// Writes float4 i of a row's output over its denominators; zeros where no weight
+// was summed.
+template <typename T, int NG>
+__device__ __forceinline__ void store_frag(const AttnQ4Params &p, int b, int h0, int nh, int i, float4 v, float den0,
+                                           float den1) {
+  const int h = 2 * (i & 3);
+  uint16_t *to = p.out + b * p.o_stride_b + (h0 + h) * p.o_stride_h + frag_dim<NG>(i >> 5, (i >> 2) & 7);
+  const float r0 = den0 == 0.f ? 0.f : 1.f / den0, r1 = den1 == 0.f ? 0.f : 1.f / den1;
+  if (h < nh) *reinterpret_cast<uint32_t *>(to) = Elem<T>::pack2(v.x * r0, v.z * r0);
+  if (h + 1 < nh) *reinterpret_cast<uint32_t *>(to + p.o_stride_h) = Elem<T>::pack2(v.y * r1, v.w * r1);
 }
 
 __device__ __forceinline__ int seq_of(const AttnQ4Params &p, int b) {
@@ -151,54 +165,48 @@ __device__ __forceinline__ int range_of(const AttnQ4Params &p, int total) {
   return max((total + p.ctas - 1) / p.ctas, p.warps);
 }
 
-// Sum of the batch's chunks per (KV head, head block), by one warp.
-__device__ __forceinline__ int batch_chunks(const AttnQ4Params &p) {
-  int n = 0;
-  for (int b = lane_id(); b < p.c.rows; b += 32) n += chunks_of(seq_of(p, b));
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) n += __shfl_xor_sync(0xffffffffu, n, x);
-  return n;
-}
-
-// Where row (b, r) ended up in the scratch: its chunks are [begin, end) of all, in
-// ranges of `per`.  Piece i is CTA i's first segment (slot 2 i), or, if the row
-// begins within CTA i's range, its last (slot 2 i + 1).  One warp per head sums
-// the pieces in order, 4 dims per lane.
-template <typename T>
-__device__ __forceinline__ void merge_row(const AttnQ4Params &p, int b, int h0, int nh, int begin, int end, int per, int warps) {
-  const int first = begin / per, pieces = (end - 1) / per - first + 1, lane = lane_id();
-  const float *po = p.scratch;
-  const float2 *pm = reinterpret_cast<const float2 *>(p.scratch + 2ll * p.ctas * kQ4Heads * kKv4Dim);
-  auto slot = [&](int i) { return 2 * (first + i) + ((first + i) * per < begin ? 1 : 0); };
-  for (int h = warp_id(); h < nh; h += warps) {
-    float2 mine = make_float2(-FLT_MAX, 0.f);
-    float gm = -FLT_MAX;
-    for (int i = lane; i < pieces; i += 32) {
-      const float2 v = __ldcg(pm + (long long)slot(i) * kQ4Heads + h);
-      if (i == lane) mine = v;
-      gm = fmaxf(gm, v.x);
-    }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, x));
-    float den = 0.f;
+// Merges row (b, r), whose chunks are [begin, end) of all in ranges of `per`, from
+// its pieces in the scratch, in order.  Piece i is CTA i's first segment (slot
+// 2 i), or, if the row begins within CTA i's range, its last (slot 2 i + 1).
+template <typename T, int NG>
+__device__ __forceinline__ void merge_row(const AttnQ4Params &p, int b, int h0, int nh, int begin, int end, int per,
+                                          int threads) {
+  const int first = begin / per, pieces = (end - 1) / per - first + 1;
+  const float4 *po = reinterpret_cast<const float4 *>(p.scratch);
+  const float4 *pm = po + 2ll * p.ctas * kQ4Frags;  // (m, l) of two heads
+  auto slot = [&](int i) { return 2ll * (first + i) + ((first + i) * per < begin ? 1 : 0); };
+  for (int k = threadIdx.x; k < kQ4Frags; k += threads) {
+    float m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = 0; i0 < pieces; i0 += 32) {
-      if (i0 > 0 && i0 + lane < pieces) mine = __ldcg(pm + (long long)slot(i0 + lane) * kQ4Heads + h);
-      const float c = i0 + lane < pieces ? ex2(mine.x - gm) : 0.f;
-      const float lc = i0 + lane < pieces ? mine.y * c : 0.f;
-      const int n = min(32, pieces - i0);
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) {
-        const float ci = __shfl_sync(0xffffffffu, c, i);
-        den += __shfl_sync(0xffffffffu, lc, i);
-        const float4 v = __ldcg(reinterpret_cast<const float4 *>(po + ((long long)slot(i0 + i) * kQ4Heads + h) * kKv4Dim) + lane);
-        acc.x = fmaf(v.x, ci, acc.x);
-        acc.y = fmaf(v.y, ci, acc.y);
-        acc.z = fmaf(v.z, ci, acc.z);
-        acc.w = fmaf(v.w, ci, acc.w);
+    for (int i0 = 0; i0 < pieces; i0 += kQ4MergeBatch) {
+      float4 ml[kQ4MergeBatch], v[kQ4MergeBatch];  // all in flight at once
+#pragma unroll
+      for (int i = 0; i < kQ4MergeBatch; ++i) {
+        const bool in = i0 + i < pieces;
+        const long long at = slot(in ? i0 + i : i0);
+        ml[i] = __ldcg(pm + at * (kQ4Heads / 2) + (k & 3));
+        v[i] = __ldcg(po + at * kQ4Frags + k);
+        if (!in) ml[i] = make_float4(-FLT_MAX, 0.f, -FLT_MAX, 0.f), v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float n0 = m0, n1 = m1;
+#pragma unroll
+      for (int i = 0; i < kQ4MergeBatch; ++i) n0 = fmaxf(n0, ml[i].x), n1 = fmaxf(n1, ml[i].z);
+      const float a0 = ex2(m0 - n0), a1 = ex2(m1 - n1);
+      m0 = n0, m1 = n1;
+      l0 *= a0, l1 *= a1;
+      acc = make_float4(acc.x * a0, acc.y * a1, acc.z * a0, acc.w * a1);
+#pragma unroll
+      for (int i = 0; i < kQ4MergeBatch; ++i) {
+        const float c0 = ex2(ml[i].x - m0), c1 = ex2(ml[i].z - m1);
+        l0 = fmaf(ml[i].y, c0, l0);
+        l1 = fmaf(ml[i].w, c1, l1);
+        acc.x = fmaf(v[i].x, c0, acc.x);
+        acc.y = fmaf(v[i].y, c1, acc.y);
+        acc.z = fmaf(v[i].z, c0, acc.z);
+        acc.w = fmaf(v[i].w, c1, acc.w);
       }
     }
-    store_out<T>(p, b, h0 + h, lane, acc, den);
+    store_frag<T, NG>(p, b, h0, nh, k, acc, l0, l1);
   }
 }
 
@@ -231,32 +239,45 @@ __global__ void __launch_bounds__(Q4Smem<NG>::threads, kQ4PerSm) attn_q4_kernel(
   // This CTA's range of chunks [lo, hi) and the row (b0, r0) that it begins in,
   // whose chunks begin at `begin`.
   const int R = p.c.kv_heads * p.head_blocks;
-  int lo, hi, begin, b0, r0, per = 0;
+  int lo, hi, begin, b0, r0, seq0, per = 0;
+  const float4 nothing = make_float4(0.f, 0.f, 0.f, 0.f);
   if (p.by_row) {
     b0 = blockIdx.x / R;
     r0 = blockIdx.x - b0 * R;
     lo = begin = 0;
-    hi = chunks_of(seq_of(p, b0));
-    if (hi == 0) {  // threads 0..nh-1 x 32 lanes would do; the block is small
-      const int h0 = r0 / p.head_blocks * p.group + r0 % p.head_blocks * p.block_heads;
-      const int nh = min(p.block_heads, p.group - r0 % p.head_blocks * p.block_heads);
-      for (int h = warp; h < nh; h += W) store_out<T>(p, b0, h0 + h, lane, make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
+    seq0 = seq_of(p, b0);
+    hi = chunks_of(seq0);
+    if (hi == 0) {
+      const int hb = r0 % p.head_blocks;
+      for (int k = threadIdx.x; k < kQ4Frags; k += S::threads)
+        store_frag<T, NG>(p, b0, r0 / p.head_blocks * p.group + hb * p.block_heads,
+                          min(p.block_heads, p.group - hb * p.block_heads), k, nothing, 0.f, 0.f);
       return;
     }
   } else {
+    // Lengths of the first 32 sequences, one per lane; most batches need no more.
+    int seqs = lane < p.c.rows ? seq_of(p, lane) : 0;
+    int n = chunks_of(seqs), total = n;
+    for (int b = 32 + lane; b < p.c.rows; b += 32) total += chunks_of(seq_of(p, b));
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+    total *= R;
     for (int b = blockIdx.x; b < p.c.rows; b += p.ctas)  // sequences of no tokens belong to no range
       if (seq_of(p, b) == 0)
-        for (int h = warp; h < p.num_q_heads; h += W) store_out<T>(p, b, h, lane, make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
-    const int total = batch_chunks(p) * R;
+        for (int h = 0; h < p.num_q_heads; h += kQ4Heads)
+          for (int k = threadIdx.x; k < kQ4Frags; k += S::threads)
+            store_frag<T, NG>(p, b, h, p.num_q_heads - h, k, nothing, 0.f, 0.f);
     per = range_of(p, total);
     if ((long long)blockIdx.x * per >= total) return;
     lo = blockIdx.x * per;
     hi = min(total, lo + per);
     int before = 0;  // chunks of the sequences before this block of 32
-    b0 = r0 = begin = 0;
     for (int base = 0;; base += 32) {
-      const int n = base + lane < p.c.rows ? chunks_of(seq_of(p, base + lane)) * R : 0;
-      int incl = n;
+      if (base > 0) {
+        seqs = base + lane < p.c.rows ? seq_of(p, base + lane) : 0;
+        n = chunks_of(seqs);
+      }
+      int incl = n * R;
 #pragma unroll
       for (int x = 1; x < 32; x <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, incl, x);
@@ -264,23 +285,45 @@ __global__ void __launch_bounds__(Q4Smem<NG>::threads, kQ4PerSm) attn_q4_kernel(
       }
       const uint32_t past = __ballot_sync(0xffffffffu, before + incl > lo);
       if (past) {
-        const int at = __ffs(past) - 1;
-        const int seq_n = __shfl_sync(0xffffffffu, n, at);
-        const int seq_begin = before + __shfl_sync(0xffffffffu, incl, at) - seq_n;
-        b0 = base + at;
-        r0 = (lo - seq_begin) / (seq_n / R);
-        begin = seq_begin + r0 * (seq_n / R);
+        const int l0 = __ffs(past) - 1, row_n = __shfl_sync(0xffffffffu, n, l0);
+        const int seq_begin = before + __shfl_sync(0xffffffffu, incl, l0) - row_n * R;
+        b0 = base + l0;
+        r0 = (lo - seq_begin) / row_n;
+        begin = seq_begin + r0 * row_n;
+        seq0 = __shfl_sync(0xffffffffu, seqs, l0);
         break;
       }
       before += __shfl_sync(0xffffffffu, incl, 31);
     }
   }
 
+  // Word w (0..3) of a K row that this lane multiplies, 8 dims each: all the
+  // words of one group meet in the same MMA steps.
+  auto k_word = [&](int w) {
+    return NG == 1 ? 4 * cq + w : NG == 2 ? 8 * (w >> 1) + 2 * cq + (w & 1) : 4 * w + cq;
+  };
+  // Query words of head g of a row, as they are; used when the row's turn comes.
+  uint4 qraw[4];
+  auto heads_of = [&](int r, int &h0, int &nh) {
+    const int hb = r % p.head_blocks;
+    h0 = r / p.head_blocks * p.group + hb * p.block_heads;
+    nh = min(p.block_heads, p.group - hb * p.block_heads);
+  };
+  auto fetch_query = [&](int b, int r) {
+    int h0, nh;
+    heads_of(r, h0, nh);
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      qraw[w] = g < nh ? *reinterpret_cast<const uint4 *>(p.query + b * p.q_stride_b + (h0 + g) * p.q_stride_h + 8 * k_word(w))
+                       : make_uint4(0u, 0u, 0u, 0u);
+  };
+  fetch_query(b0, r0);
+
   // Copies, ahead of the arithmetic: this warp takes chunks lo + warp, + 4, ...
   // The position (row, table entries) of the copy after next is worked out while
   // the chunks in flight are multiplied.
   const uint64_t pol = l2_policy_evict_first();
-  int at = lo + warp, at_b = b0, at_r = r0, at_begin = begin, at_seq = seq_of(p, b0), at_n = chunks_of(at_seq);
+  int at = lo + warp, at_b = b0, at_r = r0, at_begin = begin, at_seq = seq0, at_n = chunks_of(at_seq);
   int entry = 0, pages = 0, issued = 0;
   auto locate = [&]() {
     if (at >= hi) return;
@@ -319,25 +362,18 @@ __global__ void __launch_bounds__(Q4Smem<NG>::threads, kQ4PerSm) attn_q4_kernel(
   for (int j = 0; j < kQ4Stages; ++j)
     if (at < hi) issue();
 
-  // Word w (0..3) of a K row that this lane multiplies, 8 dims each: all the
-  // words of one group meet in the same MMA steps.
-  auto k_word = [&](int w) {
-    return NG == 1 ? 4 * cq + w : NG == 2 ? 8 * (w >> 1) + 2 * cq + (w & 1) : 4 * w + cq;
-  };
   // Query of head g: scaled by a power of two to below 2^14 and to float16 (the
   // values that float16 cannot hold are 2^-38 of the largest), and summed
   // over each group for the zeros' share.
   uint32_t qf[8][2];
   float qs[2][NG], f[2];
-  auto load_query = [&](int b, int h0, int nh) {
+  auto ready_query = [&]() {
     float x[4][8], mx = 0.f, sum[NG];
 #pragma unroll
     for (int n = 0; n < NG; ++n) sum[n] = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (g < nh)
-        v = *reinterpret_cast<const uint4 *>(p.query + b * p.q_stride_b + (h0 + g) * p.q_stride_h + 8 * k_word(w));
+      const uint4 v = qraw[w];
       const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -617,23 +653,15 @@ __global__ void __launch_bounds__(Q4Smem<NG>::threads, kQ4PerSm) attn_q4_kernel(
   };
 
   float *sm_m = reinterpret_cast<float *>(smem + S::m_off), *sm_l = reinterpret_cast<float *>(smem + S::l_off);
-  float *sm_o = reinterpret_cast<float *>(smem + S::o_off);
+  float4 *sm_o = reinterpret_cast<float4 *>(smem + S::o_off);
   int done = 0, dead_at = -1;  // chunks taken; the chunk whose copy never came
-  int b = b0, r = r0, seq = seq_of(p, b0), n = chunks_of(seq);
+  int b = b0, r = r0, seq = seq0, n = chunks_of(seq0);
   for (int s0 = lo; s0 < hi;) {
     // The segment [s0, s1) of row (b, r), whose chunks begin at `begin`.
-    while (s0 >= begin + n) {
-      begin += n;
-      if (n == 0 || ++r == R) {
-        r = 0;
-        seq = seq_of(p, ++b);
-        n = chunks_of(seq);
-      }
-    }
     const int s1 = min(hi, begin + n);
-    const int hb = r % p.head_blocks, h0 = r / p.head_blocks * p.group + hb * p.block_heads;
-    const int nh = min(p.block_heads, p.group - hb * p.block_heads);
-    load_query(b, h0, nh);
+    int h0, nh;
+    heads_of(r, h0, nh);
+    ready_query();
 #pragma unroll
     for (int t = 0; t < 8; ++t)
 #pragma unroll
@@ -659,6 +687,21 @@ __global__ void __launch_bounds__(Q4Smem<NG>::threads, kQ4PerSm) attn_q4_kernel(
       if (at < hi) issue();
     }
 
+    // The row after this one, and its query.
+    const bool whole = s0 == begin && s1 == begin + n;
+    const int row_b = b, row_r = r, row_begin = begin, row_end = begin + n;
+    if (s1 < hi) {
+      begin = s1;
+      if (++r == R) {
+        r = 0;
+        do {
+          seq = seq_of(p, ++b);
+        } while (seq == 0);  // there is one: the range goes on
+        n = chunks_of(seq);
+      }
+      fetch_query(b, r);
+    }
+
     // Add up the warps: statistics first, then each warp its share in turn.
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -670,73 +713,64 @@ __global__ void __launch_bounds__(Q4Smem<NG>::threads, kQ4PerSm) attn_q4_kernel(
       }
     }
     __syncthreads();
-    float c[2];
+    float gm[2], even[2], odd[2];  // heads 2 cq, 2 cq + 1
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int h = 2 * cq + e;
-      float gm = sm_m[h];
+      gm[e] = sm_m[2 * cq + e];
 #pragma unroll
-      for (int w = 1; w < W; ++w) gm = fmaxf(gm, sm_m[w * kQ4Heads + h]);
-      c[e] = ex2(m[e] - gm);
+      for (int w = 1; w < W; ++w) gm[e] = fmaxf(gm[e], sm_m[w * kQ4Heads + 2 * cq + e]);
+      even[e] = ex2(m[e] - gm[e]) * 0x1p24f;
+      odd[e] = ex2(m[e] - gm[e]) * 0x1p20f;
     }
     const int live = min(W, s1 - s0);  // warps that had a chunk of this segment
     for (int turn = 0; turn < live; ++turn) {
-      // Chunk s0 + turn is this warp's.
-      if ((s0 - lo + turn) % W == warp) {
+      if ((s0 - lo + turn) % W == warp) {  // chunk s0 + turn is this warp's
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int h = 2 * cq + e;
-          if (h >= nh) continue;
-#pragma unroll
-          for (int t = 0; t < 8; ++t) {
-            const int q = t >> 1;
-            const int d =
-                (NG == 1 ? 16 * g + 4 * q : NG == 2 ? 64 * (q >> 1) + 8 * g + 4 * (q & 1) : 32 * q + 4 * g) + 2 * (t & 1);
-            float2 *to = reinterpret_cast<float2 *>(sm_o + h * kKv4Dim + d);
-            float2 v = turn == 0 ? make_float2(0.f, 0.f) : *to;
-            v.x = fmaf(o[t][e] * 0x1p24f, c[e], v.x);
-            v.y = fmaf(o[t][2 + e] * 0x1p20f, c[e], v.y);
-            *to = v;
-          }
+        for (int t = 0; t < 8; ++t) {
+          float4 v = turn == 0 ? nothing : sm_o[t * 32 + lane];
+          v.x = fmaf(o[t][0], even[0], v.x);
+          v.y = fmaf(o[t][1], even[1], v.y);
+          v.z = fmaf(o[t][2], odd[0], v.z);
+          v.w = fmaf(o[t][3], odd[1], v.w);
+          sm_o[t * 32 + lane] = v;
         }
       }
       __syncthreads();
     }
-    // A warp per head: the output, or a piece of it.
-    const bool whole = s0 == begin && s1 == begin + n;
-    for (int h = warp; h < nh; h += W) {
-      float gm = sm_m[h], den = 0.f;
+    float den[2] = {0.f, 0.f};
 #pragma unroll
-      for (int w = 1; w < W; ++w) gm = fmaxf(gm, sm_m[w * kQ4Heads + h]);
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
-      for (int w = 0; w < W; ++w) den = fmaf(sm_l[w * kQ4Heads + h], ex2(sm_m[w * kQ4Heads + h] - gm), den);
-      const float4 v = *reinterpret_cast<const float4 *>(sm_o + h * kKv4Dim + 4 * lane);
-      if (whole) {
-        store_out<T>(p, b, h0 + h, lane, v, den);
-      } else {
-        const long long slot = (2ll * blockIdx.x + (s0 == lo ? 0 : 1)) * kQ4Heads + h;
-        __stcg(reinterpret_cast<float4 *>(p.scratch + slot * kKv4Dim) + lane, v);
-        if (lane == 0)
-          __stcg(reinterpret_cast<float2 *>(p.scratch + 2ll * p.ctas * kQ4Heads * kKv4Dim) + slot, make_float2(gm, den));
-      }
+      for (int w = 0; w < W; ++w)
+        den[e] = fmaf(sm_l[w * kQ4Heads + 2 * cq + e], ex2(sm_m[w * kQ4Heads + 2 * cq + e] - gm[e]), den[e]);
+    // The output, or a piece of it; a thread's float4s are all of heads 2 cq and + 1.
+    const long long slot = 2ll * blockIdx.x + (s0 == lo ? 0 : 1);
+    for (int k = threadIdx.x; k < kQ4Frags; k += S::threads) {
+      if (whole)
+        store_frag<T, NG>(p, row_b, h0, nh, k, sm_o[k], den[0], den[1]);
+      else
+        __stcg(reinterpret_cast<float4 *>(p.scratch) + slot * kQ4Frags + k, sm_o[k]);
     }
+    if (!whole && threadIdx.x < 4)
+      __stcg(reinterpret_cast<float4 *>(p.scratch) + 2ll * p.ctas * kQ4Frags + slot * (kQ4Heads / 2) + cq,
+             make_float4(gm[0], den[0], gm[1], den[1]));
     if (!whole && p.counters) {
       // The CTA that finishes the row last merges it and resets the counter.
       int *last = reinterpret_cast<int *>(smem + S::flag_off + 8);
       __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) {
-        int32_t *counter = p.counters + (long long)b * R + r;
-        *last = atomicAdd(counter, 1) == (begin + n - 1) / per - begin / per;
+        int32_t *counter = p.counters + (long long)row_b * R + row_r;
+        *last = atomicAdd(counter, 1) == (row_end - 1) / per - row_begin / per;
         if (*last) *counter = 0;
       }
       __syncthreads();
       if (*last) {
         __threadfence();
-        merge_row<T>(p, b, h0, nh, begin, begin + n, per, W);
+        merge_row<T, NG>(p, row_b, h0, nh, row_begin, row_end, per, S::threads);
       }
     }
-    __syncthreads();  // the statistics are free again
+    __syncthreads();  // statistics and outputs are free again
     s0 = s1;
   }
   if (dead_at >= 0 && lane == 0) {
@@ -747,8 +781,8 @@ __global__ void __launch_bounds__(Q4Smem<NG>::threads, kQ4PerSm) attn_q4_kernel(
 }
 
 // The merge as a launch of its own, one CTA per row.
-template <typename T>
-__global__ void __launch_bounds__(kQ4MergeWarps * 32) attn_q4_merge_kernel(const __grid_constant__ AttnQ4Params p) {
+template <typename T, int NG>
+__global__ void __launch_bounds__(kQ4Frags) attn_q4_merge_kernel(const __grid_constant__ AttnQ4Params p) {
   pdl_enter(p.pdl);
   const int R = p.c.kv_heads * p.head_blocks;
   const int b = blockIdx.x / R, r = blockIdx.x - b * R;
@@ -767,8 +801,8 @@ __global__ void __launch_bounds__(kQ4MergeWarps * 32) attn_q4_merge_kernel(const
   const int per = range_of(p, total * R), begin = before * R + r * n;
   if (n == 0 || begin / per == (begin + n - 1) / per) return;  // written already
   const int hb = r % p.head_blocks;
-  merge_row<T>(p, b, r / p.head_blocks * p.group + hb * p.block_heads, min(p.block_heads, p.group - hb * p.block_heads), begin,
-               begin + n, per, kQ4MergeWarps);
+  merge_row<T, NG>(p, b, r / p.head_blocks * p.group + hb * p.block_heads, min(p.block_heads, p.group - hb * p.block_heads),
+                   begin, begin + n, per, kQ4Frags);
 }
 
 template <typename T, int NG, int P>
@@ -778,7 +812,7 @@ cudaError_t launch_attn(const AttnQ4Params &p, int rows, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   e = launch_ex(kern, dim3(p.ctas), dim3(Q4Smem<NG>::threads), Q4Smem<NG>::bytes, s, 1, p.pdl != 0, p);
   if (e != cudaSuccess || p.by_row || p.counters) return e;
-  return launch_ex(attn_q4_merge_kernel<T>, dim3(rows), dim3(kQ4MergeWarps * 32), 0, s, 1, p.pdl != 0, p);
+  return launch_ex(attn_q4_merge_kernel<T, NG>, dim3(rows), dim3(kQ4Frags), 0, s, 1, p.pdl != 0, p);
 }
 
 template <typename T, int NG>

@@ -62,6 +62,7 @@ int kv4_view(const dak_kv4_cache *a, Kv4Cache *out) {
   c.rows = a->batch;
   c.kv_heads = a->kv_heads;
   c.page_size = a->page_size;
+  c.page_log2 = a->page_size == 16 ? 4 : a->page_size == 32 ? 5 : 6;
   c.status = device_status_word();
   if (!c.status) return fail(DAK_ERR_CUDA, "no device status word");
   return DAK_OK;
@@ -71,6 +72,8 @@ namespace {
 
 constexpr int kKv4Threads = 256;
 constexpr int kKv4Warps = kKv4Threads / 32;
+constexpr int kAppendWarps = 3500, kReadWarps = 9472;  // for the q heads of a call (and half that for k, v each); for a read
+constexpr int kBatch = 4;  // heads whose loads are in flight at once
 
 struct AppendParams {
   Kv4Cache c;
@@ -137,12 +140,23 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const __grid_co
       const RopeUnit unit = rope_unit(u, p.rotary_dim, p.interleaved);
       float c[8], s[8];
       rope_unit_angles(unit, pos, p.inv_freq, p.scale, c, s);
-      for (int h = role; h < p.q_heads; h += p.q_groups) {
-        const uint4 *src = reinterpret_cast<const uint4 *>(row + h * kKv4Dim);
-        uint4 *dst = reinterpret_cast<uint4 *>(p.q_out + ((long long)t * p.q_heads + h) * kKv4Dim);
-        const uint4 a = src[unit.v0];
-        const uint4 b = unit.v1 >= 0 ? src[unit.v1] : a;
-        rope_unit_apply<T>(unit, p.interleaved, a, b, c, s, dst);
+      for (int h0 = role; h0 < p.q_heads; h0 += kBatch * p.q_groups) {
+        uint4 a[kBatch], b[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const int h = h0 + k * p.q_groups;
+          if (h >= p.q_heads) break;
+          const uint4 *src = reinterpret_cast<const uint4 *>(row + h * kKv4Dim);
+          a[k] = src[unit.v0];
+          b[k] = unit.v1 >= 0 ? src[unit.v1] : a[k];
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const int h = h0 + k * p.q_groups;
+          if (h >= p.q_heads) break;
+          rope_unit_apply<T>(unit, p.interleaved, a[k], b[k], c, s,
+                             reinterpret_cast<uint4 *>(p.q_out + ((long long)t * p.q_heads + h) * kKv4Dim));
+        }
       }
     }
     return;
@@ -153,12 +167,12 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const __grid_co
   int tier = 0;
   uint8_t *page = nullptr;
   if (live) {
-    page = pos < 0 ? nullptr : kv4_page(p.c, p.seq_index ? p.seq_index[t] : t, pos / P, &tier);
+    page = pos < 0 ? nullptr : kv4_page(p.c, p.seq_index ? p.seq_index[t] : t, pos >> p.c.page_log2, &tier);
     if (!page && lane8 == 0) atomicCAS(p.c.status, 0, DAK_ERR_INVALID_ARG);
   }
   const int half = kv4_half_bytes(P, NG);
-  const long long in_slab = (long long)isv * half + (pos % P) * 64;
-  const long long pair_off = (long long)isv * half + P * 64 + (pos % P) * 4 * NG;
+  const long long in_slab = (long long)isv * half + (pos & (P - 1)) * 64;
+  const long long pair_off = (long long)isv * half + P * 64 + (pos & (P - 1)) * 4 * NG;
   // Half layout: dims 16 lane8 .. +15 and, R/2 dims away, their partners; each
   // lane keeps its own side of the pairs.
   const int R = isv ? 0 : p.rotary_dim;
@@ -178,24 +192,39 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const __grid_co
       }
     }
   }
+  // The vectors of this lane and, where they are rotated in halves, their
+  // partners; the next head's are loaded while this one's are packed.
+  const bool paired = !p.interleaved && R > 0;
+  auto head = [&](int h) {
+    return reinterpret_cast<const uint4 *>(row + (long long)(p.q_heads + isv * p.c.kv_heads + h) * kKv4Dim);
+  };
+  auto partner = [&](int v) { return v < part ? v + part : v < 2 * part ? v - part : v; };
+  uint4 own[2], other[2];
+  auto load = [&](int h) {
+    const uint4 *src = head(h);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      own[k] = src[lane8 * 2 + k];
+      other[k] = paired ? src[partner(lane8 * 2 + k)] : own[k];
+    }
+  };
+  load(g);
   for (int h = g; h < p.c.kv_heads; h += p.kv_groups) {
-    const uint4 *src =
-        reinterpret_cast<const uint4 *>(row + (long long)(p.q_heads + isv * p.c.kv_heads + h) * kKv4Dim);
     float x[16];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int v = lane8 * 2 + k;
       float y[8];
-      unpack8<T>(src[v], y);
-      if (!p.interleaved && v < 2 * part) {
+      unpack8<T>(own[k], y);
+      if (paired && lane8 * 2 + k < 2 * part) {
         float z[8];
-        unpack8<T>(src[v < part ? v + part : v - part], z);
+        unpack8<T>(other[k], z);
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = fmaf(y[i], c[8 * k + i], z[i] * s[8 * k + i]);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[8 * k + i] = y[i];
     }
+    if (h + p.kv_groups < p.c.kv_heads) load(h + p.kv_groups);
     if (p.interleaved) {
 #pragma unroll
       for (int i = 0; i < 16; i += 2)
@@ -219,37 +248,51 @@ struct ReadParams {
 template <typename T, int NG>
 __global__ void __launch_bounds__(kKv4Threads) kv4_read_kernel(const __grid_constant__ ReadParams p) {
   pdl_enter(p.pdl);
-  const int roles = 2 * p.groups;
   const long long w = (long long)blockIdx.x * kKv4Warps + warp_id();
-  const int role = (int)(w % roles);
-  const int isv = role >= p.groups ? 1 : 0;
+  const int g = (int)(w % p.groups);
   const int lane8 = lane_id() & 7;
-  const long long t = (w / roles) * 4 + (lane_id() >> 3);
+  const long long t = (w / p.groups) * 4 + (lane_id() >> 3);
   if (t >= p.tokens) return;
   const int P = p.c.page_size;
   const int pos = p.positions[t];
   int tier = 0;
-  const uint8_t *page = pos < 0 ? nullptr : kv4_page(p.c, p.seq_index ? p.seq_index[t] : (int)t, pos / P, &tier);
+  const uint8_t *page =
+      pos < 0 ? nullptr : kv4_page(p.c, p.seq_index ? p.seq_index[t] : (int)t, pos >> p.c.page_log2, &tier);
   if (!page && lane8 == 0) atomicCAS(p.c.status, 0, DAK_ERR_INVALID_ARG);
-  const int half = kv4_half_bytes(P, NG);
-  for (int h = role - isv * p.groups; h < p.c.kv_heads; h += p.groups) {
-    uint2 w2 = make_uint2(0u, 0u);
-    float s = 0.f, z = 0.f;
-    if (page) {
-      const uint8_t *slab = page + (long long)h * p.c.slab_bytes + isv * half;
-      w2 = *reinterpret_cast<const uint2 *>(slab + (pos % P) * 64 + lane8 * 8);
-      const uint32_t sz = *reinterpret_cast<const uint32_t *>(slab + P * 64 + ((pos % P) * NG + lane8 / (8 / NG)) * 4);
-      s = __half2float(__ushort_as_half((unsigned short)(sz & 0xffffu)));
-      z = __half2float(__ushort_as_half((unsigned short)(sz >> 16)));
+  const int half = kv4_half_bytes(P, NG), items = 2 * p.c.kv_heads;  // K rows of all heads, then V rows
+  const int code_at = (pos & (P - 1)) * 64 + lane8 * 8;
+  const int pair_at = P * 64 + ((pos & (P - 1)) * NG + lane8 / (8 / NG)) * 4;
+  for (int i0 = g; i0 < items; i0 += kBatch * p.groups) {
+    uint2 codes[kBatch];
+    uint32_t pair[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int i = i0 + k * p.groups;
+      codes[k] = make_uint2(0u, 0u);
+      pair[k] = 0u;
+      if (i < items && page) {
+        const int isv = i >= p.c.kv_heads;
+        const uint8_t *slab = page + (long long)(i - isv * p.c.kv_heads) * p.c.slab_bytes + isv * half;
+        codes[k] = __ldcs(reinterpret_cast<const uint2 *>(slab + code_at));
+        pair[k] = *reinterpret_cast<const uint32_t *>(slab + pair_at);
+      }
     }
-    uint4 *dst = reinterpret_cast<uint4 *>(p.out[isv] + (t * p.c.kv_heads + h) * kKv4Dim) + lane8 * 2;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const uint32_t word = k ? w2.y : w2.x;
-      float x[8];
+    for (int k = 0; k < kBatch; ++k) {
+      const int i = i0 + k * p.groups;
+      if (i >= items) break;
+      const int isv = i >= p.c.kv_heads;
+      const float s = __half2float(__ushort_as_half((unsigned short)(pair[k] & 0xffffu)));
+      const float z = __half2float(__ushort_as_half((unsigned short)(pair[k] >> 16)));
+      uint4 *dst = reinterpret_cast<uint4 *>(p.out[isv] + (t * p.c.kv_heads + (i - isv * p.c.kv_heads)) * kKv4Dim) + lane8 * 2;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = fmaf(s, (float)((word >> (4 * i)) & 15u), z);
-      dst[k] = pack8<T>(x);
+      for (int v = 0; v < 2; ++v) {
+        const uint32_t word = v ? codes[k].y : codes[k].x;
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = fmaf(s, (float)((word >> (4 * e)) & 15u), z);
+        __stcs(dst + v, pack8<T>(x));
+      }
     }
   }
 }
@@ -272,10 +315,10 @@ cudaError_t launch_read(const ReadParams &p, unsigned grid, cudaStream_t s) {
   }
 }
 
-// Warps for the heads of `quads` token quads: one head per warp until the GPU
-// is full, then more heads per warp.
-int head_groups(long long quads, int heads) {
-  return (int)std::min<long long>(heads, std::max<long long>(1, 9472 / std::max(1ll, quads)));
+// Warps that share `heads` heads of each of `quads` token quads: one head per
+// warp until about `warps` warps fill the GPU, then more heads per warp.
+int head_groups(long long quads, int heads, int warps) {
+  return (int)std::min<long long>(heads, std::max<long long>(1, warps / std::max(1ll, quads)));
 }
 
 int check_tokens(int tokens, const int32_t *positions, const int32_t *seq_index, int batch) {
@@ -327,8 +370,8 @@ extern "C" int dak_rope_kv_append_q4(const dak_kv4_cache *cache, const dak_kv4_a
   p.interleaved = a->interleaved != 0;
   p.units = rope_units(kKv4Dim, a->rotary_dim, p.interleaved);
   const long long quads = (a->tokens + 3ll) / 4;
-  p.q_groups = a->q_heads > 0 ? head_groups(quads, a->q_heads) : 0;
-  p.kv_groups = head_groups(quads, cache->kv_heads);
+  p.q_groups = a->q_heads > 0 ? head_groups(quads, a->q_heads, kAppendWarps) : 0;
+  p.kv_groups = head_groups(quads, cache->kv_heads, kAppendWarps / 2);
   p.pdl = decode_pdl_enabled() ? 1 : 0;
   const long long grid = (quads * (p.q_groups + 2 * p.kv_groups) + kKv4Warps - 1) / kKv4Warps;
   if (grid > 0x7fffffffll) return fail(DAK_ERR_UNSUPPORTED, "too many tokens for one launch");
@@ -362,9 +405,9 @@ extern "C" int dak_kv_read_q4(const dak_kv4_cache *cache, const int32_t *positio
   p.out[1] = static_cast<uint16_t *>(v_out);
   p.tokens = tokens;
   const long long quads = (tokens + 3ll) / 4;
-  p.groups = head_groups(quads, cache->kv_heads);
+  p.groups = head_groups(quads, 2 * cache->kv_heads, kReadWarps);
   p.pdl = decode_pdl_enabled() ? 1 : 0;
-  const long long grid = (quads * 2 * p.groups + kKv4Warps - 1) / kKv4Warps;
+  const long long grid = (quads * p.groups + kKv4Warps - 1) / kKv4Warps;
   if (grid > 0x7fffffffll) return fail(DAK_ERR_UNSUPPORTED, "too many tokens for one launch");
   auto s = static_cast<cudaStream_t>(stream);
   return cuda_status(dtype == DAK_DTYPE_F16 ? launch_read<__half>(p, (unsigned)grid, s)

@@ -24,7 +24,7 @@ struct Kv4Cache {
   const int32_t *table;
   long long table_stride;
   int max_pages, rows;     // table entries per sequence, sequences
-  int kv_heads, page_size, ng;
+  int kv_heads, page_size, page_log2, ng;
   int *status;
 };
 

@@ -19,7 +19,8 @@ constexpr int kCopyThreads = 256;
 constexpr int kCopyUnroll = 4;
 constexpr int kPieceVecs = kCopyThreads * kCopyUnroll;  // 16 KB per CTA
 constexpr int kMaxMoves = 3584;                         // 28 KB of the 32,764 parameter bytes
-constexpr int kFewMoves = 120;                          // 1 KB of parameters
+constexpr int kFewMoves = 120;                          // 1 KB of parameters: cheaper to launch
+constexpr int kSomeMoves = 500;                         // 4 KB
 
 template <int N>
 struct CopyParams {
@@ -105,9 +106,14 @@ extern "C" int dak_copy_pages(void *pool_dev, int64_t dev_pages, void *pool_host
   for (int i = 1; i < n; ++i)
     if (sorted[i] == sorted[i - 1])
       return fail(DAK_ERR_INVALID_ARG, "copy_pages: page %d is a destination twice", (int)sorted[i]);
-  for (int i = 0; i < n; ++i)
-    if (std::binary_search(sorted, sorted + n, src[i]))
-      return fail(DAK_ERR_INVALID_ARG, "copy_pages: page %d is both a source and a destination", (int)src[i]);
+  int32_t from[kMaxMoves];
+  std::copy(src, src + n, from);
+  std::sort(from, from + n);
+  for (int i = 0, j = 0; i < n && j < n;) {
+    if (from[i] == sorted[j])
+      return fail(DAK_ERR_INVALID_ARG, "copy_pages: page %d is both a source and a destination", (int)from[i]);
+    from[i] < sorted[j] ? ++i : ++j;
+  }
   int st;
   if (pool_dev && (st = check_gpu_accessible(pool_dev, "pool_dev"))) return st;
   if (pool_host && (st = check_gpu_accessible(pool_host, "pool_host"))) return st;
@@ -116,6 +122,8 @@ extern "C" int dak_copy_pages(void *pool_dev, int64_t dev_pages, void *pool_host
   const cudaError_t e =
       n <= kFewMoves
           ? launch_copy<kFewMoves>(pool_dev, pool_host, dev_slab_stride, host_slab_stride, page_bytes, slabs, src, dst, n, s)
+      : n <= kSomeMoves
+          ? launch_copy<kSomeMoves>(pool_dev, pool_host, dev_slab_stride, host_slab_stride, page_bytes, slabs, src, dst, n, s)
           : launch_copy<kMaxMoves>(pool_dev, pool_host, dev_slab_stride, host_slab_stride, page_bytes, slabs, src, dst, n, s);
   return cuda_status(e, "copy_pages launch");
 }

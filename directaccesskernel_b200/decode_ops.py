@@ -4,11 +4,12 @@ transformers' Llama arithmetic op by op (app/python/llama/vanila_llama.py:
 227-400 runs the same ops as separate torch kernels)."""
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
 
-from ._lib import LIB, check
+from ._lib import LIB, RotaryArgs, check
 from .runtime import dak_dtype
 from .trace import traced
 
@@ -26,7 +27,7 @@ def stream_of(device: int) -> int:
 def current_device_of(t: torch.Tensor, name: str) -> int:
     """The index of t's device, which must be the current CUDA device."""
     device = t.get_device()
-    if device < 0 or device != torch.cuda.current_device():
+    if device < 0 or device != torch._C._cuda_getDevice():
         raise RuntimeError(f"{name} must be on the current CUDA device")
     return device
 
@@ -151,23 +152,32 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
     and head strides are free (multiples of 8), so x may be the q and k heads of
     a fused projection; ``out`` may be x itself, else must not overlap it."""
     device = current_device_of(x, "x")
-    _check16(x)
-    if x.dim() != 3:
-        raise RuntimeError("x must be [tokens, heads, head_dim]")
-    T, H, D = x.shape
+    dtype = x.dtype
+    if x.dim() != 3 or dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError("x must be a float16 or bfloat16 [tokens, heads, head_dim] tensor")
+    T, H, D = shape = x.shape
+    xt, xh, xd = x.stride()
+    if xd != 1 and D > 1:
+        raise RuntimeError("x must have a contiguous last dimension")
     _check_rope(positions, inv_freq, T, D, device)
     if out is None:
-        out = torch.empty(T, H, D, dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or (D > 1 and out.stride(2) != 1):
-        raise RuntimeError("out must match x in shape, dtype and device, with a contiguous last dimension")
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    elif out.shape != shape or out.dtype != dtype or out.get_device() != device:
+        raise RuntimeError("out must match x in shape, dtype and device")
     if T and H:
-        xt, xh, _ = x.stride()
-        ot, oh, _ = out.stride()
+        ot, oh, od = out.stride()
+        if od != 1 and D > 1:
+            raise RuntimeError("out must have a contiguous last dimension")
+        a = RotaryArgs()
+        a.x, a.out, a.positions, a.inv_freq = x.data_ptr(), out.data_ptr(), positions.data_ptr(), inv_freq.data_ptr()
         # A dimension of one entry has no stride to speak of.
-        check(LIB.dak_rotary(x.data_ptr(), xt if T > 1 else 0, xh if H > 1 else 0, positions.data_ptr(),
-                             inv_freq.data_ptr(), float(rope_scale), int(interleaved), out.data_ptr(),
-                             ot if T > 1 else 0, oh if H > 1 else 0, T, H, D, 2 * inv_freq.numel(),
-                             dak_dtype(x.dtype), stream_of(device)), "rotary")
+        if T > 1:
+            a.x_stride_t, a.o_stride_t = xt, ot
+        if H > 1:
+            a.x_stride_h, a.o_stride_h = xh, oh
+        a.tokens, a.heads, a.head_dim, a.rotary_dim = T, H, D, 2 * inv_freq.numel()
+        a.interleaved, a.rope_scale, a.dtype = interleaved, rope_scale, dak_dtype(dtype)
+        check(LIB.dak_rotary(ctypes.byref(a), stream_of(device)), "rotary")
     return out
 
 

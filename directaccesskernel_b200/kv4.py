@@ -29,12 +29,13 @@ from . import _lib
 from ._lib import LIB, check
 from .attention import HEAD_DIM
 from .decode_ops import _check_rope, current_device_of, stream_of
-from .runtime import dak_dtype
+from .runtime import NUM_SMS, dak_dtype
 from .trace import traced
 
 PAGE_SIZES = (16, 32, 64)
 GROUPS = (32, 64, 128)
 MAX_BLOCK_HEADS = 8  # query heads that one CTA of the attention serves
+SHORT_ROWS = 512     # tokens up to which the attention does not split a row
 
 
 def page_bytes(page_size: int, group: int = 128) -> int:
@@ -165,11 +166,9 @@ def kv_read_q4(pool_dev: torch.Tensor | None, pool_host: torch.Tensor | None, bl
     for t, nm in ((k_out, "k_out"), (v_out, "v_out")):
         if t is not None and (t.shape != shape or t.dtype != dtype or t.get_device() != device or not t.is_contiguous()):
             raise RuntimeError(f"{nm} must be a contiguous [tokens, kv_heads, 128] tensor of dtype")
-    if k_out is None and v_out is None:  # one allocation for both
-        k_out, v_out = torch.empty((2, *shape), dtype=dtype, device=block_table.device)
-    elif k_out is None:
-        k_out = torch.empty_like(v_out)
-    elif v_out is None:
+    if k_out is None:
+        k_out = block_table.new_empty(shape, dtype=dtype)
+    if v_out is None:
         v_out = torch.empty_like(k_out)
     if T:
         check(LIB.dak_kv_read_q4(ctypes.byref(c), positions.data_ptr(),
@@ -232,14 +231,16 @@ def decode_paged_q4(query: torch.Tensor, pool_dev: torch.Tensor | None, pool_hos
     elif not 0 < max_seq_len <= c.max_pages * c.page_size:
         raise RuntimeError("max_seq_len must be positive and within the block table's pages")
     if out is None:
-        out = torch.empty((B, Hq, HEAD_DIM), dtype=dtype, device=query.device)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
     elif out.shape != query.shape or out.dtype != dtype or out.get_device() != device or out.stride(2) != 1:
         raise RuntimeError("out must be [B, Hq, 128] of the query dtype with a contiguous last dimension")
     a = _lib.AttnQ4Args()
-    need = LIB.dak_attn_q4_scratch(ctypes.byref(c), Hq, max_seq_len)
+    # A call of short rows, no more of them than SMs, takes none.
+    short = max_seq_len <= SHORT_ROWS and B * Hq <= NUM_SMS
+    need = 0 if short else LIB.dak_attn_q4_scratch(ctypes.byref(c), Hq, max_seq_len)
     if need > 0:
         if scratch is None:
-            scratch = torch.empty(need, dtype=torch.float32, device=query.device)
+            scratch = query.new_empty(need, dtype=torch.float32)
         elif scratch.dtype != torch.float32 or scratch.get_device() != device or scratch.numel() < need \
                 or not scratch.is_contiguous():
             raise RuntimeError(f"scratch must be a contiguous float32 CUDA tensor of {need} entries")

@@ -10,6 +10,8 @@ sequence (app/python/pinned_static_cache.py:8-115).
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from ._lib import LIB, check
@@ -20,13 +22,15 @@ MAX_MOVES = 3584  # pages per launch
 
 
 def _entries(t, name: str) -> torch.Tensor:
-    if isinstance(t, torch.Tensor):
-        if t.is_cuda or t.dim() != 1 or t.is_floating_point():
-            raise RuntimeError(f"{name} must be a list or a 1-D CPU tensor of page entries")
-        if t.dtype != torch.int32 and t.numel() and (int(t.max()) > 2**31 - 1 or int(t.min()) < -2**31):
-            raise RuntimeError(f"{name} does not fit int32")
-        return t.to(torch.int32).contiguous()
-    return torch.tensor(t, dtype=torch.int32)
+    if not isinstance(t, torch.Tensor):
+        return torch.tensor(t, dtype=torch.int32)
+    if t.is_cuda or t.dim() != 1 or t.is_floating_point():
+        raise RuntimeError(f"{name} must be a list or a 1-D CPU tensor of page entries")
+    if t.dtype == torch.int32:
+        return t.contiguous()
+    if t.numel() and (int(t.max()) > 2**31 - 1 or int(t.min()) < -2**31):
+        raise RuntimeError(f"{name} does not fit int32")
+    return t.to(torch.int32).contiguous()
 
 
 @traced
@@ -46,41 +50,40 @@ def copy_pages(pool_dev: torch.Tensor | None, pool_host: torch.Tensor | None, sr
     if not 0 <= page_dim < pool.dim():
         raise RuntimeError("page_dim is outside the pool's dimensions")
     device = current_device_of(pool_dev, "pool_dev") if pool_dev is not None else torch.cuda.current_device()
-    if pool_host is not None and (pool_host.is_cuda or not pool_host.is_pinned()):
-        raise RuntimeError("pool_host must be pinned host memory")
-    for t in (pool_dev, pool_host):
-        if t is not None and (not t.is_contiguous() or t.dtype != pool.dtype or t.shape[:page_dim] != pool.shape[:page_dim]
-                              or t.shape[page_dim + 1:] != pool.shape[page_dim + 1:]):
+    shape = pool.shape
+    if not pool.is_contiguous():
+        raise RuntimeError("the pools must be contiguous")
+    if pool_host is not None:
+        if pool_host.is_cuda or not pool_host.is_pinned():
+            raise RuntimeError("pool_host must be pinned host memory")
+        if pool_host.dtype != pool.dtype or pool_host.shape[:page_dim] != shape[:page_dim] \
+                or pool_host.shape[page_dim + 1:] != shape[page_dim + 1:] or not pool_host.is_contiguous():
             raise RuntimeError("the pools must be contiguous and differ in nothing but their pages")
     src, dst = _entries(src, "src"), _entries(dst, "dst")
     n = src.numel()
     if dst.numel() != n:
         raise RuntimeError("src and dst must have the same length")
-    if n > MAX_MOVES:  # several launches: what one launch refuses is refused over all of them
-        d = dst.sort().values
-        if bool((d[1:] == d[:-1]).any()):
-            raise RuntimeError("copy_pages: a page is a destination twice")
-        if bool(torch.isin(src, dst).any()):
-            raise RuntimeError("copy_pages: a page is both a source and a destination")
-    page = pool.element_size()
-    for size in pool.shape[page_dim + 1:]:
-        page *= size
-    slabs = 1
-    for size in pool.shape[:page_dim]:
-        slabs *= size
+    slabs, page = math.prod(shape[:page_dim]), math.prod(shape[page_dim + 1:]) * pool.element_size()
     if n == 0 or slabs == 0 or page == 0:
         return
     nd = pool_dev.shape[page_dim] if pool_dev is not None else 0
     nh = pool_host.shape[page_dim] if pool_host is not None else 0
-    if n > MAX_MOVES:  # no launch before the last list is known to be in range
-        both = torch.cat([src, dst])
-        if int(both.max()) >= nd or int(both.min()) < -nh:
-            raise RuntimeError("copy_pages: an entry is outside its pool")
+    to = (pool_dev.data_ptr() if nd else None, nd, pool_host.data_ptr() if nh else None, nh, page, slabs, nd * page, nh * page)
+    if n <= MAX_MOVES:
+        check(LIB.dak_copy_pages(*to, src.data_ptr(), dst.data_ptr(), n, stream_of(device)), "copy_pages")
+        return
+    # Several launches: what one launch refuses is refused over all of them, before the first.
+    d = dst.sort().values
+    if bool((d[1:] == d[:-1]).any()):
+        raise RuntimeError("copy_pages: a page is a destination twice")
+    if bool(torch.isin(src, dst).any()):
+        raise RuntimeError("copy_pages: a page is both a source and a destination")
+    both = torch.cat([src, dst])
+    if int(both.max()) >= nd or int(both.min()) < -nh:
+        raise RuntimeError("copy_pages: an entry is outside its pool")
     for i in range(0, n, MAX_MOVES):
         s, d = src[i:i + MAX_MOVES], dst[i:i + MAX_MOVES]
-        check(LIB.dak_copy_pages(pool_dev.data_ptr() if nd else None, nd, pool_host.data_ptr() if nh else None, nh, page,
-                                 slabs, nd * page, nh * page, s.data_ptr(), d.data_ptr(), s.numel(), stream_of(device)),
-              "copy_pages")
+        check(LIB.dak_copy_pages(*to, s.data_ptr(), d.data_ptr(), s.numel(), stream_of(device)), "copy_pages")
 
 
 class PageTable:

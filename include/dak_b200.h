@@ -416,10 +416,18 @@ DAK_API int dak_silu_mul(const void *gate_up, int64_t ld, void *out, int rows, i
  * 16 in the half layout.  out may be x itself (same strides).  No reference
  * counterpart as a kernel: the reference rotates in torch, whole heads in the
  * half layout (app/python/llama/vanila_llama.py:212-246). */
-DAK_API int dak_rotary(const void *x, int64_t x_stride_t, int64_t x_stride_h, const int32_t *positions,
-                       const float *inv_freq, float rope_scale, int interleaved, void *out, int64_t o_stride_t,
-                       int64_t o_stride_h, int tokens, int heads, int head_dim, int rotary_dim, int dtype,
-                       void *stream);
+typedef struct dak_rotary_args {
+  const void *x;              /* [tokens, heads, head_dim]                      */
+  int64_t x_stride_t, x_stride_h;
+  const int32_t *positions;   /* [tokens]                                       */
+  const float *inv_freq;      /* [rotary_dim / 2]                               */
+  void *out;                  /* [tokens, heads, head_dim]                      */
+  int64_t o_stride_t, o_stride_h;
+  int tokens, heads, head_dim, rotary_dim, interleaved;
+  float rope_scale;
+  int dtype;
+} dak_rotary_args;
+DAK_API int dak_rotary(const dak_rotary_args *args, void *stream);
 
 /* ------------------------------------------------- 4-bit tiered, paged KV */
 /* A pool is [pages, kv_heads, slab] bytes; the slab of one (page, head) of

@@ -127,8 +127,8 @@ def test_append_refusals(bad, status, msg):
 
 def test_rotary_refusals():
     def call(tokens=2, heads=2, d=128, r=128, inter=0, st=(256, 128, 256, 128), x=BUF, out=BUF, dtype=_lib.DTYPE_F16):
-        return _status(_lib.LIB.dak_rotary, x, st[0], st[1], BUF, BUF, 1.0, inter, out, st[2], st[3], tokens, heads, d, r,
-                       dtype, None)
+        a = _lib.RotaryArgs(x, st[0], st[1], BUF, BUF, out, st[2], st[3], tokens, heads, d, r, inter, 1.0, dtype)
+        return _status(_lib.LIB.dak_rotary, ctypes.byref(a), None)
 
     assert call(dtype=_lib.DTYPE_F32)[0] == _lib.DAK_ERR_UNSUPPORTED
     for kw, status, msg in ((dict(heads=0), _lib.DAK_ERR_INVALID_ARG, "positive"),

@@ -99,7 +99,7 @@ def test_rotary_of_nothing_and_refusals():
     assert rotary(x[:0], pos[:0], inv).shape == (0, 2, 128)
     for kw, msg in ((dict(x=x.float()), "float16"), (dict(positions=pos.long()), "int32"), (dict(positions=pos[:3]), "per token"),
                     (dict(inv_freq=inv.double()), "float32"), (dict(inv_freq=torch.ones(65, device="cuda")), "head_dim / 2"),
-                    (dict(out=torch.empty_like(x[:2])), "out must match"), (dict(x=x[..., 1:125]), "multiple of 8"),
+                    (dict(out=torch.empty_like(x[:2])), "out must match"), (dict(x=x[..., 1:125]), "multiple of 8"), (dict(x=x[..., ::2]), "contiguous"),
                     (dict(inv_freq=inv[:20]), "multiple of 16")):
         with pytest.raises(RuntimeError, match=msg):
             rotary(**{**dict(x=x, positions=pos, inv_freq=inv), **kw})
