@@ -12,7 +12,10 @@
 // Both are bound by memory.  Eight lanes own a (token, head) row, 16 dims each
 // (two 16-byte loads, one 8-byte code store), so a group's minimum and maximum
 // are 1, 2 or 3 shuffles away; a warp takes the same head of four neighbouring
-// tokens, whose code rows are neighbours in the page.
+// tokens, whose code rows are neighbours in the page.  The append's CTA takes
+// four tokens and up to 48 heads of each: four bulk copies bring them into shared
+// memory, all in flight at once, while the threads work out the tokens' angles,
+// one each, and look up their pages.
 #include <cstring>
 
 #include "dak_host.h"
@@ -72,8 +75,10 @@ namespace {
 
 constexpr int kKv4Threads = 256;
 constexpr int kKv4Warps = kKv4Threads / 32;
-constexpr int kAppendWarps = 3500, kReadWarps = 9472;  // for the q heads of a call (and half that for k, v each); for a read
-constexpr int kBatch = 4;  // heads whose loads are in flight at once
+constexpr int kAppendHeads = 48;            // of an append's CTA, at most: 48 KB of shared memory
+constexpr long long kAppendCtas = 148 * 6;  // an append's CTAs, where its tokens alone give fewer
+constexpr int kReadWarps = 9472;            // a read's warps, likewise
+constexpr int kBatch = 4;                   // rows a reading thread has in flight
 
 struct AppendParams {
   Kv4Cache c;
@@ -84,7 +89,7 @@ struct AppendParams {
   float scale;
   uint16_t *q_out;
   int tokens, q_heads, rotary_dim, interleaved, units;
-  int q_groups, kv_groups;  // warps that share a token's q heads, and its k (and v) heads
+  int slice;  // heads (q, then k, then v) per CTA
   int pdl;
 };
 
@@ -121,121 +126,107 @@ __device__ __forceinline__ void kv4_quantise(const float (&x)[16], int lane8, ui
   }
 }
 
-// A warp's roles for its four tokens: q head groups first, then k, then v.
+struct AppendSmem {
+  alignas(16) float tab[2 * 4 * kKv4Dim / 2];  // angles of the four tokens
+  uint8_t *page[4];
+  uint64_t bar;
+  int tier[4];
+  int abort_flag[2];  // [1]: of the second wait
+};
+
+// A head of the four tokens at a time per warp: q heads are rotated, k heads
+// rotated and packed, v heads packed.
 template <typename T, int NG>
 __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const __grid_constant__ AppendParams p) {
+  extern __shared__ __align__(128) uint8_t rows_s[];  // [tokens][slice][128] 16-bit, then the rest
+  AppendSmem &sm = *reinterpret_cast<AppendSmem *>(rows_s + 4 * p.slice * kKv4Dim * 2);
   pdl_enter(p.pdl);
-  const int roles = p.q_groups + 2 * p.kv_groups;
-  const long long w = (long long)blockIdx.x * kKv4Warps + warp_id();
-  const int role = (int)(w % roles);
-  const int lane8 = lane_id() & 7;
-  const long long t64 = (w / roles) * 4 + (lane_id() >> 3);
-  const bool live = t64 < p.tokens;
-  const int t = live ? (int)t64 : 0;  // idle lanes stay for the shuffles
-  const int pos = p.positions[t];
-  const uint16_t *row = p.qkv + t * p.ld;
-  if (role < p.q_groups) {
-    if (!live) return;  // no shuffles below
-    for (int u = lane8; u < p.units; u += 8) {
-      const RopeUnit unit = rope_unit(u, p.rotary_dim, p.interleaved);
-      float c[8], s[8];
-      rope_unit_angles(unit, pos, p.inv_freq, p.scale, c, s);
-      for (int h0 = role; h0 < p.q_heads; h0 += kBatch * p.q_groups) {
-        uint4 a[kBatch], b[kBatch];
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-          const int h = h0 + k * p.q_groups;
-          if (h >= p.q_heads) break;
-          const uint4 *src = reinterpret_cast<const uint4 *>(row + h * kKv4Dim);
-          a[k] = src[unit.v0];
-          b[k] = unit.v1 >= 0 ? src[unit.v1] : a[k];
-        }
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-          const int h = h0 + k * p.q_groups;
-          if (h >= p.q_heads) break;
-          rope_unit_apply<T>(unit, p.interleaved, a[k], b[k], c, s,
-                             reinterpret_cast<uint4 *>(p.q_out + ((long long)t * p.q_heads + h) * kKv4Dim));
-        }
-      }
-    }
+  const int t0 = blockIdx.x * 4, nt = min(4, p.tokens - t0);
+  const int lane8 = lane_id() & 7, sub = lane_id() >> 3;
+  const bool live = sub < nt;
+  const int t = t0 + (live ? sub : 0);  // idle lanes stay for the shuffles
+  const int P = p.c.page_size, Hkv = p.c.kv_heads;
+  const int h0 = blockIdx.y * p.slice, h_end = min(p.q_heads + 2 * Hkv, h0 + p.slice);
+  const uint32_t bar_a = smem_u32(&sm.bar), token_bytes = (h_end - h0) * kKv4Dim * 2;
+  const WaitCtx wc{&sm.abort_flag[0], p.c.status};
+  if (threadIdx.x == 0) {
+    sm.abort_flag[0] = sm.abort_flag[1] = 0;
+    mbar_init(bar_a, 1);
+    fence_mbar_init();
+    mbar_arrive_expect_tx(bar_a, nt * token_bytes);
+    const uint64_t pol = l2_policy_evict_first();
+    for (int i = 0; i < nt; ++i)
+      bulk_load(smem_u32(rows_s) + i * token_bytes, p.qkv + (long long)(t0 + i) * p.ld + h0 * kKv4Dim, token_bytes, bar_a, pol);
+  }
+  if (threadIdx.x < nt) {
+    const int pos = p.positions[t0 + threadIdx.x];
+    int tier = 0;
+    uint8_t *page = pos < 0 ? nullptr
+                            : kv4_page(p.c, p.seq_index ? p.seq_index[t0 + threadIdx.x] : t0 + (int)threadIdx.x,
+                                       pos >> p.c.page_log2, &tier);
+    if (!page) atomicCAS(p.c.status, 0, DAK_ERR_INVALID_ARG);
+    sm.page[threadIdx.x] = page;
+    sm.tier[threadIdx.x] = tier;
+  }
+  const int stride = rope_stride(p.rotary_dim);
+  rope_table(sm.tab, p.positions + t0, nt, 4, p.inv_freq, p.rotary_dim, p.scale);
+  __syncthreads();
+  const float *cos_row = sm.tab + (live ? sub : 0) * stride, *sin_row = cos_row + 4 * stride;
+  const int slot = p.positions[t] & (P - 1);
+  uint8_t *page = live ? sm.page[sub] : nullptr;
+  const int half = kv4_half_bytes(P, NG);
+  const int R = p.rotary_dim, part = R / 16;  // vectors between the partners of the half layout
+  const uint8_t *row = rows_s + (live ? sub : 0) * token_bytes;
+  if (!mbar_wait<false>(bar_a, 0, wc)) {  // gave up: let the copies land (bounded again), then leave
+    mbar_wait<false>(bar_a, 0, WaitCtx{&sm.abort_flag[1], p.c.status});
     return;
   }
-  const int isv = role >= p.q_groups + p.kv_groups ? 1 : 0;
-  const int g = role - p.q_groups - isv * p.kv_groups;
-  const int P = p.c.page_size;
-  int tier = 0;
-  uint8_t *page = nullptr;
-  if (live) {
-    page = pos < 0 ? nullptr : kv4_page(p.c, p.seq_index ? p.seq_index[t] : t, pos >> p.c.page_log2, &tier);
-    if (!page && lane8 == 0) atomicCAS(p.c.status, 0, DAK_ERR_INVALID_ARG);
-  }
-  const int half = kv4_half_bytes(P, NG);
-  const long long in_slab = (long long)isv * half + (pos & (P - 1)) * 64;
-  const long long pair_off = (long long)isv * half + P * 64 + (pos & (P - 1)) * 4 * NG;
-  // Half layout: dims 16 lane8 .. +15 and, R/2 dims away, their partners; each
-  // lane keeps its own side of the pairs.
-  const int R = isv ? 0 : p.rotary_dim;
-  const int part = R / 16;  // vectors between partners
-  float c[16], s[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    c[i] = 1.f;
-    s[i] = 0.f;
-    const int d = lane8 * 16 + i;
-    if (d < R) {
-      if (p.interleaved) {
-        if (i % 2 == 0) rope_cos_sin(pos, p.inv_freq[d / 2], p.scale, c[i], s[i]);
-      } else {
-        rope_cos_sin(pos, p.inv_freq[d < R / 2 ? d : d - R / 2], p.scale, c[i], s[i]);
-        if (d < R / 2) s[i] = -s[i];
+
+  for (int h = h0 + warp_id(); h < h_end; h += kKv4Warps) {
+    const uint4 *src = reinterpret_cast<const uint4 *>(row + (h - h0) * kKv4Dim * 2);
+    if (h < p.q_heads) {
+      if (!live) continue;
+      uint4 *dst = reinterpret_cast<uint4 *>(p.q_out + ((long long)t * p.q_heads + h) * kKv4Dim);
+      for (int u = lane8; u < p.units; u += 8) {
+        const RopeUnit unit = rope_unit(u, R, p.interleaved);
+        float c[8], s[8];
+        rope_unit_angles(unit, cos_row, sin_row, c, s);
+        rope_unit_apply<T>(unit, p.interleaved, src[unit.v0], src[unit.v1 >= 0 ? unit.v1 : unit.v0], c, s, dst);
       }
+      continue;
     }
-  }
-  // The vectors of this lane and, where they are rotated in halves, their
-  // partners; the next head's are loaded while this one's are packed.
-  const bool paired = !p.interleaved && R > 0;
-  auto head = [&](int h) {
-    return reinterpret_cast<const uint4 *>(row + (long long)(p.q_heads + isv * p.c.kv_heads + h) * kKv4Dim);
-  };
-  auto partner = [&](int v) { return v < part ? v + part : v < 2 * part ? v - part : v; };
-  uint4 own[2], other[2];
-  auto load = [&](int h) {
-    const uint4 *src = head(h);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      own[k] = src[lane8 * 2 + k];
-      other[k] = paired ? src[partner(lane8 * 2 + k)] : own[k];
-    }
-  };
-  load(g);
-  for (int h = g; h < p.c.kv_heads; h += p.kv_groups) {
+    const int isv = h >= p.q_heads + Hkv ? 1 : 0;
     float x[16];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       float y[8];
-      unpack8<T>(own[k], y);
-      if (paired && lane8 * 2 + k < 2 * part) {
-        float z[8];
-        unpack8<T>(other[k], z);
+      const int v = lane8 * 2 + k;
+      unpack8<T>(src[v], y);
+      if (!isv && !p.interleaved && v < 2 * part) {
+        float z[8], c[8], s[8];
+        unpack8<T>(src[v < part ? v + part : v - part], z);  // each lane keeps its own side of the pairs
+        const int f = 8 * (v < part ? v : v - part);
+        load4(cos_row + f, c), load4(cos_row + f + 4, c + 4);
+        load4(sin_row + f, s), load4(sin_row + f + 4, s + 4);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = fmaf(y[i], c[8 * k + i], z[i] * s[8 * k + i]);
+        for (int i = 0; i < 8; ++i) y[i] = fmaf(y[i], c[i], z[i] * (v < part ? -s[i] : s[i]));
+      } else if (!isv && p.interleaved && v * 8 < R) {
+        float c[4], s[4];
+        load4(cos_row + 4 * v, c);
+        load4(sin_row + 4 * v, s);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (v * 8 + 2 * i < R) rope_turn(y[2 * i], y[2 * i + 1], c[i], s[i]);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[8 * k + i] = y[i];
     }
-    if (h + p.kv_groups < p.c.kv_heads) load(h + p.kv_groups);
-    if (p.interleaved) {
-#pragma unroll
-      for (int i = 0; i < 16; i += 2)
-        if (lane8 * 16 + i < R) rope_turn(x[i], x[i + 1], c[i], s[i]);
-    }
-    uint8_t *slab = page ? page + (long long)h * p.c.slab_bytes : nullptr;
-    kv4_quantise<NG>(x, lane8, slab ? slab + in_slab : nullptr, slab ? slab + pair_off : nullptr);
+    uint8_t *slab = page ? page + (long long)(h - p.q_heads - isv * Hkv) * p.c.slab_bytes + isv * half : nullptr;
+    kv4_quantise<NG>(x, lane8, slab ? slab + slot * 64 : nullptr, slab ? slab + P * 64 + slot * 4 * NG : nullptr);
   }
   // Host pages are read back over the host link by the next kernels of the
   // stream; make the writes visible system-wide before this grid completes.
-  if (tier == 1) __threadfence_system();
+  if (live && sm.tier[sub] == 1) __threadfence_system();
 }
 
 struct ReadParams {
@@ -297,12 +288,19 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_read_kernel(const __grid_cons
   }
 }
 
+template <typename T, int NG>
+cudaError_t launch_append_g(const AppendParams &p, dim3 grid, cudaStream_t s) {
+  auto kern = kv4_append_kernel<T, NG>;
+  const cudaError_t e = prepare_kernel_attributes(reinterpret_cast<const void *>(kern));
+  return e != cudaSuccess ? e : launch_ex(kern, grid, dim3(kKv4Threads), 4 * p.slice * kKv4Dim * 2 + sizeof(AppendSmem), s, 1, p.pdl != 0, p);
+}
+
 template <typename T>
-cudaError_t launch_append(const AppendParams &p, unsigned grid, cudaStream_t s) {
+cudaError_t launch_append(const AppendParams &p, dim3 grid, cudaStream_t s) {
   switch (p.c.ng) {
-    case 1: return launch_ex(kv4_append_kernel<T, 1>, dim3(grid), dim3(kKv4Threads), 0, s, 1, p.pdl != 0, p);
-    case 2: return launch_ex(kv4_append_kernel<T, 2>, dim3(grid), dim3(kKv4Threads), 0, s, 1, p.pdl != 0, p);
-    default: return launch_ex(kv4_append_kernel<T, 4>, dim3(grid), dim3(kKv4Threads), 0, s, 1, p.pdl != 0, p);
+    case 1: return launch_append_g<T, 1>(p, grid, s);
+    case 2: return launch_append_g<T, 2>(p, grid, s);
+    default: return launch_append_g<T, 4>(p, grid, s);
   }
 }
 
@@ -313,12 +311,6 @@ cudaError_t launch_read(const ReadParams &p, unsigned grid, cudaStream_t s) {
     case 2: return launch_ex(kv4_read_kernel<T, 2>, dim3(grid), dim3(kKv4Threads), 0, s, 1, p.pdl != 0, p);
     default: return launch_ex(kv4_read_kernel<T, 4>, dim3(grid), dim3(kKv4Threads), 0, s, 1, p.pdl != 0, p);
   }
-}
-
-// Warps that share `heads` heads of each of `quads` token quads: one head per
-// warp until about `warps` warps fill the GPU, then more heads per warp.
-int head_groups(long long quads, int heads, int warps) {
-  return (int)std::min<long long>(heads, std::max<long long>(1, warps / std::max(1ll, quads)));
 }
 
 int check_tokens(int tokens, const int32_t *positions, const int32_t *seq_index, int batch) {
@@ -370,14 +362,18 @@ extern "C" int dak_rope_kv_append_q4(const dak_kv4_cache *cache, const dak_kv4_a
   p.interleaved = a->interleaved != 0;
   p.units = rope_units(kKv4Dim, a->rotary_dim, p.interleaved);
   const long long quads = (a->tokens + 3ll) / 4;
-  p.q_groups = a->q_heads > 0 ? head_groups(quads, a->q_heads, kAppendWarps) : 0;
-  p.kv_groups = head_groups(quads, cache->kv_heads, kAppendWarps / 2);
   p.pdl = decode_pdl_enabled() ? 1 : 0;
-  const long long grid = (quads * (p.q_groups + 2 * p.kv_groups) + kKv4Warps - 1) / kKv4Warps;
-  if (grid > 0x7fffffffll) return fail(DAK_ERR_UNSUPPORTED, "too many tokens for one launch");
+  // All heads of four tokens on one CTA, or on as many as keep the GPU busy, down
+  // to one head per warp.
+  const long long heads = a->q_heads + 2ll * cache->kv_heads;
+  const long long slices = std::max((heads + kAppendHeads - 1) / kAppendHeads,
+                                    std::min((heads + kKv4Warps - 1) / kKv4Warps, kAppendCtas / quads));
+  if (heads > 65535ll * kKv4Warps) return fail(DAK_ERR_UNSUPPORTED, "too many heads");
+  p.slice = (int)(((heads + slices - 1) / slices + kKv4Warps - 1) / kKv4Warps * kKv4Warps);
+  const dim3 grid((unsigned)quads, (unsigned)((heads + p.slice - 1) / p.slice));
   auto s = static_cast<cudaStream_t>(stream);
-  return cuda_status(a->dtype == DAK_DTYPE_F16 ? launch_append<__half>(p, (unsigned)grid, s)
-                                               : launch_append<__nv_bfloat16>(p, (unsigned)grid, s),
+  return cuda_status(a->dtype == DAK_DTYPE_F16 ? launch_append<__half>(p, grid, s)
+                                               : launch_append<__nv_bfloat16>(p, grid, s),
                      "4-bit append launch");
 }
 
@@ -405,7 +401,8 @@ extern "C" int dak_kv_read_q4(const dak_kv4_cache *cache, const int32_t *positio
   p.out[1] = static_cast<uint16_t *>(v_out);
   p.tokens = tokens;
   const long long quads = (tokens + 3ll) / 4;
-  p.groups = head_groups(quads, 2 * cache->kv_heads, kReadWarps);
+  // One row per warp until the GPU is full, then more.
+  p.groups = (int)std::min<long long>(2ll * cache->kv_heads, std::max<long long>(1, kReadWarps / quads));
   p.pdl = decode_pdl_enabled() ? 1 : 0;
   const long long grid = (quads * p.groups + kKv4Warps - 1) / kKv4Warps;
   if (grid > 0x7fffffffll) return fail(DAK_ERR_UNSUPPORTED, "too many tokens for one launch");

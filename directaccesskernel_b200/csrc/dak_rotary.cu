@@ -2,10 +2,12 @@
 // or interleaved pairs, all or part of the head, frequencies and attention
 // factor as the model's scaling gives them.
 //
-// Bound by memory: each 16-byte vector is read once and written once.  One
-// thread owns one unit (dak_rotary.cuh) of a token and walks over heads, four at
-// a time so that eight loads are in flight, and the FP64 angles and sincospif are
-// paid once per unit and head group, not per head.
+// Bound by memory: each 16-byte vector is read once and written once.  A CTA
+// takes up to four tokens and puts the cosines and sines of their angles into
+// shared memory, one angle per thread.  A thread then owns one unit
+// (dak_rotary.cuh) of one of the tokens, keeps its angles in registers and walks
+// over heads, four at a time so that eight loads are in flight; the first are on
+// their way while the angles are worked out.
 #include "dak_host.h"
 #include "dak_rotary.cuh"
 
@@ -13,7 +15,9 @@ namespace dak {
 namespace {
 
 constexpr int kRotaryThreads = 256;
-constexpr long long kRotaryTarget = 200000;  // threads that fill the GPU
+constexpr int kRotaryBatch = 4;
+constexpr int kRotaryTokens = 4;              // per CTA, while their angles number at most 256
+constexpr long long kRotaryTarget = 148 * 4;  // CTAs that fill the GPU
 
 struct RotaryParams {
   const uint16_t *x;
@@ -22,39 +26,48 @@ struct RotaryParams {
   const int32_t *positions;
   const float *inv_freq;
   float scale;
-  int tokens, heads, units, groups;  // groups: head groups; group g owns heads g, g + groups, ...
+  int tokens, heads, units;
+  int cta_tokens, cta_heads;  // per CTA
+  int lanes;                  // heads of a token that the CTA's threads take at once
   int rotary_dim, interleaved, pdl;
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
+__global__ void __launch_bounds__(kRotaryThreads, 3) rotary_kernel(const __grid_constant__ RotaryParams p) {
+  extern __shared__ __align__(16) float tab[];
   pdl_enter(p.pdl);
-  const long long i = (long long)blockIdx.x * kRotaryThreads + threadIdx.x;
-  const long long row = i / p.units;
-  const int u = (int)(i - row * p.units);
-  const int t = (int)(row / p.groups);
-  const int g = (int)(row - (long long)t * p.groups);
-  if (t >= p.tokens) return;
-  const RopeUnit unit = rope_unit(u, p.rotary_dim, p.interleaved);
+  const int t0 = blockIdx.x * p.cta_tokens, nt = min(p.cta_tokens, p.tokens - t0);
+  const int h_end = min(p.heads, (int)(blockIdx.y + 1) * p.cta_heads);
+  const int row = threadIdx.x / p.units, tok = row % p.cta_tokens;
+  const RopeUnit unit = rope_unit(threadIdx.x - row * p.units, p.rotary_dim, p.interleaved);
+  int h = blockIdx.y * p.cta_heads + row / p.cta_tokens;
+  if (tok >= nt || row >= p.lanes * p.cta_tokens) h = h_end;  // no unit for this thread
+  const uint4 *src = reinterpret_cast<const uint4 *>(p.x + (t0 + tok) * p.xt);
+  uint4 *dst = reinterpret_cast<uint4 *>(p.out + (t0 + tok) * p.ot);
+  const long long src_h = p.xh / 8, dst_h = p.oh / 8;
+  uint4 a[kRotaryBatch], b[kRotaryBatch];
+  auto load = [&](int h) {
+#pragma unroll
+    for (int k = 0; k < kRotaryBatch; ++k) {
+      if (h + k * p.lanes >= h_end) break;
+      a[k] = src[(h + k * p.lanes) * src_h + unit.v0];
+      if (unit.v1 >= 0) b[k] = src[(h + k * p.lanes) * src_h + unit.v1];
+    }
+  };
+  load(h);
+  rope_table(tab, p.positions + t0, nt, p.cta_tokens, p.inv_freq, p.rotary_dim, p.scale);
+  __syncthreads();
+  const int stride = rope_stride(p.rotary_dim);
   float c[8], s[8];
-  rope_unit_angles(unit, p.positions[t], p.inv_freq, p.scale, c, s);
-  constexpr int kBatch = 4;
-  for (int h0 = g; h0 < p.heads; h0 += kBatch * p.groups) {
-    uint4 a[kBatch], b[kBatch];
+  rope_unit_angles(unit, tab + tok * stride, tab + (p.cta_tokens + tok) * stride, c, s);
+  while (h < h_end) {
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int h = h0 + k * p.groups;
-      if (h >= p.heads) break;
-      const uint4 *src = reinterpret_cast<const uint4 *>(p.x + t * p.xt + h * p.xh);
-      a[k] = src[unit.v0];
-      b[k] = unit.v1 >= 0 ? src[unit.v1] : a[k];
+    for (int k = 0; k < kRotaryBatch; ++k) {
+      if (h + k * p.lanes >= h_end) break;
+      rope_unit_apply<T>(unit, p.interleaved, a[k], b[k], c, s, dst + (h + k * p.lanes) * dst_h);
     }
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int h = h0 + k * p.groups;
-      if (h >= p.heads) break;
-      rope_unit_apply<T>(unit, p.interleaved, a[k], b[k], c, s, reinterpret_cast<uint4 *>(p.out + t * p.ot + h * p.oh));
-    }
+    h += kRotaryBatch * p.lanes;
+    load(h);
   }
 }
 
@@ -93,20 +106,28 @@ extern "C" int dak_rotary(const dak_rotary_args *r, void *stream) {
   p.tokens = r->tokens;
   p.heads = r->heads;
   p.units = rope_units(r->head_dim, r->rotary_dim, r->interleaved != 0);
-  // One head per thread until the GPU's threads are all taken, then more heads
-  // per thread.
-  const long long per_group = (long long)r->tokens * p.units;
-  p.groups = (int)std::min<long long>(r->heads, std::max<long long>(1, kRotaryTarget / per_group));
   p.rotary_dim = r->rotary_dim;
   p.interleaved = r->interleaved != 0;
   p.pdl = decode_pdl_enabled() ? 1 : 0;
-  const long long blocks = (per_group * p.groups + kRotaryThreads - 1) / kRotaryThreads;
-  if (blocks > 0x7fffffffll) return fail(DAK_ERR_UNSUPPORTED, "rotary: too many tokens for one launch");
+  const int stride = rope_stride(r->rotary_dim), rows = kRotaryThreads / p.units;
+  // Four tokens share a CTA where there are enough to fill the GPU.
+  p.cta_tokens = 1;
+  while (p.cta_tokens < kRotaryTokens && 2 * p.cta_tokens * stride <= kRotaryThreads && 2 * p.cta_tokens <= rows &&
+         r->tokens >= 2 * p.cta_tokens * kRotaryTarget)
+    p.cta_tokens *= 2;
+  p.lanes = rows / p.cta_tokens;
+  const long long tiles = ((long long)r->tokens + p.cta_tokens - 1) / p.cta_tokens;
+  // Few tokens: their heads on several CTAs, down to one unit per thread.
+  const long long slices = std::max(1ll, kRotaryTarget / tiles);
+  p.cta_heads = (int)std::max<long long>(std::min(p.lanes, r->heads), (r->heads + slices - 1) / slices);
+  const dim3 grid((unsigned)tiles, (unsigned)((r->heads + p.cta_heads - 1) / p.cta_heads));
+  if (grid.y > 65535u) return fail(DAK_ERR_UNSUPPORTED, "rotary: too many heads for one launch");
+  const size_t smem = 2u * p.cta_tokens * stride * sizeof(float);
   auto s = static_cast<cudaStream_t>(stream);
   const cudaError_t e =
       r->dtype == DAK_DTYPE_F16
-          ? launch_ex(rotary_kernel<__half>, dim3((unsigned)blocks), dim3(kRotaryThreads), 0, s, 1, p.pdl != 0, p)
-          : launch_ex(rotary_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(kRotaryThreads), 0, s, 1, p.pdl != 0, p);
+          ? launch_ex(rotary_kernel<__half>, grid, dim3(kRotaryThreads), smem, s, 1, p.pdl != 0, p)
+          : launch_ex(rotary_kernel<__nv_bfloat16>, grid, dim3(kRotaryThreads), smem, s, 1, p.pdl != 0, p);
   return cuda_status(e, "rotary launch");
 }
 

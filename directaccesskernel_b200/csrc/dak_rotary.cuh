@@ -75,14 +75,38 @@ __device__ __forceinline__ RopeUnit rope_unit(int u, int rotary_dim, int interle
   return r;
 }
 
-// cos and sin (times the attention factor) of a unit's pairs at a position.
-__device__ __forceinline__ void rope_unit_angles(const RopeUnit &u, int pos, const float *inv_freq, float scale,
-                                                 float (&c)[8], float (&s)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    c[i] = 1.f;
-    s[i] = 0.f;
-    if (i < u.pairs) rope_cos_sin(pos, inv_freq[u.freq0 + i], scale, c[i], s[i]);
+// The angles of `tokens` tokens for a whole CTA, each worked out once: cosines
+// [tokens][stride], then sines, in shared memory.  stride is rotary_dim / 2
+// rounded up to 8 so that 4 neighbours are one aligned load.
+__host__ __device__ __forceinline__ int rope_stride(int rotary_dim) { return (rotary_dim / 2 + 7) / 8 * 8; }
+
+__device__ __forceinline__ void rope_table(float *tab, const int32_t *positions, int tokens, int max_tokens,
+                                           const float *inv_freq, int rotary_dim, float scale) {
+  const int stride = rope_stride(rotary_dim), half = rotary_dim / 2;
+  for (int i = threadIdx.x; i < tokens * stride; i += blockDim.x) {
+    const int t = i / stride, f = i - t * stride;
+    float c = 1.f, s = 0.f;
+    if (f < half) rope_cos_sin(positions[t], inv_freq[f], scale, c, s);
+    tab[i] = c;
+    tab[max_tokens * stride + i] = s;
+  }
+}
+
+__device__ __forceinline__ void load4(const float *from, float *to) {
+  const float4 v = *reinterpret_cast<const float4 *>(from);
+  to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+}
+
+// cos and sin of a unit's pairs from a token's row of the table.
+__device__ __forceinline__ void rope_unit_angles(const RopeUnit &u, const float *cos_row, const float *sin_row, float (&c)[8],
+                                                 float (&s)[8]) {
+  if (u.pairs > 0) {
+    load4(cos_row + u.freq0, c);
+    load4(sin_row + u.freq0, s);
+  }
+  if (u.pairs > 4) {
+    load4(cos_row + u.freq0 + 4, c + 4);
+    load4(sin_row + u.freq0 + 4, s + 4);
   }
 }
 
