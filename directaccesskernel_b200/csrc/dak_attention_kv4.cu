@@ -23,10 +23,16 @@
 namespace dak {
 namespace {
 
+// Two CTAs of four warps per SM: two warps for each of its four schedulers, with
+// all the registers that they can use.  Three warps per scheduler with 168
+// registers each, as two CTAs of six warps, took 10 to 30% longer, and five warps
+// a CTA, which the schedulers cannot share evenly, 20%.
+constexpr int kQ4Warps = 4;
+constexpr int kQ4Threads = 32 * kQ4Warps;
+constexpr int kQ4PerSm = 2;
 constexpr int kQ4Heads = 8;    // query heads per CTA: the MMA's N
 constexpr int kQ4Chunk = 64;   // tokens a warp takes at a time
 constexpr int kQ4Stages = 2;   // chunks in flight per warp
-constexpr int kQ4PerSm = 2;    // CTAs per SM
 constexpr int kQ4MergeBatch = 8;  // pieces of a row read at once
 constexpr int kQ4RowChunks = 8;  // rows up to this long are not split while the GPU holds them all
 
@@ -42,24 +48,21 @@ struct alignas(64) AttnQ4Params {
   int32_t *counters;  // [rows]: the CTA that finishes a split row last merges it (nullptr: merge kernel)
   int num_q_heads, group, block_heads, head_blocks;  // group: query heads per KV head
   int max_seq_len;
-  int ctas, warps, by_row;  // by_row: CTA i takes row i, and no row is split
+  int ctas, by_row;  // by_row: CTA i takes row i, and no row is split
   float scale_log2;                                  // scaling * log2(e)
   int pdl;
 };
 
 // Shared memory of a CTA: per warp a ring of chunks; the warps' statistics and
-// one block of outputs that they add up in turn; barriers.  Two CTAs share an SM,
-// and have as many warps as their rings leave room for.
+// one block of outputs that they add up in turn; barriers.
 template <int NG>
 struct Q4Smem {
-  static constexpr int warps = NG == 4 ? 5 : 6;
-  static constexpr int threads = 32 * warps;
   static constexpr uint32_t stage = 2 * kQ4Chunk * (64 + 4 * NG);
-  static constexpr uint32_t o_off = warps * kQ4Stages * stage;            // [heads][128]
+  static constexpr uint32_t o_off = kQ4Warps * kQ4Stages * stage;         // [heads][128]
   static constexpr uint32_t m_off = o_off + kQ4Heads * kKv4Dim * 4;       // [warps][heads]
-  static constexpr uint32_t l_off = m_off + warps * kQ4Heads * 4;
-  static constexpr uint32_t bar_off = l_off + warps * kQ4Heads * 4;
-  static constexpr uint32_t flag_off = bar_off + warps * kQ4Stages * 8;   // abort, abort of the drain, last
+  static constexpr uint32_t l_off = m_off + kQ4Warps * kQ4Heads * 4;
+  static constexpr uint32_t bar_off = l_off + kQ4Warps * kQ4Heads * 4;
+  static constexpr uint32_t flag_off = bar_off + kQ4Warps * kQ4Stages * 8;   // abort, abort of the drain, last
   static constexpr uint32_t bytes = flag_off + 16 + 496;                  // 496: alignment to 512
   static_assert(stage % 512 == 0, "the swizzle is computed from the offset in a stage");
   static_assert(kQ4PerSm * (bytes + 1024) <= 228 * 1024, "CTAs per SM");
@@ -162,7 +165,7 @@ __device__ __forceinline__ int chunks_of(int seq) { return (seq + kQ4Chunk - 1) 
 // Chunks of a CTA's range, given those of all rows: every CTA the same, at least
 // one for each warp.
 __device__ __forceinline__ int range_of(const AttnQ4Params &p, int total) {
-  return max((total + p.ctas - 1) / p.ctas, p.warps);
+  return max((total + p.ctas - 1) / p.ctas, kQ4Warps);
 }
 
 // Merges row (b, r), whose chunks are [begin, end) of all in ranges of `per`, from
@@ -211,10 +214,10 @@ __device__ __forceinline__ void merge_row(const AttnQ4Params &p, int b, int h0, 
 }
 
 template <typename T, int NG, int P>
-__global__ void __launch_bounds__(Q4Smem<NG>::threads, kQ4PerSm) attn_q4_kernel(const __grid_constant__ AttnQ4Params p) {
+__global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __grid_constant__ AttnQ4Params p) {
   extern __shared__ uint8_t smem_raw[];
   using S = Q4Smem<NG>;
-  constexpr int W = S::warps;
+  constexpr int W = kQ4Warps;
   // The weights of a float16 output are split into two float16 terms.
   constexpr bool kTwoTerms = std::is_same<T, __half>::value;
   uint8_t *smem = smem_raw + ((512u - (smem_u32(smem_raw) & 511u)) & 511u);
@@ -249,7 +252,7 @@ __global__ void __launch_bounds__(Q4Smem<NG>::threads, kQ4PerSm) attn_q4_kernel(
     hi = chunks_of(seq0);
     if (hi == 0) {
       const int hb = r0 % p.head_blocks;
-      for (int k = threadIdx.x; k < kQ4Frags; k += S::threads)
+      for (int k = threadIdx.x; k < kQ4Frags; k += kQ4Threads)
         store_frag<T, NG>(p, b0, r0 / p.head_blocks * p.group + hb * p.block_heads,
                           min(p.block_heads, p.group - hb * p.block_heads), k, nothing, 0.f, 0.f);
       return;
@@ -265,7 +268,7 @@ __global__ void __launch_bounds__(Q4Smem<NG>::threads, kQ4PerSm) attn_q4_kernel(
     for (int b = blockIdx.x; b < p.c.rows; b += p.ctas)  // sequences of no tokens belong to no range
       if (seq_of(p, b) == 0)
         for (int h = 0; h < p.num_q_heads; h += kQ4Heads)
-          for (int k = threadIdx.x; k < kQ4Frags; k += S::threads)
+          for (int k = threadIdx.x; k < kQ4Frags; k += kQ4Threads)
             store_frag<T, NG>(p, b, h, p.num_q_heads - h, k, nothing, 0.f, 0.f);
     per = range_of(p, total);
     if ((long long)blockIdx.x * per >= total) return;
@@ -745,7 +748,7 @@ __global__ void __launch_bounds__(Q4Smem<NG>::threads, kQ4PerSm) attn_q4_kernel(
         den[e] = fmaf(sm_l[w * kQ4Heads + 2 * cq + e], ex2(sm_m[w * kQ4Heads + 2 * cq + e] - gm[e]), den[e]);
     // The output, or a piece of it; a thread's float4s are all of heads 2 cq and + 1.
     const long long slot = 2ll * blockIdx.x + (s0 == lo ? 0 : 1);
-    for (int k = threadIdx.x; k < kQ4Frags; k += S::threads) {
+    for (int k = threadIdx.x; k < kQ4Frags; k += kQ4Threads) {
       if (whole)
         store_frag<T, NG>(p, row_b, h0, nh, k, sm_o[k], den[0], den[1]);
       else
@@ -767,7 +770,7 @@ __global__ void __launch_bounds__(Q4Smem<NG>::threads, kQ4PerSm) attn_q4_kernel(
       __syncthreads();
       if (*last) {
         __threadfence();
-        merge_row<T, NG>(p, row_b, h0, nh, row_begin, row_end, per, S::threads);
+        merge_row<T, NG>(p, row_b, h0, nh, row_begin, row_end, per, kQ4Threads);
       }
     }
     __syncthreads();  // statistics and outputs are free again
@@ -810,7 +813,7 @@ cudaError_t launch_attn(const AttnQ4Params &p, int rows, cudaStream_t s) {
   auto kern = attn_q4_kernel<T, NG, P>;
   cudaError_t e = prepare_kernel_attributes(reinterpret_cast<const void *>(kern));
   if (e != cudaSuccess) return e;
-  e = launch_ex(kern, dim3(p.ctas), dim3(Q4Smem<NG>::threads), Q4Smem<NG>::bytes, s, 1, p.pdl != 0, p);
+  e = launch_ex(kern, dim3(p.ctas), dim3(kQ4Threads), Q4Smem<NG>::bytes, s, 1, p.pdl != 0, p);
   if (e != cudaSuccess || p.by_row || p.counters) return e;
   return launch_ex(attn_q4_merge_kernel<T, NG>, dim3(rows), dim3(kQ4Frags), 0, s, 1, p.pdl != 0, p);
 }
@@ -838,7 +841,7 @@ cudaError_t launch_attn_t(const AttnQ4Params &p, int rows, cudaStream_t s) {
 // the GPU holds at once, or as there can be warps with a chunk.
 struct Q4Plan {
   long long rows;
-  int ctas, warps, by_row;
+  int ctas, by_row;
   long long scratch_floats;
 };
 
@@ -848,10 +851,9 @@ Q4Plan q4_plan(const dak_kv4_cache *c, int num_q_heads, int max_seq_len) {
   plan.rows = (long long)c->batch * c->kv_heads * ((group + kQ4Heads - 1) / kQ4Heads);
   const long long chunks = ((long long)max_seq_len + kQ4Chunk - 1) / kQ4Chunk;
   const int resident = device_sms() * kQ4PerSm;
-  plan.warps = c->group == 32 ? Q4Smem<4>::warps : Q4Smem<1>::warps;
   plan.by_row = plan.rows <= resident && chunks <= kQ4RowChunks;
   plan.ctas = plan.by_row ? (int)plan.rows
-                          : (int)std::min<long long>(resident, (plan.rows * chunks + plan.warps - 1) / plan.warps);
+                          : (int)std::min<long long>(resident, (plan.rows * chunks + kQ4Warps - 1) / kQ4Warps);
   plan.scratch_floats = plan.by_row ? 0 : 2ll * plan.ctas * kQ4Heads * (kKv4Dim + 2);
   return plan;
 }
@@ -936,7 +938,6 @@ extern "C" int dak_attn_decode_paged_q4(const dak_kv4_cache *cache, const dak_at
   p.block_heads = (p.group + p.head_blocks - 1) / p.head_blocks;
   p.max_seq_len = a->max_seq_len;
   p.ctas = plan.ctas;
-  p.warps = plan.warps;
   p.by_row = plan.by_row;
   p.scale_log2 = a->scaling * 1.4426950408889634f;
   p.pdl = decode_pdl_enabled() ? 1 : 0;

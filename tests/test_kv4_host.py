@@ -91,7 +91,7 @@ def test_attention_scratch():
     c = _cache()
     assert _lib.LIB.dak_attn_q4_scratch(ctypes.byref(c), 4, 32) == 0 == kv4.scratch_floats(3, 4, 2, 16, 32, 32)
     assert _lib.LIB.dak_attn_q4_scratch(ctypes.byref(c), 5, 32) < 0
-    assert kv4.scratch_floats(1, 8, 1, 64, 128, 513) == 2 * 2 * 8 * 130  # 9 chunks: 2 CTAs of 6 warps
+    assert kv4.scratch_floats(1, 8, 1, 64, 128, 513) == 2 * 3 * 8 * 130  # 9 chunks: 3 CTAs of 4 warps
     sms = _lib.constants().num_sms
     assert kv4.scratch_floats(64, 64, 8, 64, 128, 16384) == 2 * 2 * sms * 8 * 130  # two CTAs per SM
     c.max_pages = c.table_stride = 64
