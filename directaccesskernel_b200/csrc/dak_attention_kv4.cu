@@ -121,6 +121,24 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// D += A (16x32 unsigned bytes, row) * B (32x8 bytes, col; signed or not), int32.
+template <bool kSigned>
+__device__ __forceinline__ void mma_u8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  if constexpr (kSigned)
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // The transpose of an 8x8 matrix of 16-bit elements spread over the warp.
 __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
   uint32_t d;
@@ -365,55 +383,90 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
   for (int j = 0; j < kQ4Stages; ++j)
     if (at < hi) issue();
 
-  // Query of head g: scaled by a power of two to below 2^14 and to float16 (the
-  // values that float16 cannot hold are 2^-38 of the largest), and summed
-  // over each group for the zeros' share.
+  // Scores.  With groups of 64 or 128 dims they are formed in integers: a byte of
+  // codes is n_even + 16 n_odd, so with integers A = q_odd S / 16 and
+  // B = q_even S - A for a power of two S,
+  //   sum q n S = sum A * byte + B * (byte & 15)
+  // and half of the codes need no unpacking.  S takes the largest |q| to 2^18: A
+  // has 16 bits and B 20, as bytes for the MMAs the high one signed and the
+  // others unsigned; what is dropped is below 2^-15 of the largest |q|.  With
+  // groups of 32 dims the integer sums would not fill an MMA: there the codes are
+  // taken out one by one as float16 subnormals and meet q in float16, scaled by a
+  // power of two to below 2^14.
+  constexpr bool kIntegers = NG < 4;
+  uint32_t qa[2][2][2], qb[3][2][2];  // [digit, low first][word pair][word]
   uint32_t qf[8][2];
-  float qs[2][NG], f[2];
+  float qs[2][NG], f[2];  // q summed over each group (for the zeros' share); raw scores to base 2
   auto ready_query = [&]() {
-    float x[4][8], mx = 0.f, sum[NG];
+    float x[4][8], mx = 0.f, bad = 0.f, sum[NG];
 #pragma unroll
     for (int n = 0; n < NG; ++n) sum[n] = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const uint4 v = qraw[w];
-      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+      const uint32_t u[4] = {qraw[w].x, qraw[w].y, qraw[w].z, qraw[w].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 y = Elem<T>::to_float2(u[e]);
         x[w][2 * e] = y.x;
         x[w][2 * e + 1] = y.y;
-        mx = fmaxf(mx, fmaxf(fabsf(y.x), fabsf(y.y)));
+        mx = max3(mx, fabsf(y.x), fabsf(y.y));
+        bad += y.x * 0.f + y.y * 0.f;  // NaN for a query that is not finite
       }
     }
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    const int k = mx > 0.f ? max(-100, min(100, 13 - ((int)(__float_as_uint(mx) >> 23) - 127))) : 0;
+    bad += __shfl_xor_sync(0xffffffffu, bad, 1);
+    bad += __shfl_xor_sync(0xffffffffu, bad, 2);
+    constexpr int kTop = kIntegers ? 18 : 13;
+    const int k = mx > 0.f ? max(-100, min(100, kTop - ((int)(__float_as_uint(mx) >> 23) - 127))) : 0;
     // A negative scaling turns the query over, so that a larger raw score is
     // always a larger score.
     const float up = copysignf(__uint_as_float((uint32_t)(127 + k) << 23), p.scale_log2);
+    if constexpr (kIntegers) {
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
+      for (int w = 0; w < 4; ++w) {
+        uint32_t da[2] = {0u, 0u}, db[3] = {0u, 0u, 0u};
+        int total = 0;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float a = x[w][2 * h] * up, c = x[w][2 * h + 4] * up;
-        const float d = x[w][2 * h + 1] * up, e = x[w][2 * h + 5] * up;
-        qf[2 * w + h][0] = pack_half2(a, c);
-        qf[2 * w + h][1] = pack_half2(d * 0.0625f, e * 0.0625f);
-        sum[w * NG / 4] += (a + c) + (d + e);
+        for (int j = 0; j < 4; ++j) {
+          const int odd = __float2int_rn(x[w][2 * j + 1] * up * 0.0625f), even = __float2int_rn(x[w][2 * j] * up);
+          const int rest = even - odd;
+          total += even + 16 * odd;
+#pragma unroll
+          for (int d = 0; d < 2; ++d) da[d] |= ((uint32_t)odd >> (8 * d) & 255u) << (8 * j);
+#pragma unroll
+          for (int d = 0; d < 3; ++d) db[d] |= ((uint32_t)rest >> (8 * d) & 255u) << (8 * j);
+        }
+#pragma unroll
+        for (int d = 0; d < 2; ++d) qa[d][w >> 1][w & 1] = da[d];
+#pragma unroll
+        for (int d = 0; d < 3; ++d) qb[d][w >> 1][w & 1] = db[d];
+        sum[w * NG / 4] += (float)total;
       }
+    } else {
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float a = x[w][2 * h] * up, c = x[w][2 * h + 4] * up;
+          const float d = x[w][2 * h + 1] * up, e = x[w][2 * h + 5] * up;
+          qf[2 * w + h][0] = pack_half2(a, c);
+          qf[2 * w + h][1] = pack_half2(d * 0.0625f, e * 0.0625f);
+          sum[w * NG / 4] += ((a + c) + (d + e)) * 0x1p-24f;
+        }
+    }
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
       sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 1);
       sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 2);
     }
-    const float fh = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 + 24 - k) << 23);
+    const float fh = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 + (kIntegers ? 0 : 24) - k) << 23) + bad;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {  // lane 4h holds head h
       const int src = 4 * (2 * cq + e);
       f[e] = __shfl_sync(0xffffffffu, fh, src);
 #pragma unroll
-      for (int n = 0; n < NG; ++n) qs[e][n] = __shfl_sync(0xffffffffu, sum[n], src) * 0x1p-24f;
+      for (int n = 0; n < NG; ++n) qs[e][n] = __shfl_sync(0xffffffffu, sum[n], src);
     }
   };
 
@@ -463,8 +516,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       if (!kFull && t * 16 >= valid) continue;
-      // S^T = K Q^T with the codes as they are: a nibble at bits 0-3 of a half word
-      // is the subnormal code * 2^-24, at bits 4-7 code * 2^-20 (its q is / 16).
+      // S^T = K Q^T
       uint32_t w0[4], w1[4];  // tokens g and g + 8
       if constexpr (NG == 1) {
         const uint8_t *a = st + swz(rows_at(t), g, 16 * cq);
@@ -497,14 +549,34 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       }
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        float acc[4];
+        if constexpr (kIntegers) {
+          int c[3][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};  // by digit
 #pragma unroll
-        for (int w = n * 4 / NG; w < (n + 1) * 4 / NG; ++w) {
-          mma_f16(acc, w0[w] & 0x000F000Fu, w1[w] & 0x000F000Fu, w0[w] & 0x00F000F0u, w1[w] & 0x00F000F0u, qf[2 * w][0],
-                  qf[2 * w][1]);
-          const uint32_t s0 = w0[w] >> 8, s1 = w1[w] >> 8;
-          mma_f16(acc, s0 & 0x000F000Fu, s1 & 0x000F000Fu, s0 & 0x00F000F0u, s1 & 0x00F000F0u, qf[2 * w + 1][0],
-                  qf[2 * w + 1][1]);
+          for (int v = n * 2 / NG; v < (n + 1) * 2 / NG; ++v) {
+            const uint32_t a0 = w0[2 * v], a1 = w1[2 * v], a2 = w0[2 * v + 1], a3 = w1[2 * v + 1];
+            const uint32_t l0 = a0 & 0x0F0F0F0Fu, l1 = a1 & 0x0F0F0F0Fu, l2 = a2 & 0x0F0F0F0Fu, l3 = a3 & 0x0F0F0F0Fu;
+            mma_u8<false>(c[0], a0, a1, a2, a3, qa[0][v][0], qa[0][v][1]);
+            mma_u8<true>(c[1], a0, a1, a2, a3, qa[1][v][0], qa[1][v][1]);
+            mma_u8<false>(c[0], l0, l1, l2, l3, qb[0][v][0], qb[0][v][1]);
+            mma_u8<false>(c[1], l0, l1, l2, l3, qb[1][v][0], qb[1][v][1]);
+            mma_u8<true>(c[2], l0, l1, l2, l3, qb[2][v][0], qb[2][v][1]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] = (float)(c[2][e] * 65536 + c[1][e] * 256 + c[0][e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] = 0.f;
+          // A nibble at bits 0-3 of a half word is the subnormal code * 2^-24, at bits
+          // 4-7 code * 2^-20 (its q is / 16).
+#pragma unroll
+          for (int w = n * 4 / NG; w < (n + 1) * 4 / NG; ++w) {
+            mma_f16(acc, w0[w] & 0x000F000Fu, w1[w] & 0x000F000Fu, w0[w] & 0x00F000F0u, w1[w] & 0x00F000F0u, qf[2 * w][0],
+                    qf[2 * w][1]);
+            const uint32_t s0 = w0[w] >> 8, s1 = w1[w] >> 8;
+            mma_f16(acc, s0 & 0x000F000Fu, s1 & 0x000F000Fu, s0 & 0x00F000F0u, s1 & 0x00F000F0u, qf[2 * w + 1][0],
+                    qf[2 * w + 1][1]);
+          }
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -517,10 +589,14 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
         }
       }
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (kFull || t * 16 + 8 * r + g < valid) mx[e] = fmaxf(mx[e], y[t][2 * r + e]);
+      for (int e = 0; e < 2; ++e) {
+        if (kFull) {
+          mx[e] = max3(mx[e], y[t][e], y[t][2 + e]);
+        } else {
+          if (t * 16 + g < valid) mx[e] = fmaxf(mx[e], y[t][e]);
+          if (t * 16 + 8 + g < valid) mx[e] = fmaxf(mx[e], y[t][2 + e]);
+        }
+      }
     }
     // A larger V scale than any before raises E (rarely, after the first chunks).
     const uint32_t sm = __reduce_max_sync(0xffffffffu, *reinterpret_cast<const uint32_t *>(&vmax) & 0xffffu);
@@ -675,7 +751,8 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
     s_max = 0u;
     for (; lo + warp + W * done < s1; ++done) {
       const int id = lo + warp + W * done, s = done % kQ4Stages;
-      const bool ok = dead_at < 0 && mbar_wait<false>(bar0 + 8 * s, (done / kQ4Stages) & 1, wc);
+      const uint32_t parity = (done / kQ4Stages) & 1;
+      const bool ok = dead_at < 0 && (mbar_try_wait(bar0 + 8 * s, parity) || mbar_wait<false>(bar0 + 8 * s, parity, wc));
       if (!__all_sync(0xffffffffu, ok)) {  // give up, but keep to the barriers below
         if (dead_at < 0) dead_at = done;
         continue;
