@@ -74,6 +74,8 @@ def parse_args():
     ap.add_argument("--layers", type=int, default=80, help="llama70b: decoder layers")
     ap.add_argument("--batch", type=int, default=32, help="llama70b: sequences")
     ap.add_argument("--ctx", type=int, default=16384, help="llama70b: context tokens per sequence")
+    ap.add_argument("--kv-bits", type=int, choices=[16, 4], default=16,
+                    help="llama70b: 4 keeps the KV cache in 4-bit codes")
     ap.add_argument("--breakdown", action="store_true",
                     help="llama70b: after the timed region, one eager step with CUDA events around every op group "
                          "(per-op milliseconds in the JSON line)")
@@ -1239,8 +1241,8 @@ def run_llama70b(args, torch, rank, world):
     max_ctx = ctx + W + 2 * K + 4
     budget_gb = 60.0 if args.hbm_budget_gb is None else args.hbm_budget_gb
     frac = (args.host_fraction if args.host_fraction is not None
-            else budget_fraction(shape, world, B, max_ctx, int(budget_gb * 1e9)))
-    per_rank_total = shape.weight_bytes_per_rank(world) + shape.kv_bytes_per_rank(world, B, max_ctx)
+            else budget_fraction(shape, world, B, max_ctx, int(budget_gb * 1e9), args.kv_bits))
+    per_rank_total = shape.weight_bytes_per_rank(world) + shape.kv_bytes_per_rank(world, B, max_ctx, kv_bits=args.kv_bits)
     host_need = frac * per_rank_total * world
     # The ranks share the box's host-memory bandwidth unevenly; give each rank a
     # share of the host bytes proportional to its concurrently measured
@@ -1260,7 +1262,7 @@ def run_llama70b(args, torch, rank, world):
     t0 = time.perf_counter()
     fused = world > 1 and not args.nccl_allreduce
     dec = TPLlamaDecoder(shape, batch=B, max_ctx=max_ctx, weight_offload=my_frac, kv_host_fraction=my_frac,
-                         fused_allreduce=fused)
+                         fused_allreduce=fused, kv_bits=args.kv_bits)
     dec.init_random(seed=0)
     dec.fill_kv_random(ctx, seed=1)
     g = torch.Generator().manual_seed(3)
@@ -1345,7 +1347,8 @@ def run_llama70b(args, torch, rank, world):
         "data": "synthetic: random N(0,0.02) weights, N(0,1) KV for the context, random token ids",
         "config": {"workload": f"BASELINE config 5: Llama-3-70B arch, {shape.layers} layers, batch {B}, ctx {ctx}, "
                                f"TP{world}, per-GPU HBM budget {budget_gb:g} GB"
-                               + ("" if args.host_fraction is None else f", fixed host fraction {frac:g}"),
+                               + ("" if args.host_fraction is None else f", fixed host fraction {frac:g}")
+                               + ("" if args.kv_bits == 16 else ", KV cache in 4 bits (groups of 128)"),
                    "host_fraction": round(frac, 4), "per_rank_host_fractions": [round(f, 4) for f in fracs],
                    "rank0_host_bytes": int(lin_host + kv_host),
                    "rank0_device_bytes": int(lin_dev + kv_dev), "build_s": round(build_s, 1),

@@ -15,6 +15,8 @@ paged (64-token pages): the first pages of every sequence live in pinned host
 memory, the rest in HBM; ``attention.rope_kv_append`` rotates each new token's
 k and writes it with v straight into its page, and ``attention.decode_paged``
 reads both tiers in one launch.  A decode step, greedy pick included, is one CUDA graph.
+With ``kv_bits=4`` the pages hold 4-bit codes (``kv4``): a quarter of the bytes on
+the host link, and ``fork`` copies a sequence's pages to another row either way.
 
 The layer arithmetic follows transformers' Llama (RMSNorm in FP32, rotary
 embedding in the activation dtype, SiLU-gated MLP), which is also what the
@@ -31,7 +33,7 @@ import torch
 import torch.distributed as dist
 from torch import nn
 
-from .attention import auto_split_size, decode_paged, rope_kv_append
+from .attention import auto_split_size, decode_paged, kv_append_paged, rope_kv_append
 
 # Tokens per KV page.  One page of one KV head is a TMA box of page x 64 dims per
 # half head; 64-token pages give 8 KB boxes, which stream from HBM about twice
@@ -50,6 +52,8 @@ class LlamaShape:
     vocab: int
     rope_theta: float
     eps: float
+    rope_scaling: dict | None = None  # the configuration's rope dictionary where it is not the default rotary
+    max_position: int | None = None
 
     @classmethod
     def from_config(cls, cfg) -> "LlamaShape":
@@ -58,10 +62,12 @@ class LlamaShape:
         theta = rope.get("rope_theta", getattr(cfg, "rope_theta", None))
         if theta is None:
             theta = 10000.0
-        if rope.get("rope_type", "default") != "default":
-            raise ValueError(f"rope_type {rope.get('rope_type')!r} is not supported (default rotary only)")
+        kind = rope.get("rope_type", rope.get("type", "default"))
+        if kind not in ("default", "linear", "llama3", "yarn"):
+            raise ValueError(f"rope_type {kind!r} is not supported (default, linear, llama3 or yarn)")
         return cls(cfg.hidden_size, cfg.num_hidden_layers, cfg.num_attention_heads, cfg.num_key_value_heads, hd,
-                   cfg.intermediate_size, cfg.vocab_size, float(theta), float(cfg.rms_norm_eps))
+                   cfg.intermediate_size, cfg.vocab_size, float(theta), float(cfg.rms_norm_eps),
+                   None if kind == "default" else dict(rope), getattr(cfg, "max_position_embeddings", None))
 
     def weight_bytes_per_rank(self, world: int, dtype_bytes: int = 2) -> int:
         """Bytes of this rank's linears, norms and the replicated embedding."""
@@ -70,8 +76,13 @@ class LlamaShape:
         vocab_r = -(-self.vocab // world)
         return dtype_bytes * (self.layers * (per_layer + 2 * h) + h + self.vocab * h + vocab_r * h)
 
-    def kv_bytes_per_rank(self, world: int, batch: int, ctx: int, dtype_bytes: int = 2) -> int:
+    def kv_bytes_per_rank(self, world: int, batch: int, ctx: int, dtype_bytes: int = 2, kv_bits: int = 16,
+                          kv_group: int = 128) -> int:
         pages = -(-ctx // PAGE)
+        if kv_bits == 4:
+            from .kv4 import page_bytes
+
+            return self.layers * batch * pages * (self.kv_heads // world) * page_bytes(PAGE, kv_group)
         return dtype_bytes * 2 * self.layers * batch * pages * PAGE * (self.kv_heads // world) * self.head_dim
 
 
@@ -82,10 +93,12 @@ def vocab_rows_per_rank(vocab: int, world: int) -> int:
     return -(-vocab // (world * 64)) * 64
 
 
-def budget_fraction(shape: LlamaShape, world: int, batch: int, ctx: int, hbm_budget_bytes: int) -> float:
+def budget_fraction(shape: LlamaShape, world: int, batch: int, ctx: int, hbm_budget_bytes: int,
+                    kv_bits: int = 16, kv_group: int = 128) -> float:
     """Host fraction f of both weights and KV such that (1 - f) x (this rank's weights
     + KV) fits the per-GPU HBM budget (0 when everything fits)."""
-    total = shape.weight_bytes_per_rank(world) + shape.kv_bytes_per_rank(world, batch, ctx)
+    total = shape.weight_bytes_per_rank(world) + shape.kv_bytes_per_rank(world, batch, ctx, kv_bits=kv_bits,
+                                                                         kv_group=kv_group)
     return max(0.0, 1.0 - hbm_budget_bytes / total)
 
 
@@ -103,12 +116,19 @@ class TPLlamaDecoder(nn.Module):
     ``weight_offload`` is the host fraction of every linear shard (split by
     ``LinearHorizontal`` at 64-feature granularity); ``kv_host_fraction`` is the
     fraction of each sequence's KV pages kept in pinned host memory (its first
-    pages).  ``max_ctx`` bounds the tokens a sequence can hold."""
+    pages).  ``max_ctx`` bounds the tokens a sequence can hold.  ``kv_bits=4`` keeps
+    the KV in 4-bit codes with a scale and a zero per ``kv_group`` dims (128, 64 or
+    32: fewer are more exact and take more bytes)."""
+
+    kv_bits, rope_scale = 16, 1.0
 
     def __init__(self, shape: LlamaShape, *, batch: int, max_ctx: int, weight_offload: float = 0.0,
                  kv_host_fraction: float = 0.0, group=None, dtype=torch.float16, device="cuda",
-                 fused_allreduce: bool = False):
+                 fused_allreduce: bool = False, kv_bits: int = 16, kv_group: int = 128):
         super().__init__()
+        if kv_bits not in (4, 16):
+            raise ValueError("kv_bits must be 16 or 4")
+        self.kv_bits, self.kv_group = kv_bits, kv_group
         self.s = shape
         self.group = group
         self.world = dist.get_world_size(group) if dist.is_initialized() else 1
@@ -243,14 +263,20 @@ class TPLlamaDecoder(nn.Module):
         self.pages_per_seq, self.host_pages_per_seq = pages, n_host
         B, L, hkv, d = self.B, self.s.layers, self.hkv, self.s.head_dim
         dev_pages, host_pages = B * (pages - n_host), B * n_host
-        self.kv_dev = (torch.empty(L, 2, dev_pages, hkv, PAGE, d, dtype=self.dtype, device=self.device)
-                       if dev_pages else None)
-        self.kv_host = (torch.empty(L, 2, host_pages, hkv, PAGE, d, dtype=self.dtype, pin_memory=True)
-                        if host_pages else None)
+        if self.kv_bits == 4:
+            from .kv4 import page_bytes
+
+            lead, rest, dt = (L,), (hkv, page_bytes(PAGE, self.kv_group)), torch.uint8
+        else:
+            lead, rest, dt = (L, 2), (hkv, PAGE, d), self.dtype
+        self.page_dim = len(lead)  # of the pools
+        self.kv_dev = torch.empty(*lead, dev_pages, *rest, dtype=dt, device=self.device) if dev_pages else None
+        self.kv_host = torch.empty(*lead, host_pages, *rest, dtype=dt, pin_memory=True) if host_pages else None
         table = torch.empty(B, pages, dtype=torch.int32)
         for b in range(B):
             for j in range(pages):
                 table[b, j] = (-1 - (b * n_host + j)) if j < n_host else b * (pages - n_host) + (j - n_host)
+        self.host_table = table
         self.block_table = table.to(self.device)
         self.split = auto_split_size(B, hkv, self.max_ctx)
 
@@ -263,8 +289,13 @@ class TPLlamaDecoder(nn.Module):
     @torch.no_grad()
     def fill_kv_random(self, ctx: int, seed: int = 0) -> None:
         """Stands in for a prefill of ``ctx`` tokens per sequence: N(0, 1) K/V in every
-        page, positions set so that the next decode step writes token ``ctx``."""
+        page (4-bit: random codes over the range that N(0, 1) would have), positions
+        set so that the next decode step writes token ``ctx``."""
         g = torch.Generator(device=self.device).manual_seed(seed + 7 * self.rank)
+        if self.kv_bits == 4:
+            self._fill_kv4_random(g)
+            self.set_positions(ctx)
+            return
         if self.kv_dev is not None:
             self.kv_dev.normal_(generator=g)
         if self.kv_host is not None:
@@ -276,7 +307,48 @@ class TPLlamaDecoder(nn.Module):
         torch.cuda.synchronize()
         self.set_positions(ctx)
 
+    def _fill_kv4_random(self, g: torch.Generator) -> None:
+        from .kv4 import page_bytes
+
+        # 16 steps from -2.6 to 2.6, about the extremes of 128 draws.
+        pair = torch.tensor([5.2 / 15, -2.6], dtype=torch.float16).view(torch.uint8)
+        half = page_bytes(PAGE, self.kv_group) // 2
+        slab = torch.empty(1, 2 * half, dtype=torch.uint8, device=self.device)
+        for at in (0, half):
+            slab[:, at + PAGE * 64:at + half] = pair.repeat((half - PAGE * 64) // 4).to(self.device)
+        codes = torch.zeros(2 * half, dtype=torch.bool, device=self.device)
+        codes[:PAGE * 64] = codes[half:half + PAGE * 64] = True
+        for pool in (self.kv_dev, self.kv_host):
+            if pool is None:
+                continue
+            flat = pool.view(-1, 2 * half)
+            step = max(1, (1 << 26) // half)
+            for i in range(0, flat.shape[0], step):
+                n = min(step, flat.shape[0] - i)
+                fill = torch.randint(0, 256, (n, 2 * half), generator=g, device=self.device, dtype=torch.uint8)
+                flat[i:i + n].copy_(torch.where(codes, fill, slab))
+        torch.cuda.synchronize()
+
+    @torch.no_grad()
+    def fork(self, src: int, dst: int, tokens: int) -> None:
+        """Makes row ``dst`` continue row ``src`` after its first ``tokens`` tokens: copies
+        the pages that hold them, in every layer and tier, with one launch on the
+        current stream, and the row's next token and position."""
+        if not (0 <= src < self.B and 0 <= dst < self.B) or src == dst:
+            raise ValueError(f"src and dst must be two different rows of {self.B}")
+        if not 0 <= tokens <= self.max_ctx:
+            raise ValueError(f"tokens must be within 0..{self.max_ctx}")
+        from .kv_pages import copy_pages
+
+        n = -(-tokens // PAGE)
+        copy_pages(self.kv_dev, self.kv_host, self.host_table[src, :n], self.host_table[dst, :n], page_dim=self.page_dim)
+        self.ids[dst].copy_(self.ids[src])
+        self.pos[dst].copy_(self.pos[src])
+
     def _pools(self, l: int):
+        if self.kv_bits == 4:
+            return (self.kv_dev[l] if self.kv_dev is not None else None,
+                    self.kv_host[l] if self.kv_host is not None else None)
         kd = self.kv_dev[l, 0] if self.kv_dev is not None else None
         vd = self.kv_dev[l, 1] if self.kv_dev is not None else None
         kh = self.kv_host[l, 0] if self.kv_host is not None else None
@@ -290,13 +362,27 @@ class TPLlamaDecoder(nn.Module):
         self.pos = torch.zeros(B, dtype=torch.int32, device=self.device)
         self.seq_lens = torch.ones(B, dtype=torch.int32, device=self.device)
         self.attn_out = torch.empty(B, self.hq, d, dtype=self.dtype, device=self.device)
-        ns = -(-self.max_ctx // auto_split_size(B, self.hkv, self.max_ctx))
-        self.partial_o = torch.empty(B, self.hq, ns, d, dtype=torch.float32, device=self.device)
-        self.partial_ml = torch.empty(B, self.hq, ns, 2, dtype=torch.float32, device=self.device)
+        counters = B * self.hkv
+        if self.kv_bits == 4:
+            from .kv4 import merge_counter_count, scratch_floats
+
+            counters = merge_counter_count(B, self.hq, self.hkv)
+            self.scratch = torch.empty(scratch_floats(B, self.hq, self.hkv, PAGE, self.kv_group, self.max_ctx),
+                                       dtype=torch.float32, device=self.device)
+        else:
+            ns = -(-self.max_ctx // auto_split_size(B, self.hkv, self.max_ctx))
+            self.partial_o = torch.empty(B, self.hq, ns, d, dtype=torch.float32, device=self.device)
+            self.partial_ml = torch.empty(B, self.hq, ns, 2, dtype=torch.float32, device=self.device)
         # The last split of each (sequence, KV head) merges in the attention
         # kernel; every call leaves these counters at zero.
-        self.merge_counters = torch.zeros(B * self.hkv, dtype=torch.int32, device=self.device)
-        self.inv_freq = 1.0 / (self.s.rope_theta ** (torch.arange(0, d, 2, dtype=torch.float32, device=self.device) / d))
+        self.merge_counters = torch.zeros(counters, dtype=torch.int32, device=self.device)
+        if self.s.rope_scaling is None:
+            self.inv_freq = 1.0 / (self.s.rope_theta ** (torch.arange(0, d, 2, dtype=torch.float32, device=self.device) / d))
+        else:
+            from .decode_ops import rope_frequencies
+
+            self.inv_freq, self.rope_scale = rope_frequencies(d, self.s.rope_theta, self.s.rope_scaling,
+                                                              self.s.max_position, device=self.device)
         self.next_ids = torch.zeros(B, dtype=torch.long, device=self.device)
         self.logits_full = None
         h = self.s.hidden
@@ -350,6 +436,40 @@ class TPLlamaDecoder(nn.Module):
         wh, wd = self._tiers(mod)
         return linear_split(x, out, wh, wd, glu=True)
 
+    def _attend(self, l: int, qkv: torch.Tensor, scale: float) -> None:
+        """Rotates layer l's q and k, appends k and v to its pages and leaves the
+        attention of every sequence in ``attn_out``."""
+        B, d, t = self.B, self.s.head_dim, self._span
+        if self.kv_bits == 4:
+            from .kv4 import decode_paged_q4, rope_kv_append_q4
+
+            dev, host = self._pools(l)
+            with t("rope+kv_append"):
+                rope_kv_append_q4(qkv, self.pos, self.inv_freq, self.hq, self.q_buf, dev, host, self.block_table,
+                                  rope_scale=self.rope_scale)
+            with t("attention"):
+                decode_paged_q4(self.q_buf, dev, host, self.block_table, self.seq_lens, scale, out=self.attn_out,
+                                scratch=self.scratch, max_seq_len=self.max_ctx, merge_counters=self.merge_counters)
+            return
+        kdev, vdev, khost, vhost = self._pools(l)
+        q = self.q_buf
+        with t("rope+kv_append"):
+            if self.rope_scale == 1.0:
+                rope_kv_append(qkv, self.pos, self.inv_freq, self.hq, self.hkv, d, q, kdev, vdev, khost, vhost,
+                               self.block_table)
+            else:  # the attention factor of a scaled rotary
+                from .decode_ops import rotary
+
+                heads = qkv.view(B, self.hq + 2 * self.hkv, d)
+                q, k, v = heads.split([self.hq, self.hkv, self.hkv], dim=1)
+                rotary(heads[:, :self.hq + self.hkv], self.pos, self.inv_freq, rope_scale=self.rope_scale,
+                       out=heads[:, :self.hq + self.hkv])
+                kv_append_paged(k, v, kdev, vdev, khost, vhost, self.block_table, self.pos)
+        with t("attention"):
+            decode_paged(q, kdev, vdev, khost, vhost, self.block_table, self.seq_lens, scale, self.split,
+                         out=self.attn_out, partial_o=self.partial_o, partial_ml=self.partial_ml,
+                         max_seq_len=self.max_ctx, merge_counters=self.merge_counters)
+
     def forward_step(self, keep_logits: bool = False) -> torch.Tensor:
         """One decode step on the static buffers: embeds ``ids`` at ``pos``, writes
         their K/V, and leaves the greedy tokens in ``next_ids``; advances nothing.
@@ -370,14 +490,7 @@ class TPLlamaDecoder(nn.Module):
         for l, layer in enumerate(self.layers):
             with t("qkv"):
                 qkv = layer.qkv(x)
-            kdev, vdev, khost, vhost = self._pools(l)
-            with t("rope+kv_append"):
-                rope_kv_append(qkv, self.pos, self.inv_freq, self.hq, self.hkv, d, self.q_buf, kdev, vdev, khost,
-                               vhost, self.block_table)
-            with t("attention"):
-                decode_paged(self.q_buf, kdev, vdev, khost, vhost, self.block_table, self.seq_lens, scale,
-                             self.split, out=self.attn_out, partial_o=self.partial_o, partial_ml=self.partial_ml,
-                             max_seq_len=self.max_ctx, merge_counters=self.merge_counters)
+            self._attend(l, qkv, scale)
             with t("o" if self.use_fused else "o+allreduce"):
                 o = self._row_parallel(layer.o, self.attn_out.view(B, qd), self.o_buf)
             with t("allreduce+norm" if self.use_fused else "norm"):
@@ -457,10 +570,11 @@ class TPLlamaDecoder(nn.Module):
         """Launches of this library's kernels in one ``forward_step``: the first
         RMSNorm; per layer the four linears (gate_up also applies the SiLU gate
         when ``fuse_glu``, else a SiLU-gate kernel follows), rotary with the KV
-        append, attention (which also merges its splits) and two RMSNorms; then
+        append (two launches for a 16-bit cache and an attention factor), attention (which also merges its splits) and two RMSNorms; then
         lm_head.  The torch ops around them (embedding gather, greedy pick) and
         NCCL's kernels are not counted."""
-        return 1 + len(self.layers) * (8 if self.fuse_glu else 9) + 1
+        per_layer = (8 if self.fuse_glu else 9) + (self.kv_bits == 16 and self.rope_scale != 1.0)
+        return 1 + len(self.layers) * per_layer + 1
 
     def advance(self) -> None:
         """Feeds the greedy tokens back and moves every sequence one position on."""

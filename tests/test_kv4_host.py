@@ -321,3 +321,24 @@ def test_page_table_move_and_compact_keep_the_contents():
         _check(t)
         for s, rows in want.items():
             assert [data[v] for v in t.pages(s)] == rows
+
+
+# ------------------------------------------------------------ decoder's sizes
+def test_decoder_shapes_with_scaled_rotary_and_4_bit_pages():
+    from directaccesskernel_b200 import decode
+    from directaccesskernel_b200.llama_tp import LlamaShape, budget_fraction
+
+    cfg = decode.llama_config("llama-3-70b")
+    s = LlamaShape.from_config(cfg)
+    assert s.rope_scaling is None
+    # 136, 144 or 160 bytes per token, head and layer instead of 512.
+    full = s.kv_bytes_per_rank(8, 32, 16384)
+    for group, per in ((128, 136), (64, 144), (32, 160)):
+        assert s.kv_bytes_per_rank(8, 32, 16384, kv_bits=4, kv_group=group) * 512 == full * per
+    assert budget_fraction(s, 4, 32, 16384, 60 * 10**9) > 0.2
+    assert budget_fraction(s, 4, 32, 16384, 60 * 10**9, kv_bits=4) == 0.0
+    cfg.rope_parameters = dict(rope_type="yarn", factor=4.0, rope_theta=1e4, original_max_position_embeddings=4096)
+    assert LlamaShape.from_config(cfg).rope_scaling["factor"] == 4.0
+    cfg.rope_parameters = dict(rope_type="longrope", factor=4.0, rope_theta=1e4)
+    with pytest.raises(ValueError, match="not supported"):
+        LlamaShape.from_config(cfg)
