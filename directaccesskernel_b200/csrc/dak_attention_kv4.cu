@@ -10,8 +10,6 @@
 // fourth chunk, with copies running ahead across rows.  A row that spans CTAs is
 // merged by log-sum-exp.  Scores are kept in base 2; a sequence of no tokens
 // gives zeros.
-#include <cudaTypedefs.h>
-
 #include <cfloat>
 #include <cstring>
 #include <type_traits>
@@ -36,8 +34,7 @@ constexpr int kQ4Stages = 2;   // chunks in flight per warp
 constexpr int kQ4MergeBatch = 8;  // pieces of a row read at once
 constexpr int kQ4RowChunks = 8;  // rows up to this long are not split while the GPU holds them all
 
-struct alignas(64) AttnQ4Params {
-  CUtensorMap map[2];  // device, host pool: dims {64 bytes, slab rows, pages x heads}
+struct AttnQ4Params {
   Kv4Cache c;
   const uint16_t *query;
   long long q_stride_b, q_stride_h;
@@ -63,27 +60,9 @@ struct Q4Smem {
   static constexpr uint32_t l_off = m_off + kQ4Warps * kQ4Heads * 4;
   static constexpr uint32_t bar_off = l_off + kQ4Warps * kQ4Heads * 4;
   static constexpr uint32_t flag_off = bar_off + kQ4Warps * kQ4Stages * 8;   // abort, abort of the drain, last
-  static constexpr uint32_t bytes = flag_off + 16 + 496;                  // 496: alignment to 512
-  static_assert(stage % 512 == 0, "the swizzle is computed from the offset in a stage");
+  static constexpr uint32_t bytes = flag_off + 16;
   static_assert(kQ4PerSm * (bytes + 1024) <= 228 * 1024, "CTAs per SM");
 };
-
-__device__ __forceinline__ void tma_load_slab(uint32_t dst, const CUtensorMap *map, int slab, uint32_t bar,
-                                              uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      ".L2::cache_hint [%0], [%1, {%2, %2, %3}], [%4], %5;" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(slab), "r"(bar), "l"(policy)
-      : "memory");
-}
-
-// Where the 64-byte TMA swizzle put byte `lb` (below 64) of the row `row` rows
-// after offset C of a stage (C a multiple of 64, the stage 512-byte aligned):
-// bits 4-5 are xored with bits 7-8.  C is a constant at every call, so what
-// depends on the lane is the same few values for all tiles.
-__device__ __forceinline__ uint32_t swz(uint32_t C, uint32_t row, uint32_t lb) {
-  return C + row * 64 + (lb ^ ((((C >> 7) + ((row + ((C >> 6) & 1u)) >> 1)) & 3u) << 4));
-}
 
 // The (scale, zero) words of one token, one per group.
 template <int NG> __device__ __forceinline__ void load_pairs(const uint8_t *a, uint32_t (&w)[NG]) {
@@ -158,6 +137,7 @@ __device__ __forceinline__ float exponent_of(uint32_t bits) {
 // of heads 2c and 2c + 1 as (d, 2c), (d, 2c + 1), (d + 1, 2c), (d + 1, 2c + 1), d
 // being frag_dim.  Every step is then linear in the thread.
 constexpr int kQ4Frags = kQ4Heads * kKv4Dim / 4;
+static_assert(kQ4Frags == 2 * kQ4Threads, "a thread merges two of a row's float4s");
 template <int NG> __device__ __forceinline__ int frag_dim(int t, int g) {
   const int q = t >> 1;
   return (NG == 1 ? 16 * g + 4 * q : NG == 2 ? 64 * (q >> 1) + 8 * g + 4 * (q & 1) : 32 * q + 4 * g) + 2 * (t & 1);
@@ -180,65 +160,74 @@ __device__ __forceinline__ int seq_of(const AttnQ4Params &p, int b) {
 }
 __device__ __forceinline__ int chunks_of(int seq) { return (seq + kQ4Chunk - 1) / kQ4Chunk; }
 
-// Chunks of a CTA's range, given those of all rows: every CTA the same, at least
-// one for each warp.
-__device__ __forceinline__ int range_of(const AttnQ4Params &p, int total) {
-  return max((total + p.ctas - 1) / p.ctas, kQ4Warps);
+// Chunks of a CTA's range, given those of all rows and of the longest: every CTA
+// the same, at least one for each warp.  Merging a row costs the CTA that does it
+// about 0.1 us per piece, against 1.3 us for four chunks, one per warp: a row of n
+// chunks is best cut into about sqrt(9 n) pieces, which matters where one or two
+// rows are all there is.
+__device__ __forceinline__ int range_of(const AttnQ4Params &p, int total, int longest) {
+  return max(max((total + p.ctas - 1) / p.ctas, kQ4Warps), (int)sqrtf(longest * (1.f / 9.f)));
 }
 
 // Merges row (b, r), whose chunks are [begin, end) of all in ranges of `per`, from
 // its pieces in the scratch, in order.  Piece i is CTA i's first segment (slot
 // 2 i), or, if the row begins within CTA i's range, its last (slot 2 i + 1).
 template <typename T, int NG>
-__device__ __forceinline__ void merge_row(const AttnQ4Params &p, int b, int h0, int nh, int begin, int end, int per,
-                                          int threads) {
+__device__ __forceinline__ void merge_row(const AttnQ4Params &p, int b, int h0, int nh, int begin, int end, int per) {
   const int first = begin / per, pieces = (end - 1) / per - first + 1;
   const float4 *po = reinterpret_cast<const float4 *>(p.scratch);
   const float4 *pm = po + 2ll * p.ctas * kQ4Frags;  // (m, l) of two heads
   auto slot = [&](int i) { return 2ll * (first + i) + ((first + i) * per < begin ? 1 : 0); };
-  for (int k = threadIdx.x; k < kQ4Frags; k += threads) {
-    float m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = 0; i0 < pieces; i0 += kQ4MergeBatch) {
-      float4 ml[kQ4MergeBatch], v[kQ4MergeBatch];  // all in flight at once
+  const int k = threadIdx.x;  // this thread's float4s, of the same two heads: k and k + kQ4Threads
+  float m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
+  float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  for (int i0 = 0; i0 < pieces; i0 += kQ4MergeBatch) {
+    float4 ml[kQ4MergeBatch], v[kQ4MergeBatch][2];  // all in flight at once
 #pragma unroll
-      for (int i = 0; i < kQ4MergeBatch; ++i) {
-        const bool in = i0 + i < pieces;
-        const long long at = slot(in ? i0 + i : i0);
-        ml[i] = __ldcg(pm + at * (kQ4Heads / 2) + (k & 3));
-        v[i] = __ldcg(po + at * kQ4Frags + k);
-        if (!in) ml[i] = make_float4(-FLT_MAX, 0.f, -FLT_MAX, 0.f), v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      float n0 = m0, n1 = m1;
+    for (int i = 0; i < kQ4MergeBatch; ++i) {
+      const bool in = i0 + i < pieces;
+      const long long at = slot(in ? i0 + i : i0);
+      ml[i] = __ldcg(pm + at * (kQ4Heads / 2) + (k & 3));
+      if (!in) ml[i] = make_float4(-FLT_MAX, 0.f, -FLT_MAX, 0.f);
 #pragma unroll
-      for (int i = 0; i < kQ4MergeBatch; ++i) n0 = fmaxf(n0, ml[i].x), n1 = fmaxf(n1, ml[i].z);
-      const float a0 = ex2(m0 - n0), a1 = ex2(m1 - n1);
-      m0 = n0, m1 = n1;
-      l0 *= a0, l1 *= a1;
-      acc = make_float4(acc.x * a0, acc.y * a1, acc.z * a0, acc.w * a1);
-#pragma unroll
-      for (int i = 0; i < kQ4MergeBatch; ++i) {
-        const float c0 = ex2(ml[i].x - m0), c1 = ex2(ml[i].z - m1);
-        l0 = fmaf(ml[i].y, c0, l0);
-        l1 = fmaf(ml[i].w, c1, l1);
-        acc.x = fmaf(v[i].x, c0, acc.x);
-        acc.y = fmaf(v[i].y, c1, acc.y);
-        acc.z = fmaf(v[i].z, c0, acc.z);
-        acc.w = fmaf(v[i].w, c1, acc.w);
+      for (int j = 0; j < 2; ++j) {
+        v[i][j] = __ldcg(po + at * kQ4Frags + k + j * kQ4Threads);
+        if (!in) v[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
       }
     }
-    store_frag<T, NG>(p, b, h0, nh, k, acc, l0, l1);
+    float n0 = m0, n1 = m1;
+#pragma unroll
+    for (int i = 0; i < kQ4MergeBatch; ++i) n0 = fmaxf(n0, ml[i].x), n1 = fmaxf(n1, ml[i].z);
+    const float a0 = ex2(m0 - n0), a1 = ex2(m1 - n1);
+    m0 = n0, m1 = n1;
+    l0 *= a0, l1 *= a1;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[j] = make_float4(acc[j].x * a0, acc[j].y * a1, acc[j].z * a0, acc[j].w * a1);
+#pragma unroll
+    for (int i = 0; i < kQ4MergeBatch; ++i) {
+      const float c0 = ex2(ml[i].x - m0), c1 = ex2(ml[i].z - m1);
+      l0 = fmaf(ml[i].y, c0, l0);
+      l1 = fmaf(ml[i].w, c1, l1);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        acc[j].x = fmaf(v[i][j].x, c0, acc[j].x);
+        acc[j].y = fmaf(v[i][j].y, c1, acc[j].y);
+        acc[j].z = fmaf(v[i][j].z, c0, acc[j].z);
+        acc[j].w = fmaf(v[i][j].w, c1, acc[j].w);
+      }
+    }
   }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) store_frag<T, NG>(p, b, h0, nh, k + j * kQ4Threads, acc[j], l0, l1);
 }
 
 template <typename T, int NG, int P>
 __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __grid_constant__ AttnQ4Params p) {
-  extern __shared__ uint8_t smem_raw[];
+  extern __shared__ __align__(128) uint8_t smem[];
   using S = Q4Smem<NG>;
   constexpr int W = kQ4Warps;
   // The weights of a float16 output are split into two float16 terms.
   constexpr bool kTwoTerms = std::is_same<T, __half>::value;
-  uint8_t *smem = smem_raw + ((512u - (smem_u32(smem_raw) & 511u)) & 511u);
   const uint32_t sbase = smem_u32(smem);
   const int warp = warp_id(), lane = lane_id();
   const int g = lane >> 2, cq = lane & 3;  // fragment row, column pair
@@ -251,8 +240,6 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
     for (int s = 0; s < W * kQ4Stages; ++s) mbar_init(sbase + S::bar_off + 8 * s, 1);
     abort_flag[0] = abort_flag[1] = 0;  // [1]: of the wait for copies in flight
     fence_mbar_init();
-    prefetch_tensormap(&p.map[0]);
-    prefetch_tensormap(&p.map[1]);
   }
   pdl_enter(p.pdl);
   __syncthreads();
@@ -278,17 +265,20 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
   } else {
     // Lengths of the first 32 sequences, one per lane; most batches need no more.
     int seqs = lane < p.c.rows ? seq_of(p, lane) : 0;
-    int n = chunks_of(seqs), total = n;
-    for (int b = 32 + lane; b < p.c.rows; b += 32) total += chunks_of(seq_of(p, b));
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
-    total *= R;
+    int n = chunks_of(seqs), total = n, longest = n;
+    for (int b = 32 + lane; b < p.c.rows; b += 32) {
+      const int more = chunks_of(seq_of(p, b));
+      total += more;
+      longest = max(longest, more);
+    }
+    total = __reduce_add_sync(0xffffffffu, total) * R;
+    longest = __reduce_max_sync(0xffffffffu, longest);
     for (int b = blockIdx.x; b < p.c.rows; b += p.ctas)  // sequences of no tokens belong to no range
       if (seq_of(p, b) == 0)
         for (int h = 0; h < p.num_q_heads; h += kQ4Heads)
           for (int k = threadIdx.x; k < kQ4Frags; k += kQ4Threads)
             store_frag<T, NG>(p, b, h, p.num_q_heads - h, k, nothing, 0.f, 0.f);
-    per = range_of(p, total);
+    per = range_of(p, total, longest);
     if ((long long)blockIdx.x * per >= total) return;
     lo = blockIdx.x * per;
     hi = min(total, lo + per);
@@ -362,17 +352,21 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
   };
   auto issue = [&]() {
     const int s = issued % kQ4Stages;
-    if (lane == 0) mbar_arrive_expect_tx(bar0 + 8 * s, pages * slab);
+    uint8_t *to = smem + (warp * kQ4Stages + s) * S::stage;
+    const int tier = entry < 0 ? 1 : 0;
+    const long long page = entry < 0 ? -1ll - entry : entry;
+    const uint32_t good = __ballot_sync(0xffffffffu, lane < pages && page < p.c.pages[tier]);
+    if (lane == 0) mbar_arrive_expect_tx(bar0 + 8 * s, __popc(good) * slab);
     __syncwarp();
-    if (lane < pages) {
-      const int tier = entry < 0 ? 1 : 0;
-      long long page = entry < 0 ? -1ll - entry : entry;
-      if (page >= p.c.pages[tier]) {  // the copy starts past the map's end and reads zeros
-        atomicCAS(p.c.status, 0, DAK_ERR_INVALID_ARG);
-        page = max(1ll, p.c.pages[tier]);
-      }
-      tma_load_slab(sbase + (warp * kQ4Stages + s) * S::stage + lane * slab, &p.map[tier],
-                    (int)(page * p.c.kv_heads + at_r / p.head_blocks), bar0 + 8 * s, pol);
+    if (good >> lane & 1u)
+      bulk_load(smem_u32(to) + lane * slab,
+                p.c.pool[tier] + page * p.c.page_bytes + (long long)(at_r / p.head_blocks) * slab, slab, bar0 + 8 * s, pol);
+    if (__popc(good) < pages) {  // an entry outside its pool: zeros
+      if (lane == 0) atomicCAS(p.c.status, 0, DAK_ERR_INVALID_ARG);
+      for (int i = 0; i < pages; ++i)
+        if (!(good >> i & 1u))
+          for (int v = lane; v < slab / 16; v += 32) reinterpret_cast<uint4 *>(to + i * slab)[v] = make_uint4(0u, 0u, 0u, 0u);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the stage's next fill is a copy
     }
     __syncwarp();
     ++issued;
@@ -471,8 +465,8 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
   };
 
   // V: this lane takes 4 dims at a time (piece x) of tokens 2 cq, 2 cq + 1 (and 8
-  // on).  Odd columns read the second token first, which spreads a warp's reads
-  // over all banks; the byte selectors put the pair back in order.
+  // on).  Odd columns read the second token first, so that a warp's rows are even
+  // and odd ones and use all banks; the byte selectors put the pair back in order.
   const uint32_t flip = cq & 1;
   const uint32_t sel_lo = flip ? 0x1054u : 0x5410u, sel_hi = flip ? 0x3276u : 0x7632u;
   const uint32_t sel_g = (g & 1) ? sel_hi : sel_lo;
@@ -486,15 +480,10 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
   // One chunk of `valid` tokens in the stage at `st`.
   auto chunk = [&](const uint8_t *st, int valid, auto full_c) {
     constexpr bool kFull = decltype(full_c)::value;
-    // Offset of tile t's first code row (V: + half) and of its pairs of token g + 8r.
+    // Where tile t's code rows begin (V: + half), and the pairs of token g + 8r.
     auto rows_at = [](int t) { return (uint32_t)((16 * t) / P * slab + (16 * t) % P * 64); };
     auto pairs_at = [&](int t, int r) {
-      const uint32_t c = (16 * t) / P * slab + P * 64 + (16 * t) % P * (4 * NG);
-      return NG == 4 ? swz(c + 128 * r, g >> 2, 16 * (g & 3)) : NG == 2 ? swz(c + 64 * r, 0, 8 * g) : swz(c, 0, 4 * g + 32 * r);
-    };
-    auto vpairs_at = [&](int t, int r) {
-      const uint32_t c = (16 * t) / P * slab + half + P * 64 + (16 * t) % P * (4 * NG);
-      return NG == 4 ? swz(c + 128 * r, g >> 2, 16 * (g & 3)) : NG == 2 ? swz(c + 64 * r, 0, 8 * g) : swz(c, 0, 4 * g + 32 * r);
+      return (uint32_t)((16 * t) / P * slab + P * 64 + ((16 * t) % P + g + 8 * r) * (4 * NG));
     };
     float y[4][4];  // raw scores: tile, {token g, g + 8} x {head 2 cq, 2 cq + 1}
     float mx[2] = {-INFINITY, -INFINITY};
@@ -504,7 +493,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
     uint32_t vp[4][2][NG];
     auto load_vp = [&](int t, int r, bool again) {
       if (again && NG == 1) return;
-      load_pairs<NG>(st + vpairs_at(t, r), vp[t][r]);
+      load_pairs<NG>(st + half + pairs_at(t, r), vp[t][r]);
 #pragma unroll
       for (int n = 0; n < NG; ++n)
         if (!kFull && t * 16 + 8 * r + g >= valid) vp[t][r][n] = 0u;  // anything may lie behind the last token
@@ -519,14 +508,14 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       // S^T = K Q^T
       uint32_t w0[4], w1[4];  // tokens g and g + 8
       if constexpr (NG == 1) {
-        const uint8_t *a = st + swz(rows_at(t), g, 16 * cq);
+        const uint8_t *a = st + rows_at(t) + g * 64 + 16 * cq;
         const uint4 u = *reinterpret_cast<const uint4 *>(a), v = *reinterpret_cast<const uint4 *>(a + 512);
         w0[0] = u.x, w0[1] = u.y, w0[2] = u.z, w0[3] = u.w;
         w1[0] = v.x, w1[1] = v.y, w1[2] = v.z, w1[3] = v.w;
       } else if constexpr (NG == 2) {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          const uint8_t *a = st + swz(rows_at(t), g, 32 * n + 8 * cq);
+          const uint8_t *a = st + rows_at(t) + g * 64 + 32 * n + 8 * cq;
           const uint2 u = *reinterpret_cast<const uint2 *>(a), v = *reinterpret_cast<const uint2 *>(a + 512);
           w0[2 * n] = u.x, w0[2 * n + 1] = u.y;
           w1[2 * n] = v.x, w1[2 * n + 1] = v.y;
@@ -534,7 +523,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       } else {
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-          const uint8_t *a = st + swz(rows_at(t), g, 16 * n + 4 * cq);
+          const uint8_t *a = st + rows_at(t) + g * 64 + 16 * n + 4 * cq;
           w0[n] = *reinterpret_cast<const uint32_t *>(a);
           w1[n] = *reinterpret_cast<const uint32_t *>(a + 512);
         }
@@ -679,39 +668,31 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
           }
         }
       }
-      uint32_t x[2][4];  // token pairs (2 cq, +1) and (2 cq + 8, +9): 4 pieces of 4 dims
-      const uint32_t row0 = 2 * cq + flip, row1 = 2 * cq + 1 - flip;
-      const uint32_t vc = rows_at(t) + half;
-      if constexpr (NG == 1) {
-        const uint8_t *a = st + swz(vc, row0, 8 * g), *c = st + swz(vc, row1, 8 * g);
+      // Token pairs (2 cq, + 1) and (2 cq + 8, + 9): 4 pieces of 4 dims of each.
+      uint32_t x[2][4];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const uint2 u = *reinterpret_cast<const uint2 *>(a + 512 * r), v = *reinterpret_cast<const uint2 *>(c + 512 * r);
+      for (int r = 0; r < 2; ++r) {
+        const uint8_t *a = st + half + rows_at(t) + (2 * cq + flip + 8 * r) * 64;
+        const uint8_t *c = st + half + rows_at(t) + (2 * cq + 1 - flip + 8 * r) * 64;
+        if constexpr (NG == 1) {
+          const uint2 u = *reinterpret_cast<const uint2 *>(a + 8 * g), v = *reinterpret_cast<const uint2 *>(c + 8 * g);
           x[r][0] = __byte_perm(u.x, v.x, sel_lo);
           x[r][1] = __byte_perm(u.x, v.x, sel_hi);
           x[r][2] = __byte_perm(u.y, v.y, sel_lo);
           x[r][3] = __byte_perm(u.y, v.y, sel_hi);
-        }
-      } else if constexpr (NG == 2) {
+        } else if constexpr (NG == 2) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const uint8_t *a = st + swz(vc, row0, 32 * n + 4 * g), *c = st + swz(vc, row1, 32 * n + 4 * g);
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const uint32_t u = *reinterpret_cast<const uint32_t *>(a + 512 * r);
-            const uint32_t v = *reinterpret_cast<const uint32_t *>(c + 512 * r);
+          for (int n = 0; n < 2; ++n) {
+            const uint32_t u = *reinterpret_cast<const uint32_t *>(a + 32 * n + 4 * g);
+            const uint32_t v = *reinterpret_cast<const uint32_t *>(c + 32 * n + 4 * g);
             x[r][2 * n] = __byte_perm(u, v, sel_lo);
             x[r][2 * n + 1] = __byte_perm(u, v, sel_hi);
           }
-        }
-      } else {
+        } else {
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const uint8_t *a = st + swz(vc, row0, 16 * n + 4 * (g >> 1)), *c = st + swz(vc, row1, 16 * n + 4 * (g >> 1));
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-            x[r][n] = __byte_perm(*reinterpret_cast<const uint32_t *>(a + 512 * r),
-                                  *reinterpret_cast<const uint32_t *>(c + 512 * r), sel_g);
+          for (int n = 0; n < 4; ++n)
+            x[r][n] = __byte_perm(*reinterpret_cast<const uint32_t *>(a + 16 * n + 4 * (g >> 1)),
+                                  *reinterpret_cast<const uint32_t *>(c + 16 * n + 4 * (g >> 1)), sel_g);
         }
       }
 #pragma unroll
@@ -847,7 +828,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       __syncthreads();
       if (*last) {
         __threadfence();
-        merge_row<T, NG>(p, row_b, h0, nh, row_begin, row_end, per, kQ4Threads);
+        merge_row<T, NG>(p, row_b, h0, nh, row_begin, row_end, per);
       }
     }
     __syncthreads();  // statistics and outputs are free again
@@ -862,27 +843,26 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
 
 // The merge as a launch of its own, one CTA per row.
 template <typename T, int NG>
-__global__ void __launch_bounds__(kQ4Frags) attn_q4_merge_kernel(const __grid_constant__ AttnQ4Params p) {
+__global__ void __launch_bounds__(kQ4Threads) attn_q4_merge_kernel(const __grid_constant__ AttnQ4Params p) {
   pdl_enter(p.pdl);
   const int R = p.c.kv_heads * p.head_blocks;
   const int b = blockIdx.x / R, r = blockIdx.x - b * R;
   const int n = chunks_of(seq_of(p, b));
-  int before = 0, total = 0;
+  int before = 0, total = 0, longest = 0;
   for (int i = lane_id(); i < p.c.rows; i += 32) {
     const int v = chunks_of(seq_of(p, i));
     total += v;
     before += i < b ? v : 0;
+    longest = max(longest, v);
   }
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, x);
-    before += __shfl_xor_sync(0xffffffffu, before, x);
-  }
-  const int per = range_of(p, total * R), begin = before * R + r * n;
+  total = __reduce_add_sync(0xffffffffu, total);
+  before = __reduce_add_sync(0xffffffffu, before);
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  const int per = range_of(p, total * R, longest), begin = before * R + r * n;
   if (n == 0 || begin / per == (begin + n - 1) / per) return;  // written already
   const int hb = r % p.head_blocks;
   merge_row<T, NG>(p, b, r / p.head_blocks * p.group + hb * p.block_heads, min(p.block_heads, p.group - hb * p.block_heads),
-                   begin, begin + n, per, kQ4Frags);
+                   begin, begin + n, per);
 }
 
 template <typename T, int NG, int P>
@@ -892,7 +872,7 @@ cudaError_t launch_attn(const AttnQ4Params &p, int rows, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   e = launch_ex(kern, dim3(p.ctas), dim3(kQ4Threads), Q4Smem<NG>::bytes, s, 1, p.pdl != 0, p);
   if (e != cudaSuccess || p.by_row || p.counters) return e;
-  return launch_ex(attn_q4_merge_kernel<T, NG>, dim3(rows), dim3(kQ4Frags), 0, s, 1, p.pdl != 0, p);
+  return launch_ex(attn_q4_merge_kernel<T, NG>, dim3(rows), dim3(kQ4Threads), 0, s, 1, p.pdl != 0, p);
 }
 
 template <typename T, int NG>
@@ -935,38 +915,6 @@ Q4Plan q4_plan(const dak_kv4_cache *c, int num_q_heads, int max_seq_len) {
   return plan;
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-    void *ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    const bool ok = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault, &q) ==
-                        cudaSuccess &&
-                    q == cudaDriverEntryPointSuccess;
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ok ? ptr : nullptr);
-  }();
-  return fn;
-}
-
-// Map of a pool as slabs of 64-byte rows, one box per slab, stored with the
-// 64-byte swizzle.
-int slab_map(CUtensorMap *out, const Kv4Cache &c, int tier) {
-  const int from = c.pool[tier] ? tier : 1 - tier;  // an absent tier: one page that no entry reaches
-  const long long pages = c.pool[tier] ? c.pages[tier] : 1;
-  const long long slabs = pages * c.kv_heads;
-  if (slabs + c.kv_heads > 0x7fffffffll) return fail(DAK_ERR_UNSUPPORTED, "pages x kv_heads of a pool must stay below 2^31");
-  auto fn = tensor_map_encoder();
-  if (!fn) return fail(DAK_ERR_DRIVER, "cuTensorMapEncodeTiled entry point unavailable");
-  const cuuint64_t dims[3] = {64, (cuuint64_t)c.slab_bytes / 64, (cuuint64_t)slabs};
-  const cuuint64_t strides[2] = {64, (cuuint64_t)c.slab_bytes};
-  const cuuint32_t box[3] = {64, (cuuint32_t)c.slab_bytes / 64, 1};
-  const cuuint32_t es[3] = {1, 1, 1};
-  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, c.pool[from], dims, strides, box, es,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(DAK_ERR_DRIVER, "cuTensorMapEncodeTiled (4-bit KV) failed with %d", (int)r);
-  return DAK_OK;
-}
-
 }  // namespace
 }  // namespace dak
 
@@ -998,8 +946,6 @@ extern "C" int dak_attn_decode_paged_q4(const dak_kv4_cache *cache, const dak_at
   AttnQ4Params p;
   std::memset(&p, 0, sizeof(p));
   if ((st = kv4_view(cache, &p.c))) return st;
-  for (int tier = 0; tier < 2; ++tier)
-    if ((st = slab_map(&p.map[tier], p.c, tier))) return st;
   p.query = static_cast<const uint16_t *>(a->query);
   p.q_stride_b = a->q_stride_b;
   p.q_stride_h = a->q_stride_h;
