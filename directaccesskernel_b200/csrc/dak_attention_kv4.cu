@@ -10,6 +10,27 @@
 // fourth chunk, with copies running ahead across rows.  A row that spans CTAs is
 // merged by log-sum-exp.  Scores are kept in base 2; a sequence of no tokens
 // gives zeros.
+//
+// A warp has two chunks in flight, each a bulk copy per page (one contiguous slab
+// with K and V of a head).  For 16 tokens and up to 8 heads:
+//   S^T [16 tokens x 8 heads] = K Q^T, scale and zero of the token applied to the
+//     FP32 scores;
+//   O^T [128 dims x 8 heads] += V^T P^T, with the token's scale multiplied into P
+//     and its zero added to O as sum_t p_t zero_t per chunk.
+// Codes never become floating-point values of their own: K's bytes enter integer
+// MMAs as they are (see "Scores" below), V's nibbles enter as float16 subnormals
+// (bits 0-3 of a half word are code * 2^-24, bits 4-7 code * 2^-20), so that two
+// masks and a byte permutation are all that they take.  P is float16: for bfloat16
+// outputs in one term (2^-11 relative, an eighth of the output's own rounding),
+// for float16 outputs in two, because one made the output up to 1.9 times less
+// exact than its rounding and two do not show.
+//
+// Bound, at 32 x 16384 tokens of 8 KV heads (570 MB, 89 us at the measured copy
+// rate): 114 us in bfloat16, 126 us in float16.  The copies alone take 91 us; the
+// rest is arithmetic that two warps per scheduler do not quite hide (4.3 cycles
+// per instruction and warp, a good 800 instructions per chunk).  Plain bulk
+// copies replaced tensor copies with a 64-byte swizzle: bank conflicts cost less
+// than the 64-byte rows did, and host pages come 15% faster (46 GB/s).
 #include <cfloat>
 #include <cstring>
 #include <type_traits>
@@ -31,7 +52,7 @@ constexpr int kQ4PerSm = 2;
 constexpr int kQ4Heads = 8;    // query heads per CTA: the MMA's N
 constexpr int kQ4Chunk = 64;   // tokens a warp takes at a time
 constexpr int kQ4Stages = 2;   // chunks in flight per warp
-constexpr int kQ4MergeBatch = 8;  // pieces of a row read at once
+constexpr int kQ4MergeBatch = 6;  // pieces of a row read at once
 constexpr int kQ4RowChunks = 8;  // rows up to this long are not split while the GPU holds them all
 
 struct AttnQ4Params {
@@ -162,11 +183,11 @@ __device__ __forceinline__ int chunks_of(int seq) { return (seq + kQ4Chunk - 1) 
 
 // Chunks of a CTA's range, given those of all rows and of the longest: every CTA
 // the same, at least one for each warp.  Merging a row costs the CTA that does it
-// about 0.1 us per piece, against 1.3 us for four chunks, one per warp: a row of n
-// chunks is best cut into about sqrt(9 n) pieces, which matters where one or two
-// rows are all there is.
+// about 0.1 us per piece, and four chunks, one per warp, take 1.3 us: a row of n
+// chunks is best cut into about sqrt(3 n) pieces, which matters where one or two
+// rows are all there is (one row of 131072 tokens: 57 us in 293 pieces, 27 in 79).
 __device__ __forceinline__ int range_of(const AttnQ4Params &p, int total, int longest) {
-  return max(max((total + p.ctas - 1) / p.ctas, kQ4Warps), (int)sqrtf(longest * (1.f / 9.f)));
+  return max(max((total + p.ctas - 1) / p.ctas, kQ4Warps), (int)sqrtf(longest * (1.f / 3.f)));
 }
 
 // Merges row (b, r), whose chunks are [begin, end) of all in ranges of `per`, from

@@ -137,7 +137,7 @@ struct AppendSmem {
 // A head of the four tokens at a time per warp: q heads are rotated, k heads
 // rotated and packed, v heads packed.
 template <typename T, int NG>
-__global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(kKv4Threads, 4) kv4_append_kernel(const __grid_constant__ AppendParams p) {
   extern __shared__ __align__(128) uint8_t rows_s[];  // [tokens][slice][128] 16-bit, then the rest
   AppendSmem &sm = *reinterpret_cast<AppendSmem *>(rows_s + 4 * p.slice * kKv4Dim * 2);
   pdl_enter(p.pdl);

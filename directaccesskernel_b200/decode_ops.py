@@ -181,10 +181,14 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
     return out
 
 
-def _check_rope(positions: torch.Tensor, inv_freq: torch.Tensor | None, tokens: int, head_dim: int, device: int) -> None:
+def _check_rope(positions: torch.Tensor, inv_freq: torch.Tensor, tokens: int, head_dim: int, device: int) -> None:
     if positions.dtype != torch.int32 or positions.get_device() != device or positions.numel() != tokens \
             or not positions.is_contiguous():
         raise RuntimeError("positions must be a contiguous int32 CUDA tensor with one entry per token")
-    if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.get_device() != device
-                                 or not inv_freq.is_contiguous() or 2 * inv_freq.numel() > head_dim):
+    check_inv_freq(inv_freq, head_dim, device)
+
+
+def check_inv_freq(inv_freq: torch.Tensor, head_dim: int, device: int) -> None:
+    if inv_freq.dtype != torch.float32 or inv_freq.get_device() != device or not inv_freq.is_contiguous() \
+            or 2 * inv_freq.numel() > head_dim:
         raise RuntimeError("inv_freq must be a contiguous float32 CUDA tensor of at most head_dim / 2 entries")

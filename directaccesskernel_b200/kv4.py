@@ -28,7 +28,7 @@ import torch
 from . import _lib
 from ._lib import LIB, check
 from .attention import HEAD_DIM
-from .decode_ops import _check_rope, current_device_of, stream_of
+from .decode_ops import check_inv_freq, current_device_of, stream_of
 from .runtime import NUM_SMS, dak_dtype
 from .trace import traced
 
@@ -131,7 +131,8 @@ def rope_kv_append_q4(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torc
         raise RuntimeError("qkv must be a 16-bit [tokens, (q_heads + 2 kv_heads) * 128] tensor, last dim contiguous")
     c = _cache(device, pool_dev, pool_host, block_table)
     T = _check_tokens(positions, seq_index, device, c.batch)
-    _check_rope(positions, inv_freq, T, HEAD_DIM, device)
+    if inv_freq is not None:
+        check_inv_freq(inv_freq, HEAD_DIM, device)
     if qkv.shape[0] != T or qkv.shape[1] != (q_heads + 2 * c.kv_heads) * HEAD_DIM:
         raise RuntimeError(f"qkv must be [{T}, {(q_heads + 2 * c.kv_heads) * HEAD_DIM}]")
     if q_heads and (q_out is None or not q_out.is_contiguous() or q_out.dtype != qkv.dtype or q_out.get_device() != device

@@ -469,3 +469,82 @@ def test_pack_of_the_tests_is_the_formats():
     kv4.rope_kv_append_q4(qkv, torch.arange(32, dtype=torch.int32, device="cuda").repeat(3), None, 0, None, pool, None,
                           _i32([[0], [1], [2]]), seq_index=torch.arange(3, dtype=torch.int32, device="cuda").repeat_interleave(32))
     assert torch.equal(pool.cpu(), want)
+
+
+def test_pools_beyond_32_bit_offsets():
+    """Pages whose bytes lie past 4 GiB: append, read, attend and copy."""
+    from directaccesskernel_b200.kv_pages import copy_pages
+
+    kv4 = _kv4()
+    n = 2**32 // kv4.page_bytes(64, 128) + 40
+    pool = torch.empty(n, 1, kv4.page_bytes(64, 128), dtype=torch.uint8, device="cuda")
+    small = random_pool(3, 1, 64, 128, 50)
+    pool[n - 3:] = small.cuda()
+    table, lens = _i32([[n - 1, n - 3, n - 2]]), _i32([150])
+    q = torch.randn(1, 8, D, generator=torch.Generator().manual_seed(5)).half().cuda()
+    got = kv4.decode_paged_q4(q, pool, None, table, lens, 0.1)
+    assert torch.equal(got, kv4.decode_paged_q4(q, small.cuda(), None, _i32([[2, 0, 1]]), lens, 0.1))
+    x = torch.randn(1, 2 * D, generator=torch.Generator().manual_seed(6)).half().cuda()
+    kv4.rope_kv_append_q4(x, _i32([149]), None, 0, None, pool, None, table)
+    k, v = kv4.kv_read_q4(pool, None, table, _i32([149]))
+    codes, pairs = quantise32(x.cpu().view(2, D), 128)
+    want = values(codes, pairs).half()
+    assert torch.equal(k.cpu()[0, 0], want[0]) and torch.equal(v.cpu()[0, 0], want[1])
+    copy_pages(pool, None, [n - 2], [n - 9])
+    assert torch.equal(pool[n - 9], pool[n - 2])
+
+
+def test_entry_points_refuse_another_device_or_the_cpu():
+    kv4 = _kv4()
+    pool = random_pool(2, 1, 16, 32, 51)
+    q = torch.zeros(1, 1, D, dtype=torch.float16, device="cuda")
+    one, table = _i32([3]), _i32([[0, 1]])
+    for call in (lambda: kv4.decode_paged_q4(q, pool, None, table, one, 1.0),
+                 lambda: kv4.kv_read_q4(pool, None, table, one),
+                 lambda: kv4.kv_read_q4(pool.cuda(), None, table, one.cpu()),
+                 lambda: kv4.rope_kv_append_q4(torch.zeros(1, 2 * D, dtype=torch.float16, device="cuda"), one, None, 0, None,
+                                               pool, None, table)):
+        with pytest.raises(RuntimeError, match="device|CUDA"):
+            call()
+
+
+def test_two_streams_with_their_own_scratch():
+    """The same batch on two streams at once, each with scratch and counters of its own."""
+    kv4 = _kv4()
+    pool = random_pool(60, 2, 32, 64, 52).cuda()
+    q = torch.randn(3, 10, D, generator=torch.Generator().manual_seed(7)).to(torch.bfloat16).cuda()
+    table = torch.randint(0, 60, (3, 100), generator=torch.Generator().manual_seed(8)).int().cuda()
+    lens = _i32([3200, 1700, 900])
+    want = kv4.decode_paged_q4(q, pool, None, table, lens, 0.09)
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for s in streams:
+        with torch.cuda.stream(s):
+            cnt = torch.zeros(kv4.merge_counter_count(3, 10, 2), dtype=torch.int32, device="cuda")
+            outs.append([kv4.decode_paged_q4(q, pool, None, table, lens, 0.09, merge_counters=cnt) for _ in range(10)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for out in outs for o in out)
+
+
+def test_steps_whose_lengths_change_under_one_graph():
+    """A graph captured with a long max_seq_len replayed for lengths from none to the limit."""
+    kv4 = _kv4()
+    page, group, width = 16, 32, 130
+    pool = random_pool(200, 1, page, group, 53)
+    table = torch.randint(0, 200, (2, width), generator=torch.Generator().manual_seed(9))
+    q = torch.randn(2, 4, D, generator=torch.Generator().manual_seed(10)).half()
+    dev, tab, qd, lens = pool.cuda(), table.int().cuda(), q.cuda(), _i32([5, 9])
+    cnt = torch.zeros(kv4.merge_counter_count(2, 4, 1), dtype=torch.int32, device="cuda")
+    out = torch.empty_like(qd)
+    kv4.decode_paged_q4(qd, dev, None, tab, lens, 0.1, out=out, merge_counters=cnt)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kv4.decode_paged_q4(qd, dev, None, tab, lens, 0.1, out=out, merge_counters=cnt)
+    v_range = 15 * parts(pool, page, group)[3][..., 0].double().amax()
+    k_abs = values(*parts(pool, page, group)[:2]).abs().amax()
+    for pair in ([0, 0], [1, 2080], [2080, 0], [64, 65], [700, 1300]):
+        lens.copy_(torch.tensor(pair, dtype=torch.int32))
+        graph.replay()
+        ref = attend64(q, (pool, None), page, group, table, pair, 0.1)
+        assert ((out.cpu().double() - ref).abs() <= _bound(ref, q, k_abs, v_range, 0.1, torch.float16)).all()
+        assert not cnt.any()
