@@ -121,18 +121,20 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// D += A (16x32 unsigned bytes, row) * B (32x8 bytes, col; signed or not), int32.
-template <bool kSigned>
+// D = A (16x32 unsigned bytes, row) * B (32x8 bytes, col; signed or not) + D, or
+// without the sum, int32.
+template <bool kSigned, bool kSum>
 __device__ __forceinline__ void mma_u8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
+  const int c0 = kSum ? d[0] : 0, c1 = kSum ? d[1] : 0, c2 = kSum ? d[2] : 0, c3 = kSum ? d[3] : 0;
   if constexpr (kSigned)
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
   else
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -355,37 +357,46 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
   // The position (row, table entries) of the copy after next is worked out while
   // the chunks in flight are multiplied.
   const uint64_t pol = l2_policy_evict_first();
-  int at = lo + warp, at_b = b0, at_r = r0, at_begin = begin, at_seq = seq0, at_n = chunks_of(at_seq);
+  int at = lo + warp, at_b = b0, at_r = r0, at_begin = begin, at_pages = (seq0 + P - 1) / P;
+  int at_end = begin + chunks_of(seq0);
+  const int32_t *at_row = p.c.table + b0 * p.c.table_stride + lane;
+  uint32_t head_off = (uint32_t)(r0 / p.head_blocks) * slab;
   int entry = 0, pages = 0, issued = 0;
   auto locate = [&]() {
     if (at >= hi) return;
-    while (at >= at_begin + at_n) {
-      at_begin += at_n;
-      if (at_n == 0 || ++at_r == R) {
+    while (at >= at_end) {
+      at_begin = at_end;
+      if (++at_r == R) {
         at_r = 0;
-        at_seq = seq_of(p, ++at_b);
-        at_n = chunks_of(at_seq);
+        int seq;
+        do {
+          seq = seq_of(p, ++at_b);
+        } while (seq == 0);  // there is one: the range goes on
+        at_pages = (seq + P - 1) / P;
+        at_row = p.c.table + at_b * p.c.table_stride + lane;
       }
+      at_end = at_begin + (at_pages + ppc - 1) / ppc;
+      head_off = (uint32_t)(at_r / p.head_blocks) * slab;
     }
     const int first = (at - at_begin) * ppc;
-    pages = min(ppc, (at_seq + P - 1) / P - first);
-    entry = lane < pages ? p.c.table[at_b * p.c.table_stride + first + lane] : 0;
+    pages = min(ppc, at_pages - first);
+    entry = lane < pages ? at_row[first] : 0;
   };
   auto issue = [&]() {
     const int s = issued % kQ4Stages;
     uint8_t *to = smem + (warp * kQ4Stages + s) * S::stage;
     const int tier = entry < 0 ? 1 : 0;
-    const long long page = entry < 0 ? -1ll - entry : entry;
-    const uint32_t good = __ballot_sync(0xffffffffu, lane < pages && page < p.c.pages[tier]);
-    if (lane == 0) mbar_arrive_expect_tx(bar0 + 8 * s, __popc(good) * slab);
+    const uint32_t page = entry < 0 ? ~entry : entry;  // -1 - v is ~v
+    const bool good = lane < pages && page < p.c.pages[tier];
+    const uint32_t which = __ballot_sync(0xffffffffu, good);
+    if (lane == 0) mbar_arrive_expect_tx(bar0 + 8 * s, __popc(which) * slab);
     __syncwarp();
-    if (good >> lane & 1u)
-      bulk_load(smem_u32(to) + lane * slab,
-                p.c.pool[tier] + page * p.c.page_bytes + (long long)(at_r / p.head_blocks) * slab, slab, bar0 + 8 * s, pol);
-    if (__popc(good) < pages) {  // an entry outside its pool: zeros
+    if (good)
+      bulk_load(smem_u32(to) + lane * slab, p.c.pool[tier] + page * p.c.page_bytes + head_off, slab, bar0 + 8 * s, pol);
+    if (__popc(which) < pages) {  // an entry outside its pool: zeros
       if (lane == 0) atomicCAS(p.c.status, 0, DAK_ERR_INVALID_ARG);
       for (int i = 0; i < pages; ++i)
-        if (!(good >> i & 1u))
+        if (!(which >> i & 1u))
           for (int v = lane; v < slab / 16; v += 32) reinterpret_cast<uint4 *>(to + i * slab)[v] = make_uint4(0u, 0u, 0u, 0u);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the stage's next fill is a copy
     }
@@ -561,17 +572,19 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       for (int n = 0; n < NG; ++n) {
         float acc[4];
         if constexpr (kIntegers) {
-          int c[3][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};  // by digit
-#pragma unroll
-          for (int v = n * 2 / NG; v < (n + 1) * 2 / NG; ++v) {
+          int c[3][4];  // by digit
+          auto words = [&](int v, auto sum_c) {
+            constexpr bool kSum = decltype(sum_c)::value;
             const uint32_t a0 = w0[2 * v], a1 = w1[2 * v], a2 = w0[2 * v + 1], a3 = w1[2 * v + 1];
             const uint32_t l0 = a0 & 0x0F0F0F0Fu, l1 = a1 & 0x0F0F0F0Fu, l2 = a2 & 0x0F0F0F0Fu, l3 = a3 & 0x0F0F0F0Fu;
-            mma_u8<false>(c[0], a0, a1, a2, a3, qa[0][v][0], qa[0][v][1]);
-            mma_u8<true>(c[1], a0, a1, a2, a3, qa[1][v][0], qa[1][v][1]);
-            mma_u8<false>(c[0], l0, l1, l2, l3, qb[0][v][0], qb[0][v][1]);
-            mma_u8<false>(c[1], l0, l1, l2, l3, qb[1][v][0], qb[1][v][1]);
-            mma_u8<true>(c[2], l0, l1, l2, l3, qb[2][v][0], qb[2][v][1]);
-          }
+            mma_u8<false, kSum>(c[0], a0, a1, a2, a3, qa[0][v][0], qa[0][v][1]);
+            mma_u8<true, kSum>(c[1], a0, a1, a2, a3, qa[1][v][0], qa[1][v][1]);
+            mma_u8<true, kSum>(c[2], l0, l1, l2, l3, qb[2][v][0], qb[2][v][1]);
+            mma_u8<false, true>(c[0], l0, l1, l2, l3, qb[0][v][0], qb[0][v][1]);
+            mma_u8<false, true>(c[1], l0, l1, l2, l3, qb[1][v][0], qb[1][v][1]);
+          };
+          words(n * 2 / NG, std::false_type{});
+          if constexpr (NG == 1) words(1, std::true_type{});
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[e] = (float)(c[2][e] * 65536 + c[1][e] * 256 + c[0][e]);
         } else {

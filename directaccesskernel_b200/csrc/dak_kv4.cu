@@ -16,6 +16,12 @@
 // four tokens and up to 48 heads of each: four bulk copies bring them into shared
 // memory, all in flight at once, while the threads work out the tokens' angles,
 // one each, and look up their pages.
+//
+// Append of 16384 tokens, 32 + 16 heads in bfloat16, groups of 32 (358 MB): 71 us,
+// 5.0 TB/s, 0.79 of the measured copy rate; of 4099 tokens 24 us (38 us when each
+// thread fetched its heads itself and worked out their angles); of 32 tokens
+// 3.1 us.  Read-back of 65536 tokens x 8 heads, groups of 128 (340 MB): 62 us,
+// 5.5 TB/s, 0.85 (75 us with one row in flight per thread).
 #include <cstring>
 
 #include "dak_host.h"

