@@ -26,9 +26,9 @@
 // exact than its rounding and two do not show.
 //
 // Bound, at 32 x 16384 tokens of 8 KV heads (570 MB, 89 us at the measured copy
-// rate): 114 us in bfloat16, 126 us in float16.  The copies alone take 91 us; the
+// rate): 108 us in bfloat16, 119 us in float16.  The copies alone take 91 us; the
 // rest is arithmetic that two warps per scheduler do not quite hide (4.3 cycles
-// per instruction and warp, a good 800 instructions per chunk).  Plain bulk
+// per instruction and warp, 825 instructions per chunk).  Plain bulk
 // copies replaced tensor copies with a 64-byte swizzle: bank conflicts cost less
 // than the 64-byte rows did, and host pages come 15% faster (46 GB/s).
 #include <cfloat>
@@ -53,6 +53,7 @@ constexpr int kQ4Heads = 8;    // query heads per CTA: the MMA's N
 constexpr int kQ4Chunk = 64;   // tokens a warp takes at a time
 constexpr int kQ4Stages = 2;   // chunks in flight per warp
 constexpr int kQ4MergeBatch = 6;  // pieces of a row read at once
+constexpr int kQ4RowSlack = 11;   // see Q4Deal
 constexpr int kQ4RowChunks = 8;  // rows up to this long are not split while the GPU holds them all
 
 struct AttnQ4Params {
@@ -66,7 +67,7 @@ struct AttnQ4Params {
   int32_t *counters;  // [rows]: the CTA that finishes a split row last merges it (nullptr: merge kernel)
   int num_q_heads, group, block_heads, head_blocks;  // group: query heads per KV head
   int max_seq_len;
-  int ctas, by_row;  // by_row: CTA i takes row i, and no row is split
+  int ctas, by_row;  // by_row: CTA i takes row i whatever the lengths; there is no scratch
   float scale_log2;                                  // scaling * log2(e)
   int pdl;
 };
@@ -183,14 +184,23 @@ __device__ __forceinline__ int seq_of(const AttnQ4Params &p, int b) {
 }
 __device__ __forceinline__ int chunks_of(int seq) { return (seq + kQ4Chunk - 1) / kQ4Chunk; }
 
-// Chunks of a CTA's range, given those of all rows and of the longest: every CTA
-// the same, at least one for each warp.  Merging a row costs the CTA that does it
-// about 0.1 us per piece, and four chunks, one per warp, take 1.3 us: a row of n
-// chunks is best cut into about sqrt(3 n) pieces, which matters where one or two
-// rows are all there is (one row of 131072 tokens: 57 us in 293 pieces, 27 in 79).
-__device__ __forceinline__ int range_of(const AttnQ4Params &p, int total, int longest) {
-  return max(max((total + p.ctas - 1) / p.ctas, kQ4Warps), (int)sqrtf(longest * (1.f / 3.f)));
-}
+// How the chunks are dealt out, given the sum over all rows and the longest row:
+// equal ranges of `size` chunks, at least one for each warp, or a row for each CTA.
+//
+// Merging a row costs the CTA that does it about 0.1 us per piece, and four chunks,
+// one per warp, take 1.3 us: a row of n chunks is best cut into about sqrt(3 n)
+// pieces, which matters where one or two rows are all there is (one row of 131072
+// tokens: 57 us in 293 pieces, 27 in 79).  Where there is a CTA for every row, whole
+// rows save the merge and the second row of a range, together about 4 us, or 11
+// chunks: they are dealt if the longest is no further than that from the equal share.
+struct Q4Deal {
+  int size;  // 0: CTA i takes row i
+  __device__ __forceinline__ Q4Deal(const AttnQ4Params &p, int total, int longest) {
+    const int share = (total + p.ctas - 1) / p.ctas;
+    size = max(max(share, kQ4Warps), (int)sqrtf(longest * (1.f / 3.f)));
+    if (p.by_row || (p.c.rows * p.c.kv_heads * p.head_blocks <= p.ctas && longest <= share + kQ4RowSlack)) size = 0;
+  }
+};
 
 // Merges row (b, r), whose chunks are [begin, end) of all in ranges of `per`, from
 // its pieces in the scratch, in order.  Piece i is CTA i's first segment (slot
@@ -272,8 +282,23 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
   const int R = p.c.kv_heads * p.head_blocks;
   int lo, hi, begin, b0, r0, seq0, per = 0;
   const float4 nothing = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (p.by_row) {
+  // Lengths of the first 32 sequences, one per lane; most batches need no more.
+  int seqs = 0, n32 = 0, total = 0;
+  if (!p.by_row) {
+    seqs = lane < p.c.rows ? seq_of(p, lane) : 0;
+    n32 = total = chunks_of(seqs);
+    int longest = total;
+    for (int b = 32 + lane; b < p.c.rows; b += 32) {
+      const int more = chunks_of(seq_of(p, b));
+      total += more;
+      longest = max(longest, more);
+    }
+    total = __reduce_add_sync(0xffffffffu, total) * R;
+    per = Q4Deal(p, total, __reduce_max_sync(0xffffffffu, longest)).size;
+  }
+  if (per == 0) {
     b0 = blockIdx.x / R;
+    if (b0 >= p.c.rows) return;
     r0 = blockIdx.x - b0 * R;
     lo = begin = 0;
     seq0 = seq_of(p, b0);
@@ -286,22 +311,11 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       return;
     }
   } else {
-    // Lengths of the first 32 sequences, one per lane; most batches need no more.
-    int seqs = lane < p.c.rows ? seq_of(p, lane) : 0;
-    int n = chunks_of(seqs), total = n, longest = n;
-    for (int b = 32 + lane; b < p.c.rows; b += 32) {
-      const int more = chunks_of(seq_of(p, b));
-      total += more;
-      longest = max(longest, more);
-    }
-    total = __reduce_add_sync(0xffffffffu, total) * R;
-    longest = __reduce_max_sync(0xffffffffu, longest);
     for (int b = blockIdx.x; b < p.c.rows; b += p.ctas)  // sequences of no tokens belong to no range
       if (seq_of(p, b) == 0)
         for (int h = 0; h < p.num_q_heads; h += kQ4Heads)
           for (int k = threadIdx.x; k < kQ4Frags; k += kQ4Threads)
             store_frag<T, NG>(p, b, h, p.num_q_heads - h, k, nothing, 0.f, 0.f);
-    per = range_of(p, total, longest);
     if ((long long)blockIdx.x * per >= total) return;
     lo = blockIdx.x * per;
     hi = min(total, lo + per);
@@ -309,9 +323,9 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
     for (int base = 0;; base += 32) {
       if (base > 0) {
         seqs = base + lane < p.c.rows ? seq_of(p, base + lane) : 0;
-        n = chunks_of(seqs);
+        n32 = chunks_of(seqs);
       }
-      int incl = n * R;
+      int incl = n32 * R;
 #pragma unroll
       for (int x = 1; x < 32; x <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, incl, x);
@@ -319,7 +333,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       }
       const uint32_t past = __ballot_sync(0xffffffffu, before + incl > lo);
       if (past) {
-        const int l0 = __ffs(past) - 1, row_n = __shfl_sync(0xffffffffu, n, l0);
+        const int l0 = __ffs(past) - 1, row_n = __shfl_sync(0xffffffffu, n32, l0);
         const int seq_begin = before + __shfl_sync(0xffffffffu, incl, l0) - row_n * R;
         b0 = base + l0;
         r0 = (lo - seq_begin) / row_n;
@@ -892,8 +906,8 @@ __global__ void __launch_bounds__(kQ4Threads) attn_q4_merge_kernel(const __grid_
   total = __reduce_add_sync(0xffffffffu, total);
   before = __reduce_add_sync(0xffffffffu, before);
   longest = __reduce_max_sync(0xffffffffu, longest);
-  const int per = range_of(p, total * R, longest), begin = before * R + r * n;
-  if (n == 0 || begin / per == (begin + n - 1) / per) return;  // written already
+  const int per = Q4Deal(p, total * R, longest).size, begin = before * R + r * n;
+  if (n == 0 || per == 0 || begin / per == (begin + n - 1) / per) return;  // written already
   const int hb = r % p.head_blocks;
   merge_row<T, NG>(p, b, r / p.head_blocks * p.group + hb * p.block_heads, min(p.block_heads, p.group - hb * p.block_heads),
                    begin, begin + n, per);

@@ -38,6 +38,7 @@ int kv4_check(const dak_kv4_cache *a) {
     return fail(DAK_ERR_UNSUPPORTED, "group must be 32, 64 or 128");
   if (a->batch <= 0 || a->kv_heads <= 0 || a->max_pages <= 0)
     return fail(DAK_ERR_INVALID_ARG, "batch, kv_heads and max_pages must be positive");
+  if (a->kv_heads > 65535) return fail(DAK_ERR_UNSUPPORTED, "at most 65535 KV heads");
   if (a->table_stride < a->max_pages) return fail(DAK_ERR_INVALID_ARG, "table_stride below max_pages");
   if (!a->block_table) return fail(DAK_ERR_INVALID_ARG, "block_table is required");
   if (a->dev_pages < 0 || a->host_pages < 0 || (a->dev_pages > 0) != (a->pool_dev != nullptr) ||
