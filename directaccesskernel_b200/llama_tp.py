@@ -333,7 +333,9 @@ class TPLlamaDecoder(nn.Module):
     def fork(self, src: int, dst: int, tokens: int) -> None:
         """Makes row ``dst`` continue row ``src`` after its first ``tokens`` tokens: copies
         the pages that hold them, in every layer and tier, with one launch on the
-        current stream, and the row's next token and position."""
+        current stream.  The row's position becomes ``tokens`` and its next token
+        ``src``'s, which is the one that follows if ``src`` is at that position too;
+        else set ``ids[dst]``."""
         if not (0 <= src < self.B and 0 <= dst < self.B) or src == dst:
             raise ValueError(f"src and dst must be two different rows of {self.B}")
         if not 0 <= tokens <= self.max_ctx:
@@ -343,7 +345,7 @@ class TPLlamaDecoder(nn.Module):
         n = -(-tokens // PAGE)
         copy_pages(self.kv_dev, self.kv_host, self.host_table[src, :n], self.host_table[dst, :n], page_dim=self.page_dim)
         self.ids[dst].copy_(self.ids[src])
-        self.pos[dst].copy_(self.pos[src])
+        self.pos[dst].fill_(tokens)
 
     def _pools(self, l: int):
         if self.kv_bits == 4:

@@ -116,6 +116,31 @@ def test_fork_continues_like_its_source(kv_bits):
             dec.fork(*bad)
 
 
+@pytest.mark.parametrize("kv_bits", [16, 4])
+@pytest.mark.parametrize("tokens", [0, 1, 63, 64, 66])
+def test_fork_behind_its_source_goes_on_from_there(kv_bits, tokens):
+    """A row forked at an earlier token, fed what its source was fed, comes to the
+    same logits: nothing past ``tokens`` is read before it is written."""
+    cfg = _cfg()
+    dec = _decoder(cfg, batch=3, kv_bits=kv_bits, kv_host_fraction=0.4).load_hf(_hf(cfg, seed=11))
+    prompt = torch.randint(0, cfg.vocab_size, (3, 70), generator=torch.Generator().manual_seed(5)).cuda()
+    _teacher_forced(dec, prompt)
+    dec.set_positions(70)
+    with torch.inference_mode():
+        dec.ids.copy_(prompt[:, 69])
+        dec.set_positions(69)
+        dec.forward_step(keep_logits=True)
+        want = dec.logits_full[1].clone()
+        dec.fork(1, 2, tokens)
+        assert dec.pos.tolist() == [69, 69, tokens]
+        for t in range(tokens, 70):
+            dec.ids[2] = prompt[1, t]
+            dec.pos[2] = t
+            dec.pos[:2] = 69
+            dec.forward_step(keep_logits=True)
+    assert torch.equal(dec.logits_full[2], want) and torch.equal(dec.logits_full[1], want)
+
+
 def test_random_4_bit_pages_are_sane_and_steps_run():
     cfg = _cfg()
     from directaccesskernel_b200.llama_tp import LlamaShape, TPLlamaDecoder
