@@ -393,6 +393,7 @@ extern "C" int dak_kv_read_q4(const dak_kv4_cache *cache, const int32_t *positio
     return fail(DAK_ERR_UNSUPPORTED, "the 4-bit cache is read to float16 and bfloat16");
   if ((st = check_tokens(tokens, positions, seq_index, cache->batch))) return st;
   if (!k_out || !v_out) return fail(DAK_ERR_INVALID_ARG, "k_out and v_out are required");
+  if (k_out == v_out) return fail(DAK_ERR_INVALID_ARG, "k_out and v_out must not overlap");
   if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15u)
     return fail(DAK_ERR_ALIGNMENT, "k_out and v_out must be 16-byte aligned");
   const void *ptrs[4] = {k_out, v_out, positions, seq_index};

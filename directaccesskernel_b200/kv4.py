@@ -118,7 +118,8 @@ def rope_kv_append_q4(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torc
     """Rotary embedding, 4-bit quantisation and append in one launch.
 
     ``qkv`` [tokens, (q_heads + 2 kv_heads) * 128] is the fused projection; its q
-    heads are rotated into ``q_out`` [tokens, q_heads, 128] (None with q_heads 0),
+    heads are rotated into ``q_out`` [tokens, q_heads, 128] (None with q_heads 0; not
+    over ``qkv``),
     its k heads rotated and quantised and its v heads quantised into slot
     ``positions[t]`` of sequence ``seq_index[t]`` (None: one token per sequence,
     in order, as in a decode step; else any tokens of a prompt).  ``inv_freq``,
@@ -210,8 +211,8 @@ def decode_paged_q4(query: torch.Tensor, pool_dev: torch.Tensor | None, pool_hos
     ``merge_counters`` (int32 CUDA, ``merge_counter_count`` entries, zero before
     the first call and left zero by every call) rows that were split are merged
     inside the attention kernel instead of by a second launch; the result is the
-    same.  Calls that may overlap on the GPU need scratch and counters of their
-    own."""
+    same.  ``out`` may be the query itself.  Calls that may overlap on the GPU need
+    scratch and counters of their own."""
     device = current_device_of(query, "query")
     dtype = query.dtype
     if query.dim() != 3 or query.shape[2] != HEAD_DIM or query.stride(2) != 1:

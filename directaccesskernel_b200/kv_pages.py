@@ -11,6 +11,7 @@ sequence (app/python/pinned_static_cache.py:8-115).
 from __future__ import annotations
 
 import math
+from array import array
 
 import torch
 
@@ -23,8 +24,12 @@ MAX_MOVES = 3584  # pages per launch
 
 def _entries(t, name: str) -> torch.Tensor:
     if not isinstance(t, torch.Tensor):
-        return torch.tensor(t, dtype=torch.int32)
-    if t.is_cuda or t.dim() != 1 or t.is_floating_point():
+        try:
+            t = array("i", t)
+        except (TypeError, OverflowError) as e:
+            raise RuntimeError(f"{name} must be a list or a 1-D CPU tensor of page entries ({e})") from None
+        return torch.frombuffer(t, dtype=torch.int32) if t else torch.empty(0, dtype=torch.int32)
+    if t.is_cuda or t.dim() != 1 or t.is_floating_point() or t.is_complex():
         raise RuntimeError(f"{name} must be a list or a 1-D CPU tensor of page entries")
     if t.dtype == torch.int32:
         return t.contiguous()

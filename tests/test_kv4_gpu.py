@@ -345,6 +345,22 @@ def test_attend_same_bits_with_counters_and_every_time():
         assert torch.equal(kv4.decode_paged_q4(q, pool, None, table, lens, 0.09), first)
 
 
+@pytest.mark.parametrize("counters", [True, False])
+@pytest.mark.parametrize("Hq", [8, 72])
+def test_attend_in_place(Hq, counters):
+    """out over the query, with rows that are split, whole and empty."""
+    kv4 = _kv4()
+    g = torch.Generator().manual_seed(Hq)
+    lens = [9000, 0, 70, 4000, 1, 2049]
+    pool = random_pool(200, 4, 64, 128, Hq).cuda()
+    table = torch.randint(0, 200, (6, 141), generator=g, dtype=torch.int32).cuda()
+    q = torch.randn(6, Hq, D, generator=g).to(torch.bfloat16).cuda()
+    cnt = torch.zeros(kv4.merge_counter_count(6, Hq, 4), dtype=torch.int32, device="cuda") if counters else None
+    want = kv4.decode_paged_q4(q, pool, None, table, _i32(lens), 0.1, merge_counters=cnt)
+    assert kv4.decode_paged_q4(q, pool, None, table, _i32(lens), 0.1, merge_counters=cnt, out=q) is q
+    assert torch.equal(q, want)
+
+
 def test_attend_refusals():
     kv4 = _kv4()
     pool = random_pool(4, 2, 16, 32, 16).cuda()

@@ -75,6 +75,8 @@ def test_cache_refusals(bad, status, msg):
     (dict(q_stride_h=100), _lib.DAK_ERR_ALIGNMENT, "strides"),
     (dict(o_stride_b=513), _lib.DAK_ERR_ALIGNMENT, "strides"),
     (dict(out=BUF + 2), _lib.DAK_ERR_ALIGNMENT, "aligned"),
+    (dict(o_stride_b=0), _lib.DAK_ERR_INVALID_ARG, "overlap"),
+    (dict(o_stride_h=64), _lib.DAK_ERR_INVALID_ARG, "overlap"),
 ])
 def test_attention_refusals(bad, status, msg):
     a = _lib.AttnQ4Args()
@@ -125,6 +127,21 @@ def test_append_refusals(bad, status, msg):
     assert st == status and msg in text, text
 
 
+def test_read_refuses_one_output_for_both():
+    st, text = _status(_lib.LIB.dak_kv_read_q4, ctypes.byref(_cache()), BUF, BUF, BUF, BUF, 4, _lib.DTYPE_F16, None)
+    assert st == _lib.DAK_ERR_INVALID_ARG and "overlap" in text, text
+
+
+@pytest.mark.parametrize("src", [[0.5], [[0, 1]], [1 << 31], ["0"], torch.tensor([0.0]), torch.tensor([[0]]),
+                                 torch.tensor([1 << 31])])
+def test_page_lists_are_whole_numbers(src):
+    from directaccesskernel_b200.kv_pages import _entries
+
+    with pytest.raises(RuntimeError):
+        _entries(src, "src")
+    assert _entries([], "src").numel() == 0 and _entries((1, -2), "src").tolist() == [1, -2]
+
+
 def test_rotary_refusals():
     def call(tokens=2, heads=2, d=128, r=128, inter=0, st=(256, 128, 256, 128), x=BUF, out=BUF, dtype=_lib.DTYPE_F16):
         a = _lib.RotaryArgs(x, st[0], st[1], BUF, BUF, out, st[2], st[3], tokens, heads, d, r, inter, 1.0, dtype)
@@ -138,6 +155,8 @@ def test_rotary_refusals():
                             (dict(r=40), _lib.DAK_ERR_UNSUPPORTED, "16"),
                             (dict(st=(252, 128, 256, 128)), _lib.DAK_ERR_ALIGNMENT, "strides"),
                             (dict(out=BUF + 4), _lib.DAK_ERR_ALIGNMENT, "aligned"),
+                            (dict(st=(256, 128, 0, 128)), _lib.DAK_ERR_INVALID_ARG, "overlap"),
+                            (dict(st=(256, 128, 256, 0)), _lib.DAK_ERR_INVALID_ARG, "overlap"),
                             (dict(x=None), _lib.DAK_ERR_INVALID_ARG, "required")):
         st, text = call(**kw)
         assert st == status and msg in text, (kw, text)
