@@ -15,12 +15,19 @@
 // tokens, whose code rows are neighbours in the page.  The append's CTA takes
 // four tokens and up to 48 heads of each: four bulk copies bring them into shared
 // memory, all in flight at once, while the threads work out the tokens' angles,
-// one each, and look up their pages.
+// one each, and look up their pages.  With few heads it takes 8 or 16 tokens, each
+// four with its share of the warps: the start-up is the larger part of a small CTA.
 //
-// Append of 16384 tokens, 32 + 16 heads in bfloat16, groups of 32 (358 MB): 71 us,
-// 5.0 TB/s, 0.79 of the measured copy rate; of 4099 tokens 24 us (38 us when each
-// thread fetched its heads itself and worked out their angles); of 32 tokens
-// 3.1 us.  Read-back of 65536 tokens x 8 heads, groups of 128 (340 MB): 62 us,
+// The instructions count nearly as much as the bytes (249 per head of four tokens,
+// 0.6 of the issue slots, before a q head's angles were kept in registers).  Append
+// of 16384 tokens, 32 + 16 heads in bfloat16, groups of 32 (358 MB): 64 us, 5.6 TB/s,
+// 0.87 of the measured copy rate (75 us); of 4099 tokens 21 us; of 65536 tokens, 8 + 2
+// heads 65 us (109 us with four tokens per CTA); of 32 tokens 3.4 us.  CTAs that
+// walk over tiles of 8 heads with four in flight took a quarter longer (97 us): they
+// wait at each four tokens for positions and pages.  Five or six CTAs per SM with
+// fewer registers, or fewer heads per CTA, took 10 to 30% longer.
+//
+// Read-back of 65536 tokens x 8 heads, groups of 128 (340 MB): 62 us,
 // 5.5 TB/s, 0.85 (75 us with one row in flight per thread).
 #include <cstring>
 
@@ -82,7 +89,9 @@ namespace {
 
 constexpr int kKv4Threads = 256;
 constexpr int kKv4Warps = kKv4Threads / 32;
-constexpr int kAppendHeads = 48;            // of an append's CTA, at most: 48 KB of shared memory
+constexpr int kAppendHeads = 48;            // of four tokens of an append's CTA, at most: 48 KB of shared memory
+constexpr int kAppendTokens = 16;           // of an append's CTA, at most
+constexpr long long kAppendFull = 148 * 4;  // CTAs that the GPU holds at once
 constexpr long long kAppendCtas = 148 * 6;  // an append's CTAs, where its tokens alone give fewer
 constexpr int kReadWarps = 9472;            // a read's warps, likewise
 constexpr int kBatch = 4;                   // rows a reading thread has in flight
@@ -96,19 +105,31 @@ struct AppendParams {
   float scale;
   uint16_t *q_out;
   int tokens, q_heads, rotary_dim, interleaved, units;
-  int slice;  // heads (q, then k, then v) per CTA
+  int slice;   // heads (q, then k, then v) per CTA
+  int groups;  // 1, 2 or 4 groups of four tokens per CTA, each with its share of the warps
   int pdl;
 };
+
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 // Codes of a lane's 16 values and, in the group's first lane, the (scale, zero)
 // pair, from the group's minimum and maximum over the lanes that share it.
 template <int NG>
 __device__ __forceinline__ void kv4_quantise(const float (&x)[16], int lane8, uint8_t *codes, uint8_t *pairs) {
-  float mn = x[0], mx = x[0];
+  float mn = fminf(x[0], x[1]), mx = fmaxf(x[0], x[1]);  // a NaN gives way to any number
 #pragma unroll
-  for (int i = 1; i < 16; ++i) {
-    mn = fminf(mn, x[i]);  // a NaN gives way to any number
-    mx = fmaxf(mx, x[i]);
+  for (int i = 2; i < 16; i += 2) {
+    mn = min3(mn, x[i], x[i + 1]);
+    mx = max3(mx, x[i], x[i + 1]);
   }
 #pragma unroll
   for (int m = 1; m < 8 / NG; m <<= 1) {
@@ -119,11 +140,21 @@ __device__ __forceinline__ void kv4_quantise(const float (&x)[16], int lane8, ui
   const __half s = __float2half_rn(fminf(fmaxf(__fdiv_rn(mx - mn, 15.f), 0.f), 65504.f));
   const float zf = __half2float(z), sf = __half2float(s);
   const float inv = sf > 0.f ? __frcp_rn(sf) : 0.f;
-  uint32_t w[2] = {0u, 0u};
+  // Added to 1.5 x 2^23 a number is rounded to an integer in the sum's low bits, by
+  // an addition instead of rint and a conversion, which run at a quarter of its rate
+  // (2 to 6% of the kernel's time).  The upper bits of eight sums, shifted, add up to
+  // a constant.
+  constexpr float kBig = 12582912.f;
+  constexpr uint32_t kBits = 0x4B400000u;
+  uint32_t w[2];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float n = fminf(fmaxf(rintf((x[i] - zf) * inv), 0.f), 15.f);  // NaN: 0
-    w[i >> 3] |= (uint32_t)n << (4 * (i & 7));
+  for (int j = 0; j < 2; ++j) {
+    w[j] = 0u - kBits * 0x11111111u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float n = fminf(fmaxf(__fadd_rn(__fmul_rn(x[8 * j + i] - zf, inv), kBig), kBig), kBig + 15.f);  // NaN: 0
+      w[j] += __float_as_uint(n) << (4 * i);
+    }
   }
   if (codes) {
     *reinterpret_cast<uint2 *>(codes + lane8 * 8) = make_uint2(w[0], w[1]);
@@ -134,22 +165,26 @@ __device__ __forceinline__ void kv4_quantise(const float (&x)[16], int lane8, ui
 }
 
 struct AppendSmem {
-  alignas(16) float tab[2 * 4 * kKv4Dim / 2];  // angles of the four tokens
-  uint8_t *page[4];
+  uint8_t *page[kAppendTokens];
   uint64_t bar;
-  int tier[4];
+  int tier[kAppendTokens];
   int abort_flag[2];  // [1]: of the second wait
 };
 
-// A head of the four tokens at a time per warp: q heads are rotated, k heads
-// rotated and packed, v heads packed.
-template <typename T, int NG>
+// G groups of four tokens, one for each G-th of the warps; a head of the four at a
+// time per warp: q heads are rotated, k heads rotated and packed, v heads packed.
+template <typename T, int NG, int G>
 __global__ void __launch_bounds__(kKv4Threads, 4) kv4_append_kernel(const __grid_constant__ AppendParams p) {
-  extern __shared__ __align__(128) uint8_t rows_s[];  // [tokens][slice][128] 16-bit, then the rest
-  AppendSmem &sm = *reinterpret_cast<AppendSmem *>(rows_s + 4 * p.slice * kKv4Dim * 2);
+  extern __shared__ __align__(128) uint8_t rows_s[];  // [tokens][slice][128] 16-bit, then angles, then the rest
+  constexpr int ct = 4 * G;                           // tokens of the CTA
+  const int stride = rope_stride(p.rotary_dim);
+  float *tab = reinterpret_cast<float *>(rows_s + ct * p.slice * kKv4Dim * 2);
+  AppendSmem &sm = *reinterpret_cast<AppendSmem *>(tab + 2 * ct * stride);
   pdl_enter(p.pdl);
-  const int t0 = blockIdx.x * 4, nt = min(4, p.tokens - t0);
-  const int lane8 = lane_id() & 7, sub = lane_id() >> 3;
+  const int t0 = blockIdx.x * ct, nt = min(ct, p.tokens - t0);
+  // A warp takes every warps-th head of four of the tokens.
+  constexpr int warps = kKv4Warps / G;
+  const int lane8 = lane_id() & 7, sub = warp_id() / warps * 4 + (lane_id() >> 3);
   const bool live = sub < nt;
   const int t = t0 + (live ? sub : 0);  // idle lanes stay for the shuffles
   const int P = p.c.page_size, Hkv = p.c.kv_heads;
@@ -175,10 +210,9 @@ __global__ void __launch_bounds__(kKv4Threads, 4) kv4_append_kernel(const __grid
     sm.page[threadIdx.x] = page;
     sm.tier[threadIdx.x] = tier;
   }
-  const int stride = rope_stride(p.rotary_dim);
-  rope_table(sm.tab, p.positions + t0, nt, 4, p.inv_freq, p.rotary_dim, p.scale);
+  rope_table(tab, p.positions + t0, nt, ct, p.inv_freq, p.rotary_dim, p.scale);
   __syncthreads();
-  const float *cos_row = sm.tab + (live ? sub : 0) * stride, *sin_row = cos_row + 4 * stride;
+  const float *cos_row = tab + (live ? sub : 0) * stride, *sin_row = cos_row + ct * stride;
   const int slot = p.positions[t] & (P - 1);
   uint8_t *page = live ? sm.page[sub] : nullptr;
   const int half = kv4_half_bytes(P, NG);
@@ -189,35 +223,47 @@ __global__ void __launch_bounds__(kKv4Threads, 4) kv4_append_kernel(const __grid
     return;
   }
 
-  for (int h = h0 + warp_id(); h < h_end; h += kKv4Warps) {
-    const uint4 *src = reinterpret_cast<const uint4 *>(row + (h - h0) * kKv4Dim * 2);
-    if (h < p.q_heads) {
-      if (!live) continue;
-      uint4 *dst = reinterpret_cast<uint4 *>(p.q_out + ((long long)t * p.q_heads + h) * kKv4Dim);
-      for (int u = lane8; u < p.units; u += 8) {
-        const RopeUnit unit = rope_unit(u, R, p.interleaved);
-        float c[8], s[8];
-        rope_unit_angles(unit, cos_row, sin_row, c, s);
-        rope_unit_apply<T>(unit, p.interleaved, src[unit.v0], src[unit.v1 >= 0 ? unit.v1 : unit.v0], c, s, dst);
-      }
-      continue;
+  // q: a unit at a time, its angles in registers for all of the warp's heads.
+  constexpr int row_vecs = kKv4Dim / 8;
+  const uint4 *vecs = reinterpret_cast<const uint4 *>(row);
+  int h = h0 + warp_id() % warps;
+  const int q_end = min(h_end, p.q_heads), k_end = min(h_end, p.q_heads + Hkv);
+  for (int u = live ? lane8 : p.units; u < p.units; u += 8) {
+    const RopeUnit unit = rope_unit(u, R, p.interleaved);
+    float c[8], s[8];
+    rope_unit_angles(unit, cos_row, sin_row, c, s);
+    uint4 *dst = reinterpret_cast<uint4 *>(p.q_out) + ((long long)t * p.q_heads + h) * row_vecs;
+    const uint4 *src = vecs + (h - h0) * row_vecs;
+    for (int i = h; i < q_end; i += warps) {
+      rope_unit_apply<T>(unit, p.interleaved, src[unit.v0], src[unit.v1 >= 0 ? unit.v1 : unit.v0], c, s, dst);
+      src += warps * row_vecs;
+      dst += warps * row_vecs;
     }
-    const int isv = h >= p.q_heads + Hkv ? 1 : 0;
+  }
+  if (h < q_end) h += (q_end - h + warps - 1) / warps * warps;
+  // k and v: 16 dims a lane.
+  uint8_t *codes = page ? page + slot * 64 : nullptr, *pairs = page ? page + P * 64 + slot * 4 * NG : nullptr;
+  auto store = [&](const float(&x)[16], long long at) {
+    kv4_quantise<NG>(x, lane8, page ? codes + at : nullptr, pairs + at);
+  };
+  for (; h < k_end; h += warps) {
+    const uint4 *src = vecs + (h - h0) * row_vecs;
     float x[16];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       float y[8];
       const int v = lane8 * 2 + k;
       unpack8<T>(src[v], y);
-      if (!isv && !p.interleaved && v < 2 * part) {
+      if (!p.interleaved && v < 2 * part) {
         float z[8], c[8], s[8];
         unpack8<T>(src[v < part ? v + part : v - part], z);  // each lane keeps its own side of the pairs
         const int f = 8 * (v < part ? v : v - part);
         load4(cos_row + f, c), load4(cos_row + f + 4, c + 4);
         load4(sin_row + f, s), load4(sin_row + f + 4, s + 4);
+        const float sign = v < part ? -1.f : 1.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = fmaf(y[i], c[i], z[i] * (v < part ? -s[i] : s[i]));
-      } else if (!isv && p.interleaved && v * 8 < R) {
+        for (int i = 0; i < 8; ++i) y[i] = fmaf(y[i], c[i], z[i] * (s[i] * sign));
+      } else if (p.interleaved && v * 8 < R) {
         float c[4], s[4];
         load4(cos_row + 4 * v, c);
         load4(sin_row + 4 * v, s);
@@ -228,8 +274,18 @@ __global__ void __launch_bounds__(kKv4Threads, 4) kv4_append_kernel(const __grid
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[8 * k + i] = y[i];
     }
-    uint8_t *slab = page ? page + (long long)(h - p.q_heads - isv * Hkv) * p.c.slab_bytes + isv * half : nullptr;
-    kv4_quantise<NG>(x, lane8, slab ? slab + slot * 64 : nullptr, slab ? slab + P * 64 + slot * 4 * NG : nullptr);
+    store(x, (long long)(h - p.q_heads) * p.c.slab_bytes);
+  }
+  for (; h < h_end; h += warps) {
+    const uint4 *src = vecs + (h - h0) * row_vecs + 2 * lane8;
+    float x[16], y[8];
+    unpack8<T>(src[0], y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = y[i];
+    unpack8<T>(src[1], y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[8 + i] = y[i];
+    store(x, (long long)(h - p.q_heads - Hkv) * p.c.slab_bytes + half);
   }
   // Host pages are read back over the host link by the next kernels of the
   // stream; make the writes visible system-wide before this grid completes.
@@ -295,11 +351,19 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_read_kernel(const __grid_cons
   }
 }
 
+template <typename T, int NG, int G>
+cudaError_t launch_append_t(const AppendParams &p, dim3 grid, cudaStream_t s) {
+  auto kern = kv4_append_kernel<T, NG, G>;
+  const cudaError_t e = prepare_kernel_attributes(reinterpret_cast<const void *>(kern));
+  const size_t smem = 4 * G * (p.slice * kKv4Dim * 2 + 2 * rope_stride(p.rotary_dim) * sizeof(float)) + sizeof(AppendSmem);
+  return e != cudaSuccess ? e : launch_ex(kern, grid, dim3(kKv4Threads), smem, s, 1, p.pdl != 0, p);
+}
+
 template <typename T, int NG>
 cudaError_t launch_append_g(const AppendParams &p, dim3 grid, cudaStream_t s) {
-  auto kern = kv4_append_kernel<T, NG>;
-  const cudaError_t e = prepare_kernel_attributes(reinterpret_cast<const void *>(kern));
-  return e != cudaSuccess ? e : launch_ex(kern, grid, dim3(kKv4Threads), 4 * p.slice * kKv4Dim * 2 + sizeof(AppendSmem), s, 1, p.pdl != 0, p);
+  return p.groups == 1   ? launch_append_t<T, NG, 1>(p, grid, s)
+         : p.groups == 2 ? launch_append_t<T, NG, 2>(p, grid, s)
+                         : launch_append_t<T, NG, 4>(p, grid, s);
 }
 
 template <typename T>
@@ -376,8 +440,15 @@ extern "C" int dak_rope_kv_append_q4(const dak_kv4_cache *cache, const dak_kv4_a
   const long long slices = std::max((heads + kAppendHeads - 1) / kAppendHeads,
                                     std::min((heads + kKv4Warps - 1) / kKv4Warps, kAppendCtas / quads));
   if (heads > 65535ll * kKv4Warps) return fail(DAK_ERR_UNSUPPORTED, "too many heads");
-  p.slice = (int)(((heads + slices - 1) / slices + kKv4Warps - 1) / kKv4Warps * kKv4Warps);
-  const dim3 grid((unsigned)quads, (unsigned)((heads + p.slice - 1) / p.slice));
+  p.slice = (int)(slices == 1 ? heads : ((heads + slices - 1) / slices + kKv4Warps - 1) / kKv4Warps * kKv4Warps);
+  // Few heads of many tokens: more tokens per CTA, each of which starts up once, as
+  // far as the shared memory of 48 heads goes and half the GPU still gets a CTA.  8 + 2
+  // heads of 2500 tokens: 5.7 us, 7.3 without; of 65536: 65 and 109.
+  p.groups = 1;
+  while (4 * p.groups < kAppendTokens && 2 * p.groups * p.slice <= kAppendHeads && heads <= p.slice &&
+         quads >= p.groups * kAppendFull)
+    p.groups *= 2;
+  const dim3 grid((unsigned)((quads + p.groups - 1) / p.groups), (unsigned)((heads + p.slice - 1) / p.slice));
   auto s = static_cast<cudaStream_t>(stream);
   return cuda_status(a->dtype == DAK_DTYPE_F16 ? launch_append<__half>(p, grid, s)
                                                : launch_append<__nv_bfloat16>(p, grid, s),

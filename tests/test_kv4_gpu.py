@@ -97,6 +97,33 @@ def test_append(T, B, Hq, Hkv, page, group, rotary_dim, inter, scale, pad, decod
         assert (t.view(torch.int16).transpose(1, 2)[~touched] == torch.tensor(0xABAB - 65536, dtype=torch.int16)).all()
 
 
+@pytest.mark.parametrize("T,Hq,Hkv,page,group,rotary_dim,inter", [
+    (2371, 1, 1, 64, 128, 128, False), (4739, 2, 1, 16, 64, 64, True), (5003, 0, 3, 32, 32, 48, False),
+    (3001, 16, 3, 64, 64, 128, False), (9998, 6, 3, 32, 128, 0, False), (4737, 11, 7, 64, 32, 128, True)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_append_of_many_tokens_is_that_of_few(T, Hq, Hkv, page, group, rotary_dim, inter, dtype):
+    """Many tokens share a CTA: one call writes the bytes that calls of 500 tokens write
+    (which test_append compares with the formula), in both tiers."""
+    kv4 = _kv4()
+    B = 101
+    qkv, seq, pos, table, n_dev, n_host, inv = _append_case(T, B, Hq, Hkv, page, group, rotary_dim, inter, 1.1, dtype, T)
+    qkv, pos, seq, table = qkv.cuda(), pos.int().cuda(), seq.int().cuda(), table.int().cuda()
+    inv = inv.cuda() if inv is not None else None
+    got = []
+    for step in (T, 500):
+        dev = torch.full((n_dev, Hkv, kv4.page_bytes(page, group)), 0xAB, dtype=torch.uint8, device="cuda")
+        host = torch.full((n_host, Hkv, kv4.page_bytes(page, group)), 0xAB, dtype=torch.uint8).pin_memory()
+        q_out = torch.zeros(T, Hq, D, dtype=dtype, device="cuda")
+        for i in range(0, T, step):
+            n = slice(i, min(T, i + step))
+            kv4.rope_kv_append_q4(qkv[n], pos[n], inv, Hq, q_out[n] if Hq else None, dev, host, table, seq_index=seq[n],
+                                  interleaved=inter, rope_scale=1.1)
+        torch.cuda.synchronize()
+        got.append((dev, host, q_out))
+    for one, other in zip(*got):
+        assert torch.equal(one, other)
+
+
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_append_of_extreme_values(group):
     """Constant groups, the type's extremes, infinities and NaN: finite, saturated contents."""
