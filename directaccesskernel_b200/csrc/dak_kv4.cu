@@ -27,8 +27,9 @@
 // wait at each four tokens for positions and pages.  Five or six CTAs per SM with
 // fewer registers, or fewer heads per CTA, took 10 to 30% longer.
 //
-// Read-back of 65536 tokens x 8 heads, groups of 128 (340 MB): 62 us,
-// 5.5 TB/s, 0.85 (75 us with one row in flight per thread).
+// Read-back of 65536 tokens x 8 heads, groups of 128 (340 MB): 58 us, 5.9 TB/s, 0.91
+// (63 us with four rows in flight per thread and four CTAs per SM, 75 with one row);
+// of 257 tokens 2.3 us.
 #include <cstring>
 
 #include "dak_host.h"
@@ -93,8 +94,9 @@ constexpr int kAppendHeads = 48;            // of four tokens of an append's CTA
 constexpr int kAppendTokens = 16;           // of an append's CTA, at most
 constexpr long long kAppendFull = 148 * 4;  // CTAs that the GPU holds at once
 constexpr long long kAppendCtas = 148 * 6;  // an append's CTAs, where its tokens alone give fewer
-constexpr int kReadWarps = 9472;            // a read's warps, likewise
-constexpr int kBatch = 4;                   // rows a reading thread has in flight
+constexpr long long kReadWarps = 9472;      // a read's warps, likewise
+constexpr int kReadRows = 8;                // of a token on one warp of a read, at most
+constexpr int kBatch = 2;                   // rows a reading thread has in flight
 
 struct AppendParams {
   Kv4Cache c;
@@ -300,7 +302,7 @@ struct ReadParams {
 };
 
 template <typename T, int NG>
-__global__ void __launch_bounds__(kKv4Threads) kv4_read_kernel(const __grid_constant__ ReadParams p) {
+__global__ void __launch_bounds__(kKv4Threads, 5) kv4_read_kernel(const __grid_constant__ ReadParams p) {
   pdl_enter(p.pdl);
   const long long w = (long long)blockIdx.x * kKv4Warps + warp_id();
   const int g = (int)(w % p.groups);
@@ -480,8 +482,11 @@ extern "C" int dak_kv_read_q4(const dak_kv4_cache *cache, const int32_t *positio
   p.out[1] = static_cast<uint16_t *>(v_out);
   p.tokens = tokens;
   const long long quads = (tokens + 3ll) / 4;
-  // One row per warp until the GPU is full, then more.
-  p.groups = (int)std::min<long long>(2ll * cache->kv_heads, std::max<long long>(1, kReadWarps / quads));
+  // One row per warp until the GPU is full, then more, up to eight: a warp that took
+  // all 16 rows of 8 heads wrote to so many places that HBM slowed down (65536 tokens:
+  // 57 us with 8 rows per warp, 62 with 16 or 4).
+  const long long rows = 2ll * cache->kv_heads;
+  p.groups = (int)std::max((rows + kReadRows - 1) / kReadRows, std::min(rows, kReadWarps / quads));
   p.pdl = decode_pdl_enabled() ? 1 : 0;
   const long long grid = (quads * p.groups + kKv4Warps - 1) / kKv4Warps;
   if (grid > 0x7fffffffll) return fail(DAK_ERR_UNSUPPORTED, "too many tokens for one launch");
