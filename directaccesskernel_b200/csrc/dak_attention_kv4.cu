@@ -18,17 +18,18 @@
 //   O^T [128 dims x 8 heads] += V^T P^T, with the token's scale multiplied into P
 //     and its zero added to O as sum_t p_t zero_t per chunk.
 // Codes never become floating-point values of their own: K's bytes enter integer
-// MMAs as they are (see "Scores" below), V's nibbles enter as float16 subnormals
-// (bits 0-3 of a half word are code * 2^-24, bits 4-7 code * 2^-20), so that two
-// masks and a byte permutation are all that they take.  P is float16: for bfloat16
+// MMAs as they are (see "Scores" below); V's enter as float16 subnormals, its even
+// codes and its whole bytes (even + 16 odd, units of 2^-24), which a mask or a byte
+// permutation each give; the odd dims are the difference, at the end (masks and
+// shifts for each nibble took 1 to 3% longer).  P is float16: for bfloat16
 // outputs in one term (2^-11 relative, an eighth of the output's own rounding),
 // for float16 outputs in two, because one made the output up to 1.9 times less
 // exact than its rounding and two do not show.
 //
 // Bound, at 32 x 16384 tokens of 8 KV heads (570 MB, 89 us at the measured copy
-// rate): 108 us in bfloat16, 119 us in float16.  The copies alone take 91 us; the
+// rate): 108 us in bfloat16, 116 us in float16.  The copies alone take 91 us; the
 // rest is arithmetic that two warps per scheduler do not quite hide (4.3 cycles
-// per instruction and warp, 825 instructions per chunk).  Plain bulk
+// per instruction and warp, about 800 instructions per chunk).  Plain bulk
 // copies replaced tensor copies with a 64-byte swizzle: bank conflicts cost less
 // than the 64-byte rows did, and host pages come 15% faster (46 GB/s).
 #include <cfloat>
@@ -682,13 +683,14 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       for (int n = 0; n < NG; ++n)
 #pragma unroll
         for (int x = 4; x <= 16; x <<= 1) zs[e][n] += __shfl_xor_sync(0xffffffffu, zs[e][n], x);
-    // O rows: even dims count codes * 2^-24, odd dims * 2^-20.  Adding the zeros'
-    // share chunk by chunk keeps O centred, so nothing cancels at the end.
+    // O rows: even dims in units of 2^-24, and the sum of an even dim and 16 times the
+    // odd one beside it.  Adding the zeros' share chunk by chunk keeps O centred, so
+    // nothing cancels at the end.
 #pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
-        const float even = zs[e][n] * 0x1p-24f, odd = zs[e][n] * 0x1p-20f;
+        const float even = zs[e][n] * 0x1p-24f, odd = zs[e][n] * (17 * 0x1p-24f);
 #pragma unroll
         for (int t = 8 * n / NG; t < 8 * (n + 1) / NG; ++t) {
           o[t][e] = fmaf(o[t][e], alpha[e], even);
@@ -746,15 +748,16 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int n = q * NG / 4;
-        const uint32_t s0 = x[0][q] >> 8, s1 = x[1][q] >> 8;
-        mma_f16(o[2 * q], x[0][q] & 0x000F000Fu, x[0][q] & 0x00F000F0u, x[1][q] & 0x000F000Fu, x[1][q] & 0x00F000F0u,
-                bf[n][0], bf[n][1]);
-        mma_f16(o[2 * q + 1], s0 & 0x000F000Fu, s0 & 0x00F000F0u, s1 & 0x000F000Fu, s1 & 0x00F000F0u, bf[n][0], bf[n][1]);
+        // Bytes 0 and 2 (even code + 16 odd), then bytes 1 and 3; their even codes.
+        const uint32_t b0 = x[0][q] & 0x00FF00FFu, b1 = x[1][q] & 0x00FF00FFu;
+        const uint32_t c0 = __byte_perm(x[0][q], 0u, 0x4341u), c1 = __byte_perm(x[1][q], 0u, 0x4341u);
+        const uint32_t e0 = x[0][q] & 0x000F000Fu, e1 = x[1][q] & 0x000F000Fu;
+        const uint32_t f0 = c0 & 0x000F000Fu, f1 = c1 & 0x000F000Fu;
+        mma_f16(o[2 * q], e0, b0, e1, b1, bf[n][0], bf[n][1]);
+        mma_f16(o[2 * q + 1], f0, c0, f1, c1, bf[n][0], bf[n][1]);
         if constexpr (kTwoTerms) {
-          mma_f16(o[2 * q], x[0][q] & 0x000F000Fu, x[0][q] & 0x00F000F0u, x[1][q] & 0x000F000Fu, x[1][q] & 0x00F000F0u,
-                  bl[n][0], bl[n][1]);
-          mma_f16(o[2 * q + 1], s0 & 0x000F000Fu, s0 & 0x00F000F0u, s1 & 0x000F000Fu, s1 & 0x00F000F0u, bl[n][0],
-                  bl[n][1]);
+          mma_f16(o[2 * q], e0, b0, e1, b1, bl[n][0], bl[n][1]);
+          mma_f16(o[2 * q + 1], f0, c0, f1, c1, bl[n][0], bl[n][1]);
         }
       }
     }
@@ -839,8 +842,8 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
           float4 v = turn == 0 ? nothing : sm_o[t * 32 + lane];
           v.x = fmaf(o[t][0], even[0], v.x);
           v.y = fmaf(o[t][1], even[1], v.y);
-          v.z = fmaf(o[t][2], odd[0], v.z);
-          v.w = fmaf(o[t][3], odd[1], v.w);
+          v.z = fmaf(o[t][2] - o[t][0], odd[0], v.z);
+          v.w = fmaf(o[t][3] - o[t][1], odd[1], v.w);
           sm_o[t * 32 + lane] = v;
         }
       }
