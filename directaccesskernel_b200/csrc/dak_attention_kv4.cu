@@ -4,11 +4,11 @@
 // One query token per sequence: o = softmax(scaling q K^T) V over the first
 // seq_lens[b] tokens, K and V being scale * code + zero.  A row is one
 // (sequence, KV head, block of up to 8 query heads); its tokens are cut into
-// chunks of 64.  The chunks of all rows, laid end to end, are dealt out in equal
-// contiguous ranges, one to each CTA that the GPU holds at once, whatever the
-// lengths: a CTA walks over its range row by row, its four warps taking every
-// fourth chunk, with copies running ahead across rows.  A row that spans CTAs is
-// merged by log-sum-exp.  Scores are kept in base 2; a sequence of no tokens
+// chunks of 64, and the chunks of all rows are dealt out to the CTAs that the GPU
+// holds at once, whatever the lengths (Q4Deal): a CTA takes a piece of one row, or a
+// range over several rows, which it walks over row by row; its four warps take
+// every fourth chunk, with copies running ahead across rows.  A row that spans CTAs
+// is merged by log-sum-exp.  Scores are kept in base 2; a sequence of no tokens
 // gives zeros.
 //
 // A warp has two chunks in flight, each a bulk copy per page (one contiguous slab
@@ -54,7 +54,7 @@ constexpr int kQ4Heads = 8;    // query heads per CTA: the MMA's N
 constexpr int kQ4Chunk = 64;   // tokens a warp takes at a time
 constexpr int kQ4Stages = 2;   // chunks in flight per warp
 constexpr int kQ4MergeBatch = 6;  // pieces of a row read at once
-constexpr int kQ4RowSlack = 11;   // see Q4Deal
+constexpr int kQ4Slack = 8;      // see Q4Deal
 constexpr int kQ4RowChunks = 8;  // rows up to this long are not split while the GPU holds them all
 
 struct AttnQ4Params {
@@ -73,13 +73,13 @@ struct AttnQ4Params {
   int pdl;
 };
 
-// Shared memory of a CTA: per warp a ring of chunks; the warps' statistics and
-// one block of outputs that they add up in turn; barriers.
+// Shared memory of a CTA: per warp a ring of chunks, a block of outputs and its
+// statistics; barriers.
 template <int NG>
 struct Q4Smem {
   static constexpr uint32_t stage = 2 * kQ4Chunk * (64 + 4 * NG);
-  static constexpr uint32_t o_off = kQ4Warps * kQ4Stages * stage;         // [heads][128]
-  static constexpr uint32_t m_off = o_off + kQ4Heads * kKv4Dim * 4;       // [warps][heads]
+  static constexpr uint32_t o_off = kQ4Warps * kQ4Stages * stage;               // [warps][heads][128]
+  static constexpr uint32_t m_off = o_off + kQ4Warps * kQ4Heads * kKv4Dim * 4;  // [warps][heads]
   static constexpr uint32_t l_off = m_off + kQ4Warps * kQ4Heads * 4;
   static constexpr uint32_t bar_off = l_off + kQ4Warps * kQ4Heads * 4;
   static constexpr uint32_t flag_off = bar_off + kQ4Warps * kQ4Stages * 8;   // abort, abort of the drain, last
@@ -185,33 +185,93 @@ __device__ __forceinline__ int seq_of(const AttnQ4Params &p, int b) {
 }
 __device__ __forceinline__ int chunks_of(int seq) { return (seq + kQ4Chunk - 1) / kQ4Chunk; }
 
-// How the chunks are dealt out, given the sum over all rows and the longest row:
-// equal ranges of `size` chunks, at least one for each warp, or a row for each CTA.
+// How the chunks are dealt out: rows are cut into pieces of `size` chunks, a piece
+// for each CTA (whole), or ranges of `size` chunks of all rows, end to end, a range
+// for each CTA.
 //
 // Merging a row costs the CTA that does it about 0.1 us per piece, and four chunks,
-// one per warp, take 1.3 us: a row of n chunks is best cut into about sqrt(3 n)
+// one per warp, take 1.5 us: a row of n chunks is best cut into about sqrt(3 n)
 // pieces, which matters where one or two rows are all there is (one row of 131072
-// tokens: 57 us in 293 pieces, 27 in 79).  Where there is a CTA for every row, whole
-// rows save the merge and the second row of a range, together about 4 us, or 11
-// chunks: they are dealt if the longest is no further than that from the equal share.
+// tokens: 57 us in 293 pieces, 27 in 79).  A range with chunks of two rows takes
+// longer than one of a single row, by the first row's end and warps without a chunk
+// there: pieces of up to kQ4Slack chunks more are taken before ranges.  24 ragged
+// sequences of up to 6001 tokens: 12.3 us, 19.7 in ranges; 16 of up to 20000: 16 and
+// 30; 32 x 16384 of one KV head: 23.3 and 24.9.
 struct Q4Deal {
-  int size;  // 0: CTA i takes row i
-  __device__ __forceinline__ Q4Deal(const AttnQ4Params &p, int total, int longest) {
-    const int share = (total + p.ctas - 1) / p.ctas;
-    size = max(max(share, kQ4Warps), (int)sqrtf(longest * (1.f / 3.f)));
-    if (p.by_row || (p.c.rows * p.c.kv_heads * p.head_blocks <= p.ctas && longest <= share + kQ4RowSlack)) size = 0;
-  }
+  int size;
+  bool whole;
+  int ctas;   // with work
+  int total;  // chunks
 };
+// ceil(n / size), for up to 2^20 pieces (here at most p.ctas), in a fraction of a
+// division's latency: the rounded quotient is at most two too small.
+__device__ __forceinline__ int pieces_of(int n, int size, float rcp) {
+  const uint32_t k = (uint32_t)(n * rcp), at = k * size;
+  return (int)(k + (at < (uint32_t)n) + (at + size < (uint32_t)n));
+}
+__device__ __forceinline__ float rcp_of(int size) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((float)size));
+  return r;
+}
+__device__ __forceinline__ float sqrt_of(float x) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// n32: chunks of sequence lane_id(); all lanes get the answer.
+__device__ __forceinline__ Q4Deal q4_deal(const AttnQ4Params &p, int n32) {
+  constexpr int kBlocks = 3;  // of 32 sequences behind the first whose lengths stay in registers
+  const int lane = lane_id(), R = p.c.kv_heads * p.head_blocks;
+  int total = n32, longest = n32, more[kBlocks] = {0, 0, 0};
+  if (p.c.rows > 32) {
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) {
+      const int b = 32 * (i + 1) + lane;
+      more[i] = b < p.c.rows ? chunks_of(seq_of(p, b)) : 0;
+      total += more[i];
+      longest = max(longest, more[i]);
+    }
+    for (int b = 32 * (kBlocks + 1) + lane; b < p.c.rows; b += 32) {
+      const int n = chunks_of(seq_of(p, b));
+      total += n;
+      longest = max(longest, n);
+    }
+  }
+  total = __reduce_add_sync(0xffffffffu, total) * R;
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  Q4Deal d;
+  d.total = total;
+  d.size = max(max((int)(((uint32_t)total + p.ctas - 1) / p.ctas), kQ4Warps), (int)sqrt_of(longest * (1.f / 3.f)));
+  d.whole = true;
+  const int least = (d.size + kQ4Warps - 1) / kQ4Warps * kQ4Warps;
+  for (int size = least; size <= least + kQ4Slack; size += kQ4Warps) {
+    const float rcp = rcp_of(size);
+    int pieces = pieces_of(n32, size, rcp);
+    if (p.c.rows > 32) {
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i) pieces += pieces_of(more[i], size, rcp);
+      for (int b = 32 * (kBlocks + 1) + lane; b < p.c.rows; b += 32) pieces += pieces_of(chunks_of(seq_of(p, b)), size, rcp);
+    }
+    d.ctas = __reduce_add_sync(0xffffffffu, pieces) * R;
+    if (d.ctas <= p.ctas) {
+      d.size = size;
+      return d;
+    }
+  }
+  d.whole = false;
+  d.ctas = (int)(((uint32_t)total + d.size - 1) / d.size);
+  return d;
+}
 
-// Merges row (b, r), whose chunks are [begin, end) of all in ranges of `per`, from
-// its pieces in the scratch, in order.  Piece i is CTA i's first segment (slot
-// 2 i), or, if the row begins within CTA i's range, its last (slot 2 i + 1).
+// Merges a row from its pieces in the scratch, in order.  They were left by CTA
+// `first` and those after it, as their first segments (slot 2 i of CTA i), or, if the
+// row begins within `first`'s range (late), as its last (slot 2 i + 1).
 template <typename T, int NG>
-__device__ __forceinline__ void merge_row(const AttnQ4Params &p, int b, int h0, int nh, int begin, int end, int per) {
-  const int first = begin / per, pieces = (end - 1) / per - first + 1;
+__device__ __forceinline__ void merge_row(const AttnQ4Params &p, int b, int h0, int nh, int first, int pieces, bool late) {
   const float4 *po = reinterpret_cast<const float4 *>(p.scratch);
   const float4 *pm = po + 2ll * p.ctas * kQ4Frags;  // (m, l) of two heads
-  auto slot = [&](int i) { return 2ll * (first + i) + ((first + i) * per < begin ? 1 : 0); };
+  auto slot = [&](int i) { return 2ll * (first + i) + (late && i == 0 ? 1 : 0); };
   const int k = threadIdx.x;  // this thread's float4s, of the same two heads: k and k + kQ4Threads
   float m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
   float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
@@ -281,25 +341,19 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
   // This CTA's range of chunks [lo, hi) and the row (b0, r0) that it begins in,
   // whose chunks begin at `begin`.
   const int R = p.c.kv_heads * p.head_blocks;
-  int lo, hi, begin, b0, r0, seq0, per = 0;
+  int lo, hi, begin, b0, r0, seq0;
+  int per = 0;                // chunks of a range; 0: the CTA has a piece of one row,
+  int first = 0, pieces = 1;  // of so many, the first of which CTA `first` has
   const float4 nothing = make_float4(0.f, 0.f, 0.f, 0.f);
-  // Lengths of the first 32 sequences, one per lane; most batches need no more.
-  int seqs = 0, n32 = 0, total = 0;
-  if (!p.by_row) {
-    seqs = lane < p.c.rows ? seq_of(p, lane) : 0;
-    n32 = total = chunks_of(seqs);
-    int longest = total;
-    for (int b = 32 + lane; b < p.c.rows; b += 32) {
-      const int more = chunks_of(seq_of(p, b));
-      total += more;
-      longest = max(longest, more);
-    }
-    total = __reduce_add_sync(0xffffffffu, total) * R;
-    per = Q4Deal(p, total, __reduce_max_sync(0xffffffffu, longest)).size;
-  }
-  if (per == 0) {
+  auto zero_rows = [&]() {  // sequences of no tokens belong to no CTA
+    for (int b = blockIdx.x; b < p.c.rows; b += p.ctas)
+      if (seq_of(p, b) == 0)
+        for (int h = 0; h < p.num_q_heads; h += kQ4Heads)
+          for (int k = threadIdx.x; k < kQ4Frags; k += kQ4Threads)
+            store_frag<T, NG>(p, b, h, p.num_q_heads - h, k, nothing, 0.f, 0.f);
+  };
+  if (p.by_row) {
     b0 = blockIdx.x / R;
-    if (b0 >= p.c.rows) return;
     r0 = blockIdx.x - b0 * R;
     lo = begin = 0;
     seq0 = seq_of(p, b0);
@@ -312,37 +366,51 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       return;
     }
   } else {
-    for (int b = blockIdx.x; b < p.c.rows; b += p.ctas)  // sequences of no tokens belong to no range
-      if (seq_of(p, b) == 0)
-        for (int h = 0; h < p.num_q_heads; h += kQ4Heads)
-          for (int k = threadIdx.x; k < kQ4Frags; k += kQ4Threads)
-            store_frag<T, NG>(p, b, h, p.num_q_heads - h, k, nothing, 0.f, 0.f);
-    if ((long long)blockIdx.x * per >= total) return;
-    lo = blockIdx.x * per;
-    hi = min(total, lo + per);
-    int before = 0;  // chunks of the sequences before this block of 32
+    // Lengths of 32 sequences, one per lane; most batches have no more.
+    int seqs = lane < p.c.rows ? seq_of(p, lane) : 0;
+    int n32 = chunks_of(seqs);
+    const Q4Deal deal = q4_deal(p, n32);
+    if ((int)blockIdx.x >= deal.ctas) {
+      zero_rows();
+      return;
+    }
+    // The row in which unit `from` lies, a unit being a piece or a chunk.
+    const int from = deal.whole ? blockIdx.x : blockIdx.x * deal.size;
+    int before = 0;  // units of the sequences before this block of 32
     for (int base = 0;; base += 32) {
       if (base > 0) {
         seqs = base + lane < p.c.rows ? seq_of(p, base + lane) : 0;
         n32 = chunks_of(seqs);
       }
-      int incl = n32 * R;
+      const int units = deal.whole ? pieces_of(n32, deal.size, rcp_of(deal.size)) : n32;
+      int incl = units * R;
 #pragma unroll
       for (int x = 1; x < 32; x <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, incl, x);
         if (lane >= x) incl += v;
       }
-      const uint32_t past = __ballot_sync(0xffffffffu, before + incl > lo);
+      const uint32_t past = __ballot_sync(0xffffffffu, before + incl > from);
       if (past) {
-        const int l0 = __ffs(past) - 1, row_n = __shfl_sync(0xffffffffu, n32, l0);
-        const int seq_begin = before + __shfl_sync(0xffffffffu, incl, l0) - row_n * R;
+        const int l0 = __ffs(past) - 1, row_units = __shfl_sync(0xffffffffu, units, l0);
+        const int seq_begin = before + __shfl_sync(0xffffffffu, incl, l0) - row_units * R;
         b0 = base + l0;
-        r0 = (lo - seq_begin) / row_n;
-        begin = seq_begin + r0 * row_n;
+        r0 = (from - seq_begin) / row_units;
+        begin = seq_begin + r0 * row_units;
         seq0 = __shfl_sync(0xffffffffu, seqs, l0);
+        pieces = row_units;
         break;
       }
       before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (deal.whole) {
+      first = begin;
+      lo = (from - begin) * deal.size;
+      begin = 0;
+      hi = min(chunks_of(seq0), lo + deal.size);
+    } else {
+      per = deal.size;
+      lo = from;
+      hi = min(deal.total, lo + per);
     }
   }
 
@@ -423,6 +491,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
   locate();
   for (int j = 0; j < kQ4Stages; ++j)
     if (at < hi) issue();
+  if (!p.by_row) zero_rows();
 
   // Scores.  With groups of 64 or 128 dims they are formed in integers: a byte of
   // codes is n_even + 16 n_odd, so with integers A = q_odd S / 16 and
@@ -801,7 +870,13 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
 
     // The row after this one, and its query.
     const bool whole = s0 == begin && s1 == begin + n;
-    const int row_b = b, row_r = r, row_begin = begin, row_end = begin + n;
+    const int row_b = b, row_r = r;
+    bool late = false;
+    if (per > 0) {
+      first = begin / per;
+      pieces = (begin + n - 1) / per - first + 1;
+      late = first * per < begin;
+    }
     if (s1 < hi) {
       begin = s1;
       if (++r == R) {
@@ -814,7 +889,8 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       fetch_query(b, r);
     }
 
-    // Add up the warps: statistics first, then each warp its share in turn.
+    // Add up the warps: statistics first, then each warp's share (zero from a warp
+    // that had no chunk).
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
 #pragma unroll
@@ -834,21 +910,11 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       even[e] = ex2(m[e] - gm[e]) * 0x1p24f;
       odd[e] = ex2(m[e] - gm[e]) * 0x1p20f;
     }
-    const int live = min(W, s1 - s0);  // warps that had a chunk of this segment
-    for (int turn = 0; turn < live; ++turn) {
-      if ((s0 - lo + turn) % W == warp) {  // chunk s0 + turn is this warp's
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          float4 v = turn == 0 ? nothing : sm_o[t * 32 + lane];
-          v.x = fmaf(o[t][0], even[0], v.x);
-          v.y = fmaf(o[t][1], even[1], v.y);
-          v.z = fmaf(o[t][2] - o[t][0], odd[0], v.z);
-          v.w = fmaf(o[t][3] - o[t][1], odd[1], v.w);
-          sm_o[t * 32 + lane] = v;
-        }
-      }
-      __syncthreads();
-    }
+    for (int t = 0; t < 8; ++t)
+      sm_o[warp * kQ4Frags + t * 32 + lane] = make_float4(o[t][0] * even[0], o[t][1] * even[1], (o[t][2] - o[t][0]) * odd[0],
+                                                          (o[t][3] - o[t][1]) * odd[1]);
+    __syncthreads();
     float den[2] = {0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < 2; ++e)
@@ -857,11 +923,18 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
         den[e] = fmaf(sm_l[w * kQ4Heads + 2 * cq + e], ex2(sm_m[w * kQ4Heads + 2 * cq + e] - gm[e]), den[e]);
     // The output, or a piece of it; a thread's float4s are all of heads 2 cq and + 1.
     const long long slot = 2ll * blockIdx.x + (s0 == lo ? 0 : 1);
+#pragma unroll
     for (int k = threadIdx.x; k < kQ4Frags; k += kQ4Threads) {
+      float4 v = sm_o[k];
+#pragma unroll
+      for (int w = 1; w < W; ++w) {
+        const float4 u = sm_o[w * kQ4Frags + k];
+        v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+      }
       if (whole)
-        store_frag<T, NG>(p, row_b, h0, nh, k, sm_o[k], den[0], den[1]);
+        store_frag<T, NG>(p, row_b, h0, nh, k, v, den[0], den[1]);
       else
-        __stcg(reinterpret_cast<float4 *>(p.scratch) + slot * kQ4Frags + k, sm_o[k]);
+        __stcg(reinterpret_cast<float4 *>(p.scratch) + slot * kQ4Frags + k, v);
     }
     if (!whole && threadIdx.x < 4)
       __stcg(reinterpret_cast<float4 *>(p.scratch) + 2ll * p.ctas * kQ4Frags + slot * (kQ4Heads / 2) + cq,
@@ -873,13 +946,13 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       __syncthreads();
       if (threadIdx.x == 0) {
         int32_t *counter = p.counters + (long long)row_b * R + row_r;
-        *last = atomicAdd(counter, 1) == (row_end - 1) / per - row_begin / per;
+        *last = atomicAdd(counter, 1) == pieces - 1;
         if (*last) *counter = 0;
       }
       __syncthreads();
       if (*last) {
         __threadfence();
-        merge_row<T, NG>(p, row_b, h0, nh, row_begin, row_end, per);
+        merge_row<T, NG>(p, row_b, h0, nh, first, pieces, late);
       }
     }
     __syncthreads();  // statistics and outputs are free again
@@ -898,22 +971,26 @@ __global__ void __launch_bounds__(kQ4Threads) attn_q4_merge_kernel(const __grid_
   pdl_enter(p.pdl);
   const int R = p.c.kv_heads * p.head_blocks;
   const int b = blockIdx.x / R, r = blockIdx.x - b * R;
-  const int n = chunks_of(seq_of(p, b));
-  int before = 0, total = 0, longest = 0;
-  for (int i = lane_id(); i < p.c.rows; i += 32) {
-    const int v = chunks_of(seq_of(p, i));
-    total += v;
-    before += i < b ? v : 0;
-    longest = max(longest, v);
+  const Q4Deal deal = q4_deal(p, lane_id() < p.c.rows ? chunks_of(seq_of(p, lane_id())) : 0);
+  auto units = [&](int i) {
+    const int n = chunks_of(seq_of(p, i));
+    return deal.whole ? pieces_of(n, deal.size, rcp_of(deal.size)) : n;
+  };
+  int first = 0;
+  for (int i = lane_id(); i < b; i += 32) first += units(i);
+  int pieces = units(b);
+  first = __reduce_add_sync(0xffffffffu, first) * R + r * pieces;
+  bool late = false;
+  if (!deal.whole && pieces > 0) {
+    const int begin = first;
+    first = begin / deal.size;
+    pieces = (begin + pieces - 1) / deal.size - first + 1;
+    late = first * deal.size < begin;
   }
-  total = __reduce_add_sync(0xffffffffu, total);
-  before = __reduce_add_sync(0xffffffffu, before);
-  longest = __reduce_max_sync(0xffffffffu, longest);
-  const int per = Q4Deal(p, total * R, longest).size, begin = before * R + r * n;
-  if (n == 0 || per == 0 || begin / per == (begin + n - 1) / per) return;  // written already
+  if (pieces < 2) return;  // written already
   const int hb = r % p.head_blocks;
   merge_row<T, NG>(p, b, r / p.head_blocks * p.group + hb * p.block_heads, min(p.block_heads, p.group - hb * p.block_heads),
-                   begin, begin + n, per);
+                   first, pieces, late);
 }
 
 template <typename T, int NG, int P>
@@ -961,7 +1038,7 @@ Q4Plan q4_plan(const dak_kv4_cache *c, int num_q_heads, int max_seq_len) {
   const int resident = device_sms() * kQ4PerSm;
   plan.by_row = plan.rows <= resident && chunks <= kQ4RowChunks;
   plan.ctas = plan.by_row ? (int)plan.rows
-                          : (int)std::min<long long>(resident, (plan.rows * chunks + kQ4Warps - 1) / kQ4Warps);
+                          : (int)std::min<long long>(resident, plan.rows * ((chunks + kQ4Warps - 1) / kQ4Warps));
   plan.scratch_floats = plan.by_row ? 0 : 2ll * plan.ctas * kQ4Heads * (kKv4Dim + 2);
   return plan;
 }

@@ -437,6 +437,35 @@ def test_attend_many_rows_and_dealt_ranges():
         assert cnt is None or not cnt.any()
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,longest", [(3, 2, 1, 30000), (31, 4, 2, 4000), (32, 8, 1, 6000), (33, 4, 1, 9000),
+                                              (70, 3, 3, 1500), (97, 2, 1, 4000), (128, 1, 1, 3000), (129, 16, 1, 2000),
+                                              (260, 2, 2, 700), (297, 1, 1, 900)])
+@pytest.mark.parametrize("even", [False, True])
+def test_attend_batches_of_every_deal(B, Hq, Hkv, longest, even):
+    """Lengths over the logarithm, some zero, or nearly even: pieces of rows, rows and
+    ranges, the lengths in one to many blocks of 32, both ways to merge alike."""
+    kv4 = _kv4()
+    g = torch.Generator().manual_seed(B + longest)
+    u = torch.rand(B, generator=g, dtype=torch.float64)
+    lens = (longest - 60 * u if even else torch.exp(u * math.log(longest))).long()
+    lens[2::5] = longest if even else 0
+    lens[B // 2] = longest
+    table = torch.randint(0, 61, (B, -(-longest // 64)), generator=g)  # shared pages
+    pool = random_pool(61, Hkv, 64, 128, B)
+    q = torch.randn(B, Hq, D, generator=g).to(torch.bfloat16)
+    cnt = torch.zeros(kv4.merge_counter_count(B, Hq, Hkv), dtype=torch.int32, device="cuda")
+    one, two = (kv4.decode_paged_q4(q.cuda(), pool.cuda(), None, table.int().cuda(), lens.int().cuda(), 0.088,
+                                    scratch=torch.full((kv4.scratch_floats(B, Hq, Hkv, 64, 128, 64 * table.shape[1]),),
+                                                       float("nan"), device="cuda"), merge_counters=c) for c in (cnt, None))
+    assert torch.equal(one, two) and not cnt.any()
+    some = torch.cat([torch.arange(min(B, 6)), torch.randint(0, B, (12,), generator=g), torch.tensor([B // 2, B - 1])])
+    ref = attend64(q[some], (pool, None), 64, 128, table[some], lens[some], 0.088)
+    k_abs, v_range = values(*parts(pool, 64, 128)[:2]).abs().amax(), 15 * parts(pool, 64, 128)[3][..., 0].double().amax()
+    assert ((one[some.cuda()].cpu().double() - ref).abs() <= _bound(ref, q, k_abs, v_range, 0.088, torch.bfloat16)).all()
+    zero = (lens == 0).nonzero().flatten().cuda()
+    assert not one[zero].any() and torch.isfinite(one).all()
+
+
 # ---------------------------------------------------------------- together
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_prompt_then_steps_in_a_graph_on_another_stream(dtype):
