@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
     } else {
       per = deal.size;
       lo = from;
-      hi = min(deal.total, lo + per);
+      hi = lo + min(per, deal.total - lo);
     }
   }
 
@@ -1057,6 +1057,7 @@ extern "C" int dak_attn_decode_paged_q4(const dak_kv4_cache *cache, const dak_at
     return fail(DAK_ERR_INVALID_ARG, "num_q_heads must be a positive multiple of kv_heads");
   if (a->max_seq_len <= 0 || (int64_t)cache->max_pages * cache->page_size < a->max_seq_len)
     return fail(DAK_ERR_INVALID_ARG, "max_seq_len must be positive and within the block table's pages");
+  if (a->max_seq_len > 0x7fffffff - kQ4Chunk) return fail(DAK_ERR_UNSUPPORTED, "max_seq_len is too large for one launch");
   if (!a->query || !a->out || !a->seq_lens) return fail(DAK_ERR_INVALID_ARG, "query, out and seq_lens are required");
   if (a->q_stride_b % 8 || a->q_stride_h % 8 || a->o_stride_b % 8 || a->o_stride_h % 8 ||
       ((reinterpret_cast<uintptr_t>(a->query) | reinterpret_cast<uintptr_t>(a->out) |

@@ -35,6 +35,7 @@ from .trace import traced
 PAGE_SIZES = (16, 32, 64)
 GROUPS = (32, 64, 128)
 MAX_BLOCK_HEADS = 8  # query heads that one CTA of the attention serves
+MAX_SEQ_LEN = 2**31 - 65  # int32 positions, whole chunks
 SHORT_ROWS = 512     # tokens up to which the attention does not split a row
 
 
@@ -229,8 +230,8 @@ def decode_paged_q4(query: torch.Tensor, pool_dev: torch.Tensor | None, pool_hos
     if Hq % c.kv_heads:
         raise RuntimeError("the KV heads must divide the query heads")
     if max_seq_len is None:
-        max_seq_len = c.max_pages * c.page_size
-    elif not 0 < max_seq_len <= c.max_pages * c.page_size:
+        max_seq_len = min(c.max_pages * c.page_size, MAX_SEQ_LEN)
+    elif not 0 < max_seq_len <= min(c.max_pages * c.page_size, MAX_SEQ_LEN):
         raise RuntimeError("max_seq_len must be positive and within the block table's pages")
     if out is None:
         out = torch.empty_like(query, memory_format=torch.contiguous_format)

@@ -87,6 +87,14 @@ def test_attention_refusals(bad, status, msg):
     assert st == status and msg in text, text
 
 
+def test_attention_refuses_lengths_near_2_to_31():
+    c = _cache()
+    c.max_pages = c.table_stride = 2**27
+    a = _lib.AttnQ4Args(BUF, 512, 128, BUF, BUF, 512, 128, BUF, 1 << 40, None, 4, 2**31 - 1, 0.1, _lib.DTYPE_F16)
+    st, text = _status(_lib.LIB.dak_attn_decode_paged_q4, ctypes.byref(c), ctypes.byref(a), None)
+    assert st == _lib.DAK_ERR_UNSUPPORTED and "max_seq_len" in text, text
+
+
 def test_attention_scratch():
     """None for short rows that fit the GPU at once, else two slots of 8 heads for
     every CTA; a call with less is refused."""
