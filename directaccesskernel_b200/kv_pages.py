@@ -29,10 +29,12 @@ def _entries(t, name: str) -> torch.Tensor:
         except (TypeError, OverflowError) as e:
             raise RuntimeError(f"{name} must be a list or a 1-D CPU tensor of page entries ({e})") from None
         return torch.frombuffer(t, dtype=torch.int32) if t else torch.empty(0, dtype=torch.int32)
-    if t.is_cuda or t.dim() != 1 or t.is_floating_point() or t.is_complex():
+    if t.is_cuda or t.dim() != 1:
         raise RuntimeError(f"{name} must be a list or a 1-D CPU tensor of page entries")
     if t.dtype == torch.int32:
-        return t.contiguous()
+        return t if t.is_contiguous() else t.contiguous()
+    if t.is_floating_point() or t.is_complex():
+        raise RuntimeError(f"{name} must be a list or a 1-D CPU tensor of page entries, whole numbers")
     if t.numel() and (int(t.max()) > 2**31 - 1 or int(t.min()) < -2**31):
         raise RuntimeError(f"{name} does not fit int32")
     return t.to(torch.int32).contiguous()
@@ -68,14 +70,17 @@ def copy_pages(pool_dev: torch.Tensor | None, pool_host: torch.Tensor | None, sr
     n = src.numel()
     if dst.numel() != n:
         raise RuntimeError("src and dst must have the same length")
-    slabs, page = math.prod(shape[:page_dim]), math.prod(shape[page_dim + 1:]) * pool.element_size()
+    slabs = math.prod(shape[:page_dim]) if page_dim else 1
+    page = math.prod(shape[page_dim + 1:]) * pool.element_size()
     if n == 0 or slabs == 0 or page == 0:
         return
     nd = pool_dev.shape[page_dim] if pool_dev is not None else 0
     nh = pool_host.shape[page_dim] if pool_host is not None else 0
-    to = (pool_dev.data_ptr() if nd else None, nd, pool_host.data_ptr() if nh else None, nh, page, slabs, nd * page, nh * page)
+    dev = pool_dev.data_ptr() if nd else None
+    host = pool_host.data_ptr() if nh else None
     if n <= MAX_MOVES:
-        check(LIB.dak_copy_pages(*to, src.data_ptr(), dst.data_ptr(), n, stream_of(device)), "copy_pages")
+        check(LIB.dak_copy_pages(dev, nd, host, nh, page, slabs, nd * page, nh * page, src.data_ptr(), dst.data_ptr(), n,
+                                 stream_of(device)), "copy_pages")
         return
     # Several launches: what one launch refuses is refused over all of them, before the first.
     d = dst.sort().values
@@ -88,7 +93,8 @@ def copy_pages(pool_dev: torch.Tensor | None, pool_host: torch.Tensor | None, sr
         raise RuntimeError("copy_pages: an entry is outside its pool")
     for i in range(0, n, MAX_MOVES):
         s, d = src[i:i + MAX_MOVES], dst[i:i + MAX_MOVES]
-        check(LIB.dak_copy_pages(*to, s.data_ptr(), d.data_ptr(), s.numel(), stream_of(device)), "copy_pages")
+        check(LIB.dak_copy_pages(dev, nd, host, nh, page, slabs, nd * page, nh * page, s.data_ptr(), d.data_ptr(), s.numel(),
+                                 stream_of(device)), "copy_pages")
 
 
 class PageTable:

@@ -172,6 +172,29 @@ def test_rotary_refusals():
         rotary(torch.zeros(2, 2, 128, dtype=torch.float16), torch.zeros(2, dtype=torch.int32), torch.zeros(64))
 
 
+@pytest.mark.parametrize("n", [2, 9, 120, 1000, MAX_MOVES])
+@pytest.mark.parametrize("stride", [1, 16, 4096])
+def test_copy_finds_hazards_in_long_lists(n, stride):
+    g = torch.Generator().manual_seed(n)
+    ids = (torch.randperm(2 * n, generator=g) * stride).to(torch.int32)
+    ids[::3] = -1 - ids[::3]  # some on the host
+
+    def message(src, dst):
+        return _status(_lib.LIB.dak_copy_pages, BUF, 2 * n * stride, BUF, 2 * n * stride, 64, 1, 0, 0, src.data_ptr(),
+                       dst.data_ptr(), n, None)[1]
+
+    src, dst = ids[:n].clone(), ids[n:].clone()
+    assert not any(w in message(src, dst) for w in ("twice", "both", "outside"))
+    assert not any(w in message(src[:1].repeat(n), dst) for w in ("twice", "both", "outside"))  # one page to many
+    for i, j in ((0, n - 1), (n // 2, 0)):
+        two = dst.clone()
+        two[i] = two[j]
+        assert f"page {int(dst[j])} is a destination twice" in message(src, two)
+        two = src.clone()
+        two[i] = dst[j]
+        assert f"page {int(dst[j])} is both" in message(two, dst)
+
+
 def test_copy_refusals():
     def call(src, dst, dev=4, host=4, page=64, slabs=1, strides=(256, 256), pool=BUF, n=None):
         s, d = torch.tensor(src, dtype=torch.int32), torch.tensor(dst, dtype=torch.int32)
