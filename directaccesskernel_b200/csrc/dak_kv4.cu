@@ -15,17 +15,19 @@
 // tokens, whose code rows are neighbours in the page.  The append's CTA takes
 // four tokens and up to 48 heads of each: four bulk copies bring them into shared
 // memory, all in flight at once, while the threads work out the tokens' angles,
-// one each, and look up their pages.  With few heads it takes 8 or 16 tokens, each
-// four with its share of the warps: the start-up is the larger part of a small CTA.
+// one each; their pages are looked up behind the angles and the q heads.  With few
+// heads it takes 8 or 16 tokens, each four with its share of the warps: the start-up
+// is the larger part of a small CTA.
 //
 // The instructions count nearly as much as the bytes (249 per head of four tokens,
 // 0.6 of the issue slots, before a q head's angles were kept in registers).  Append
-// of 16384 tokens, 32 + 16 heads in bfloat16, groups of 32 (358 MB): 64 us, 5.6 TB/s,
-// 0.87 of the measured copy rate (75 us); of 4099 tokens 21 us; of 65536 tokens, 8 + 2
-// heads 65 us (109 us with four tokens per CTA); of 32 tokens 3.4 us.  CTAs that
-// walk over tiles of 8 heads with four in flight took a quarter longer (97 us): they
-// wait at each four tokens for positions and pages.  Five or six CTAs per SM with
-// fewer registers, or fewer heads per CTA, took 10 to 30% longer.
+// of 16384 tokens, 32 + 16 heads in bfloat16, groups of 32 (358 MB): 59 us, 6.1 TB/s,
+// 0.94 of the measured copy rate (75 us before that, 64 us with the pages looked up
+// first); of 4099 tokens 20 us; of 65536 tokens, 8 + 2 heads 58 us (109 us with four
+// tokens per CTA); of 32 tokens 3.4 us.  CTAs that walk over tiles of 8 heads with
+// four in flight took a quarter longer (97 us): they wait at each four tokens for
+// positions and pages.  Five or six CTAs per SM with fewer registers, or fewer heads
+// per CTA, took 10 to 30% longer.
 //
 // Read-back of 65536 tokens x 8 heads, groups of 128 (340 MB): 58 us, 5.9 TB/s, 0.91
 // (63 us with four rows in flight per thread and four CTAs per SM, 75 with one row);
@@ -202,34 +204,30 @@ __global__ void __launch_bounds__(kKv4Threads, 4) kv4_append_kernel(const __grid
     for (int i = 0; i < nt; ++i)
       bulk_load(smem_u32(rows_s) + i * token_bytes, p.qkv + (long long)(t0 + i) * p.ld + h0 * kKv4Dim, token_bytes, bar_a, pol);
   }
+  // The page look-up (position, then table entry) runs behind the angles and the q
+  // heads; its result is wanted for k and v.
+  bool in = false;
+  int entry = 0;
   if (threadIdx.x < nt) {
-    const int pos = p.positions[t0 + threadIdx.x];
-    int tier = 0;
-    uint8_t *page = pos < 0 ? nullptr
-                            : kv4_page(p.c, p.seq_index ? p.seq_index[t0 + threadIdx.x] : t0 + (int)threadIdx.x,
-                                       pos >> p.c.page_log2, &tier);
-    if (!page) atomicCAS(p.c.status, 0, DAK_ERR_INVALID_ARG);
-    sm.page[threadIdx.x] = page;
-    sm.tier[threadIdx.x] = tier;
+    const int seq = p.seq_index ? p.seq_index[t0 + threadIdx.x] : t0 + (int)threadIdx.x;
+    const int page = p.positions[t0 + threadIdx.x] >> p.c.page_log2;
+    in = kv4_in_table(p.c, seq, page);
+    if (in) entry = p.c.table[(long long)seq * p.c.table_stride + page];
   }
   rope_table(tab, p.positions + t0, nt, ct, p.inv_freq, p.rotary_dim, p.scale);
   __syncthreads();
   const float *cos_row = tab + (live ? sub : 0) * stride, *sin_row = cos_row + ct * stride;
   const int slot = p.positions[t] & (P - 1);
-  uint8_t *page = live ? sm.page[sub] : nullptr;
   const int half = kv4_half_bytes(P, NG);
   const int R = p.rotary_dim, part = R / 16;  // vectors between the partners of the half layout
   const uint8_t *row = rows_s + (live ? sub : 0) * token_bytes;
-  if (!mbar_wait<false>(bar_a, 0, wc)) {  // gave up: let the copies land (bounded again), then leave
-    mbar_wait<false>(bar_a, 0, WaitCtx{&sm.abort_flag[1], p.c.status});
-    return;
-  }
+  const bool ok = mbar_wait<false>(bar_a, 0, wc);
 
   // q: a unit at a time, its angles in registers for all of the warp's heads.
   constexpr int row_vecs = kKv4Dim / 8;
   const uint4 *vecs = reinterpret_cast<const uint4 *>(row);
   int h = h0 + warp_id() % warps;
-  const int q_end = min(h_end, p.q_heads), k_end = min(h_end, p.q_heads + Hkv);
+  const int q_end = ok ? min(h_end, p.q_heads) : h, k_end = min(h_end, p.q_heads + Hkv);
   for (int u = live ? lane8 : p.units; u < p.units; u += 8) {
     const RopeUnit unit = rope_unit(u, R, p.interleaved);
     float c[8], s[8];
@@ -244,6 +242,19 @@ __global__ void __launch_bounds__(kKv4Threads, 4) kv4_append_kernel(const __grid
   }
   if (h < q_end) h += (q_end - h + warps - 1) / warps * warps;
   // k and v: 16 dims a lane.
+  if (threadIdx.x < nt) {
+    int tier = 0;
+    uint8_t *page = in ? kv4_page_of(p.c, entry, &tier) : nullptr;
+    if (!page) atomicCAS(p.c.status, 0, DAK_ERR_INVALID_ARG);
+    sm.page[threadIdx.x] = page;
+    sm.tier[threadIdx.x] = tier;
+  }
+  __syncthreads();
+  if (!ok) {  // gave up: let the copies land (bounded again), then leave
+    mbar_wait<false>(bar_a, 0, WaitCtx{&sm.abort_flag[1], p.c.status});
+    return;
+  }
+  uint8_t *page = live ? sm.page[sub] : nullptr;
   uint8_t *codes = page ? page + slot * 64 : nullptr, *pairs = page ? page + P * 64 + slot * 4 * NG : nullptr;
   auto store = [&](const float(&x)[16], long long at) {
     kv4_quantise<NG>(x, lane8, page ? codes + at : nullptr, pairs + at);
@@ -445,7 +456,7 @@ extern "C" int dak_rope_kv_append_q4(const dak_kv4_cache *cache, const dak_kv4_a
   p.slice = (int)(slices == 1 ? heads : ((heads + slices - 1) / slices + kKv4Warps - 1) / kKv4Warps * kKv4Warps);
   // Few heads of many tokens: more tokens per CTA, each of which starts up once, as
   // far as the shared memory of 48 heads goes and half the GPU still gets a CTA.  8 + 2
-  // heads of 2500 tokens: 5.7 us, 7.3 without; of 65536: 65 and 109.
+  // heads of 2500 tokens: 5.8 us, 7.3 without; of 65536: 58 and 109.
   p.groups = 1;
   while (4 * p.groups < kAppendTokens && 2 * p.groups * p.slice <= kAppendHeads && heads <= p.slice &&
          quads >= p.groups * kAppendFull)

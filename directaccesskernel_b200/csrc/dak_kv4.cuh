@@ -30,16 +30,23 @@ struct Kv4Cache {
 
 __host__ __device__ constexpr int kv4_half_bytes(int page_size, int ng) { return page_size * (64 + 4 * ng); }
 
-// First byte of page `page` of sequence `seq` (head 0), or nullptr for an entry
-// outside the table or the pools; *tier becomes 0 (device) or 1 (host).
-__device__ __forceinline__ uint8_t *kv4_page(const Kv4Cache &c, int seq, int page, int *tier) {
-  if (seq < 0 || seq >= c.rows || page < 0 || page >= c.max_pages) return nullptr;
-  const int entry = c.table[(long long)seq * c.table_stride + page];
+__device__ __forceinline__ bool kv4_in_table(const Kv4Cache &c, int seq, int page) {
+  return seq >= 0 && seq < c.rows && page >= 0 && page < c.max_pages;
+}
+
+// First byte (head 0) of the page that an entry names, or nullptr for an entry
+// outside its pool; *tier becomes 0 (device) or 1 (host).
+__device__ __forceinline__ uint8_t *kv4_page_of(const Kv4Cache &c, int entry, int *tier) {
   const int t = entry < 0 ? 1 : 0;
   const long long idx = entry < 0 ? -1ll - entry : entry;
   if (idx >= c.pages[t]) return nullptr;
   *tier = t;
   return c.pool[t] + idx * c.page_bytes;
+}
+
+// The same for page `page` of sequence `seq`, nullptr outside the table too.
+__device__ __forceinline__ uint8_t *kv4_page(const Kv4Cache &c, int seq, int page, int *tier) {
+  return kv4_in_table(c, seq, page) ? kv4_page_of(c, c.table[(long long)seq * c.table_stride + page], tier) : nullptr;
 }
 
 }  // namespace dak
