@@ -21,17 +21,21 @@
 // MMAs as they are (see "Scores" below); V's enter as float16 subnormals, its even
 // codes and its whole bytes (even + 16 odd, units of 2^-24), which a mask or a byte
 // permutation each give; the odd dims are the difference, at the end (masks and
-// shifts for each nibble took 1 to 3% longer).  P is float16: for bfloat16
-// outputs in one term (2^-11 relative, an eighth of the output's own rounding),
-// for float16 outputs in two, because one made the output up to 1.9 times less
-// exact than its rounding and two do not show.
+// shifts for each nibble took 1 to 3% longer).  P is float16, in units of each
+// chunk's largest products (see "Statistics" below): for bfloat16 outputs in one
+// term (2^-11 relative, an eighth of the output's own rounding), for float16
+// outputs in two, because one made the output up to 1.9 times less exact than its
+// rounding and two do not show.  One unit for all chunks and groups, from the
+// largest score and the largest scale, was 1.5% (groups of 32: 7%) faster and lost
+// V's codes where large scales had small weights.
 //
 // Bound, at 32 x 16384 tokens of 8 KV heads (570 MB, 89 us at the measured copy
-// rate): 108 us in bfloat16, 116 us in float16.  The copies alone take 91 us; the
-// rest is arithmetic that two warps per scheduler do not quite hide (4.3 cycles
-// per instruction and warp, about 800 instructions per chunk).  Plain bulk
-// copies replaced tensor copies with a 64-byte swizzle: bank conflicts cost less
-// than the 64-byte rows did, and host pages come 15% faster (46 GB/s).
+// rate), in a graph of calls: 110 us in bfloat16, 119 us in float16.  The copies
+// alone take 91 us; the rest is arithmetic that two warps per scheduler do not
+// quite hide (4.3 cycles per instruction and warp, about 800 instructions per
+// chunk).  Plain bulk copies replaced tensor copies with a 64-byte swizzle: bank
+// conflicts cost less than the 64-byte rows did, and host pages come 15% faster
+// (46 GB/s).
 #include <cfloat>
 #include <cstring>
 #include <type_traits>
@@ -150,12 +154,30 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
   return d;
 }
 
-// floor(log2 s) of a float16 s >= 0 given by its bits; -24 (its smallest
-// exponent) for 0.
-__device__ __forceinline__ float exponent_of(uint32_t bits) {
-  const float s = __half2float(__ushort_as_half((unsigned short)bits));
-  return fmaxf((float)((int)(__float_as_uint(s) >> 23) - 127), -24.f);
+// Two FP32 products, or products and sums, in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 a, b, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mul.rn.f32x2 d, a, b; mov.b64 {%0, %1}, d;}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{.reg .b64 a, b, c, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mov.b64 c, {%6, %7}; fma.rn.f32x2 d, a, b, c; "
+      "mov.b64 {%0, %1}, d;}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// The FP32 number whose upper half is in the lower (e = 0) or upper half of w.
+__device__ __forceinline__ float ref_of(uint32_t w, int e) { return __uint_as_float(e ? w & 0xFFFF0000u : w << 16); }
 
 // Outputs are added up and kept in scratch in the MMA's own layout, 256 float4 of
 // a row: number i holds, for c = i % 4, g = i / 4 % 8 and t = i / 32, dims d, d + 1
@@ -587,11 +609,17 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
   const uint32_t sel_lo = flip ? 0x1054u : 0x5410u, sel_hi = flip ? 0x3276u : 0x7632u;
   const uint32_t sel_g = (g & 1) ? sel_hi : sel_lo;
 
-  // Statistics: weights are 2^(score - m).  m is the largest score so far plus E,
-  // the exponent of the warp's largest V scale so far, so that weight x scale is
-  // below 2 and float16 holds it whatever V's magnitude.
-  float o[8][4], m[2], l[2], E;
-  uint32_t s_max;
+  // Statistics: weights are 2^(score - m), m being the largest score so far.  What
+  // float16 has to hold is weight x scale, and the largest product need not be that
+  // of the largest score or of the largest scale, so P and O have a unit of their
+  // own, per head and group (ref: two heads' FP32 powers of two, upper halves): each
+  // chunk takes the exponent of its largest product (several groups: of the largest
+  // sum over a lane's 8 tokens, one instruction less), so that products are below 2
+  // and those above 2^-14 keep all of their bits.  The unit falls as well as rises,
+  // and O with it, exactly; it stays at 2^-90 or above so that FP32 holds O.
+  constexpr uint32_t kRefMin = (127 - 90) << 7 | (127 - 90) << 23;
+  float o[8][4], m[2], l[2];
+  uint32_t ref[NG];
 
   // One chunk of `valid` tokens in the stage at `st`.
   auto chunk = [&](const uint8_t *st, int valid, auto full_c) {
@@ -603,21 +631,17 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
     };
     float y[4][4];  // raw scores: tile, {token g, g + 8} x {head 2 cq, 2 cq + 1}
     float mx[2] = {-INFINITY, -INFINITY};
-    // V's (scale, zero) words of tile t, token g + 8r.  With one group they stay in
-    // registers; more of them are read again where they are needed, which costs
-    // less than the registers would.
-    uint32_t vp[4][2][NG];
-    auto load_vp = [&](int t, int r, bool again) {
-      if (again && NG == 1) return;
-      load_pairs<NG>(st + half + pairs_at(t, r), vp[t][r]);
+    // V's (scale, zero) words of token g + 8r of tile t.  Several groups' are read
+    // again where they are needed, which costs less than the registers would.
+    auto load_vp = [&](int t, int r, uint32_t(&vp)[NG]) {
+      load_pairs<NG>(st + half + pairs_at(t, r), vp);
 #pragma unroll
       for (int n = 0; n < NG; ++n)
-        if (!kFull && t * 16 + 8 * r + g >= valid) vp[t][r][n] = 0u;  // anything may lie behind the last token
+        if (!kFull && t * 16 + 8 * r + g >= valid) vp[n] = 0u;  // anything may lie behind the last token
     };
     auto forget = [] {
       if (NG > 1) asm volatile("" ::: "memory");
     };
-    __half2 vmax = __float2half2_rn(0.f);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       if (!kFull && t * 16 >= valid) continue;
@@ -646,12 +670,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       }
       uint32_t kp[2][NG];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        load_pairs<NG>(st + pairs_at(t, r), kp[r]);
-        load_vp(t, r, false);
-#pragma unroll
-        for (int n = 0; n < NG; ++n) vmax = __hmax2(vmax, *reinterpret_cast<const __half2 *>(&vp[t][r][n]));
-      }
+      for (int r = 0; r < 2; ++r) load_pairs<NG>(st + pairs_at(t, r), kp[r]);
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         float acc[4];
@@ -705,67 +724,89 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
         }
       }
     }
-    // A larger V scale than any before raises E (rarely, after the first chunks).
-    const uint32_t sm = __reduce_max_sync(0xffffffffu, *reinterpret_cast<const uint32_t *>(&vmax) & 0xffffu);
-    float rise = 0.f;
-    if (sm > s_max) {
-      s_max = sm;
-      const float en = fmaxf(E, exponent_of(sm));
-      rise = en - E;
-      E = en;
-    }
-    float alpha[2], zs[2][NG];
+    float alpha[2];
+    float2 zs[2][NG], top[2][NG];  // of the tokens g and g + 8 of all tiles
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
 #pragma unroll
       for (int x = 4; x <= 16; x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
-      const float mn = fmaxf(m[e] + rise, fmaf(mx[e], f[e], E));
+      const float mn = fmaxf(m[e], mx[e] * f[e]);
       alpha[e] = ex2(m[e] - mn);
       m[e] = mn;
       l[e] *= alpha[e];
 #pragma unroll
-      for (int n = 0; n < NG; ++n) zs[e][n] = 0.f;
+      for (int n = 0; n < NG; ++n) zs[e][n] = top[e][n] = make_float2(0.f, 0.f);
     }
-    // Weights, and the zeros' share of the output: sum_t p_t zero_t per group.
+    // Weights, the zeros' share of the output, sum_t p_t zero_t per group, and the
+    // largest product.  One group's products take the weights' place.
     forget();
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       if (!kFull && t * 16 >= valid) continue;
+      uint32_t vp[2][NG];
+      load_vp(t, 0, vp[0]);
+      load_vp(t, 1, vp[1]);
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        load_vp(t, r, true);
+      for (int e = 0; e < 2; ++e) {
+        float w[2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float w = ex2(fmaf(y[t][2 * r + e], f[e], -m[e]));
-          if (!kFull && t * 16 + 8 * r + g >= valid) w = 0.f;
-          y[t][2 * r + e] = w;
-          l[e] += w;
-#pragma unroll
-          for (int n = 0; n < NG; ++n) zs[e][n] = fmaf(w, half2_of(vp[t][r][n]).y, zs[e][n]);
+        for (int r = 0; r < 2; ++r) {
+          w[r] = ex2(fmaf(y[t][2 * r + e], f[e], -m[e]));
+          if (!kFull && t * 16 + 8 * r + g >= valid) w[r] = 0.f;
+          l[e] += w[r];
         }
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          const float2 v0 = half2_of(vp[0][n]), v1 = half2_of(vp[1][n]), ww = make_float2(w[0], w[1]);
+          zs[e][n] = fma2(ww, make_float2(v0.y, v1.y), zs[e][n]);
+          if (NG == 1) {
+            const float2 a = mul2(ww, make_float2(v0.x, v1.x));
+            top[e][n].x = max3(top[e][n].x, a.x, a.y);
+            y[t][e] = a.x, y[t][2 + e] = a.y;
+          } else {
+            top[e][n] = fma2(ww, make_float2(v0.x, v1.x), top[e][n]);
+          }
+        }
+        if (NG > 1) y[t][e] = w[0], y[t][2 + e] = w[1];
       }
     }
     forget();
+    // This chunk's units, and O from the last chunk's to them.
+    float up[2][NG], beta[2][NG];
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+    for (int n = 0; n < NG; ++n) {
+      uint32_t now = __byte_perm(__float_as_uint(top[0][n].x + top[0][n].y), __float_as_uint(top[1][n].x + top[1][n].y), 0x7632u);
 #pragma unroll
-      for (int n = 0; n < NG; ++n)
+      for (int x = 4; x <= 16; x <<= 1) now = max_u16x2(now, __shfl_xor_sync(0xffffffffu, now, x));
+      now = max_u16x2(now & 0x7F807F80u, kRefMin);
 #pragma unroll
-        for (int x = 4; x <= 16; x <<= 1) zs[e][n] += __shfl_xor_sync(0xffffffffu, zs[e][n], x);
-    // O rows: even dims in units of 2^-24, and the sum of an even dim and 16 times the
-    // odd one beside it.  Adding the zeros' share chunk by chunk keeps O centred, so
-    // nothing cancels at the end.
+      for (int e = 0; e < 2; ++e) {
+        up[e][n] = __uint_as_float(0x7F000000u - (e ? now & 0xFFFF0000u : now << 16));
+        beta[e][n] = alpha[e] * (ref_of(ref[n], e) * up[e][n]);
+      }
+      ref[n] = now;
+    }
 #pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
-        const float even = zs[e][n] * 0x1p-24f, odd = zs[e][n] * (17 * 0x1p-24f);
+        zs[e][n].x += zs[e][n].y;
 #pragma unroll
-        for (int t = 8 * n / NG; t < 8 * (n + 1) / NG; ++t) {
-          o[t][e] = fmaf(o[t][e], alpha[e], even);
-          o[t][2 + e] = fmaf(o[t][2 + e], alpha[e], odd);
-        }
+        for (int x = 4; x <= 16; x <<= 1) zs[e][n].x += __shfl_xor_sync(0xffffffffu, zs[e][n].x, x);
       }
+    // O rows: even dims in units of 2^-24, and the sum of an even dim and 16 times the
+    // odd one beside it.  Adding the zeros' share chunk by chunk keeps O centred, so
+    // nothing cancels at the end.
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      const float2 even = make_float2(zs[0][n].x * up[0][n] * 0x1p-24f, zs[1][n].x * up[1][n] * 0x1p-24f);
+      const float2 odd = make_float2(even.x * 17, even.y * 17), old = make_float2(beta[0][n], beta[1][n]);
+#pragma unroll
+      for (int t = 8 * n / NG; t < 8 * (n + 1) / NG; ++t) {
+        const float2 a = fma2(make_float2(o[t][0], o[t][1]), old, even), c = fma2(make_float2(o[t][2], o[t][3]), old, odd);
+        o[t][0] = a.x, o[t][1] = a.y, o[t][2] = c.x, o[t][3] = c.y;
+      }
+    }
     // O^T += V^T P^T
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -774,11 +815,16 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       [[maybe_unused]] uint32_t bl[NG][2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        load_vp(t, r, true);
+        uint32_t vp[NG];
+        if (NG > 1) load_vp(t, r, vp);
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
-          const float s = half2_of(vp[t][r][n]).x;
-          const float a = y[t][2 * r] * s, c = y[t][2 * r + 1] * s;
+          float a = y[t][2 * r] * up[0][n], c = y[t][2 * r + 1] * up[1][n];
+          if (NG > 1) {
+            const float s = half2_of(vp[n]).x;
+            a *= s;
+            c *= s;
+          }
           const uint32_t hi = pack_half2(a, c);
           bf[n][r] = movmatrix(hi);
           if constexpr (kTwoTerms) {
@@ -848,8 +894,8 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
     m[0] = m[1] = -FLT_MAX;
     l[0] = l[1] = 0.f;
-    E = -24.f;
-    s_max = 0u;
+#pragma unroll
+    for (int x = 0; x < NG; ++x) ref[x] = kRefMin;
     for (; lo + warp + W * done < s1; ++done) {
       const int id = lo + warp + W * done, s = done % kQ4Stages;
       const uint32_t parity = (done / kQ4Stages) & 1;
@@ -901,19 +947,20 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       }
     }
     __syncthreads();
-    float gm[2], even[2], odd[2];  // heads 2 cq, 2 cq + 1
+    float gm[2], share[2];  // heads 2 cq, 2 cq + 1
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       gm[e] = sm_m[2 * cq + e];
 #pragma unroll
       for (int w = 1; w < W; ++w) gm[e] = fmaxf(gm[e], sm_m[w * kQ4Heads + 2 * cq + e]);
-      even[e] = ex2(m[e] - gm[e]) * 0x1p24f;
-      odd[e] = ex2(m[e] - gm[e]) * 0x1p20f;
+      share[e] = ex2(m[e] - gm[e]) * 0x1p24f;
     }
 #pragma unroll
-    for (int t = 0; t < 8; ++t)
-      sm_o[warp * kQ4Frags + t * 32 + lane] = make_float4(o[t][0] * even[0], o[t][1] * even[1], (o[t][2] - o[t][0]) * odd[0],
-                                                          (o[t][3] - o[t][1]) * odd[1]);
+    for (int t = 0; t < 8; ++t) {
+      const float c0 = share[0] * ref_of(ref[t * NG / 8], 0), c1 = share[1] * ref_of(ref[t * NG / 8], 1);
+      sm_o[warp * kQ4Frags + t * 32 + lane] = make_float4(o[t][0] * c0, o[t][1] * c1, (o[t][2] - o[t][0]) * (c0 * 0.0625f),
+                                                          (o[t][3] - o[t][1]) * (c1 * 0.0625f));
+    }
     __syncthreads();
     float den[2] = {0.f, 0.f};
 #pragma unroll
