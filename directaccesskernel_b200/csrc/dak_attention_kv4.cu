@@ -17,11 +17,12 @@
 //     FP32 scores;
 //   O^T [128 dims x 8 heads] += V^T P^T, with the token's scale multiplied into P
 //     and its zero added to O as sum_t p_t zero_t per chunk.
-// Codes never become floating-point values of their own: K's bytes enter integer
-// MMAs as they are (see "Scores" below); V's enter as float16 subnormals, its even
-// codes and its whole bytes (even + 16 odd, units of 2^-24), which a mask or a byte
-// permutation each give; the odd dims are the difference, at the end (masks and
-// shifts for each nibble took 1 to 3% longer).  P is float16, in units of each
+// Codes never become floating-point values of their own: they enter the MMAs as
+// float16 subnormals, K's one by one, of V the even codes and the whole bytes (even
+// + 16 odd, units of 2^-24), which a mask or a byte permutation each give; V's odd
+// dims are the difference, at the end (masks and shifts for each nibble took 1 to
+// 3% longer; K has no such form, because even - odd / 16 of a query does not fit
+// float16).  P is float16, in units of each
 // chunk's largest products (see "Statistics" below): for bfloat16 outputs in one
 // term (2^-11 relative, an eighth of the output's own rounding), for float16
 // outputs in two, because one made the output up to 1.9 times less exact than its
@@ -30,7 +31,7 @@
 // V's codes where large scales had small weights.
 //
 // Bound, at 32 x 16384 tokens of 8 KV heads (570 MB, 89 us at the measured copy
-// rate), in a graph of calls: 110 us in bfloat16, 119 us in float16.  The copies
+// rate), in a graph of calls: 113 us in bfloat16, 121 us in float16.  The copies
 // alone take 91 us; the rest is arithmetic that two warps per scheduler do not
 // quite hide (4.3 cycles per instruction and warp, about 800 instructions per
 // chunk).  Plain bulk copies replaced tensor copies with a 64-byte swizzle: bank
@@ -126,21 +127,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// D = A (16x32 unsigned bytes, row) * B (32x8 bytes, col; signed or not) + D, or
-// without the sum, int32.
-template <bool kSigned, bool kSum>
-__device__ __forceinline__ void mma_u8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                       uint32_t b1) {
-  const int c0 = kSum ? d[0] : 0, c1 = kSum ? d[1] : 0, c2 = kSum ? d[2] : 0, c3 = kSum ? d[3] : 0;
-  if constexpr (kSigned)
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
-        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
-  else
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
-        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -515,18 +501,11 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
     if (at < hi) issue();
   if (!p.by_row) zero_rows();
 
-  // Scores.  With groups of 64 or 128 dims they are formed in integers: a byte of
-  // codes is n_even + 16 n_odd, so with integers A = q_odd S / 16 and
-  // B = q_even S - A for a power of two S,
-  //   sum q n S = sum A * byte + B * (byte & 15)
-  // and half of the codes need no unpacking.  S takes the largest |q| to 2^18: A
-  // has 16 bits and B 20, as bytes for the MMAs the high one signed and the
-  // others unsigned; what is dropped is below 2^-15 of the largest |q|.  With
-  // groups of 32 dims the integer sums would not fill an MMA: there the codes are
-  // taken out one by one as float16 subnormals and meet q in float16, scaled by a
-  // power of two to below 2^14.
-  constexpr bool kIntegers = NG < 4;
-  uint32_t qa[2][2][2], qb[3][2][2];  // [digit, low first][word pair][word]
+  // Scores.  A query is scaled by a power of two so that its largest value lies
+  // between 2^13 and 2^14; float16 then holds the others exactly down to 2^-24 of it
+  // (a bfloat16 value's bits too).  Products and sums are FP32.  Integer MMAs over
+  // whole bytes, the query in 16 and 20 bits, were 2% faster with one group, no faster
+  // with two, and lost the bits of all other channels where one was far larger.
   uint32_t qf[8][2];
   float qs[2][NG], f[2];  // q summed over each group (for the zeros' share); raw scores to base 2
   auto ready_query = [&]() {
@@ -549,50 +528,26 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     bad += __shfl_xor_sync(0xffffffffu, bad, 1);
     bad += __shfl_xor_sync(0xffffffffu, bad, 2);
-    constexpr int kTop = kIntegers ? 18 : 13;
-    const int k = mx > 0.f ? max(-100, min(100, kTop - ((int)(__float_as_uint(mx) >> 23) - 127))) : 0;
+    const int k = mx > 0.f ? max(-100, min(100, 13 - ((int)(__float_as_uint(mx) >> 23) - 127))) : 0;
     // A negative scaling turns the query over, so that a larger raw score is
     // always a larger score.
     const float up = copysignf(__uint_as_float((uint32_t)(127 + k) << 23), p.scale_log2);
-    if constexpr (kIntegers) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t da[2] = {0u, 0u}, db[3] = {0u, 0u, 0u};
-        int total = 0;
+    for (int w = 0; w < 4; ++w)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int odd = __float2int_rn(x[w][2 * j + 1] * up * 0.0625f), even = __float2int_rn(x[w][2 * j] * up);
-          const int rest = even - odd;
-          total += even + 16 * odd;
-#pragma unroll
-          for (int d = 0; d < 2; ++d) da[d] |= ((uint32_t)odd >> (8 * d) & 255u) << (8 * j);
-#pragma unroll
-          for (int d = 0; d < 3; ++d) db[d] |= ((uint32_t)rest >> (8 * d) & 255u) << (8 * j);
-        }
-#pragma unroll
-        for (int d = 0; d < 2; ++d) qa[d][w >> 1][w & 1] = da[d];
-#pragma unroll
-        for (int d = 0; d < 3; ++d) qb[d][w >> 1][w & 1] = db[d];
-        sum[w * NG / 4] += (float)total;
+      for (int h = 0; h < 2; ++h) {
+        const float a = x[w][2 * h] * up, c = x[w][2 * h + 4] * up;
+        const float d = x[w][2 * h + 1] * up, e = x[w][2 * h + 5] * up;
+        qf[2 * w + h][0] = pack_half2(a, c);
+        qf[2 * w + h][1] = pack_half2(d * 0.0625f, e * 0.0625f);
+        sum[w * NG / 4] += ((a + c) + (d + e)) * 0x1p-24f;
       }
-    } else {
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float a = x[w][2 * h] * up, c = x[w][2 * h + 4] * up;
-          const float d = x[w][2 * h + 1] * up, e = x[w][2 * h + 5] * up;
-          qf[2 * w + h][0] = pack_half2(a, c);
-          qf[2 * w + h][1] = pack_half2(d * 0.0625f, e * 0.0625f);
-          sum[w * NG / 4] += ((a + c) + (d + e)) * 0x1p-24f;
-        }
-    }
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
       sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 1);
       sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 2);
     }
-    const float fh = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 + (kIntegers ? 0 : 24) - k) << 23) + bad;
+    const float fh = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 + 24 - k) << 23) + bad;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {  // lane 4h holds head h
       const int src = 4 * (2 * cq + e);
@@ -673,36 +628,16 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       for (int r = 0; r < 2; ++r) load_pairs<NG>(st + pairs_at(t, r), kp[r]);
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
-        float acc[4];
-        if constexpr (kIntegers) {
-          int c[3][4];  // by digit
-          auto words = [&](int v, auto sum_c) {
-            constexpr bool kSum = decltype(sum_c)::value;
-            const uint32_t a0 = w0[2 * v], a1 = w1[2 * v], a2 = w0[2 * v + 1], a3 = w1[2 * v + 1];
-            const uint32_t l0 = a0 & 0x0F0F0F0Fu, l1 = a1 & 0x0F0F0F0Fu, l2 = a2 & 0x0F0F0F0Fu, l3 = a3 & 0x0F0F0F0Fu;
-            mma_u8<false, kSum>(c[0], a0, a1, a2, a3, qa[0][v][0], qa[0][v][1]);
-            mma_u8<true, kSum>(c[1], a0, a1, a2, a3, qa[1][v][0], qa[1][v][1]);
-            mma_u8<true, kSum>(c[2], l0, l1, l2, l3, qb[2][v][0], qb[2][v][1]);
-            mma_u8<false, true>(c[0], l0, l1, l2, l3, qb[0][v][0], qb[0][v][1]);
-            mma_u8<false, true>(c[1], l0, l1, l2, l3, qb[1][v][0], qb[1][v][1]);
-          };
-          words(n * 2 / NG, std::false_type{});
-          if constexpr (NG == 1) words(1, std::true_type{});
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        // A nibble at bits 0-3 of a half word is the subnormal code * 2^-24, at bits
+        // 4-7 code * 2^-20 (its q is / 16).
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] = (float)(c[2][e] * 65536 + c[1][e] * 256 + c[0][e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] = 0.f;
-          // A nibble at bits 0-3 of a half word is the subnormal code * 2^-24, at bits
-          // 4-7 code * 2^-20 (its q is / 16).
-#pragma unroll
-          for (int w = n * 4 / NG; w < (n + 1) * 4 / NG; ++w) {
-            mma_f16(acc, w0[w] & 0x000F000Fu, w1[w] & 0x000F000Fu, w0[w] & 0x00F000F0u, w1[w] & 0x00F000F0u, qf[2 * w][0],
-                    qf[2 * w][1]);
-            const uint32_t s0 = w0[w] >> 8, s1 = w1[w] >> 8;
-            mma_f16(acc, s0 & 0x000F000Fu, s1 & 0x000F000Fu, s0 & 0x00F000F0u, s1 & 0x00F000F0u, qf[2 * w + 1][0],
-                    qf[2 * w + 1][1]);
-          }
+        for (int w = n * 4 / NG; w < (n + 1) * 4 / NG; ++w) {
+          mma_f16(acc, w0[w] & 0x000F000Fu, w1[w] & 0x000F000Fu, w0[w] & 0x00F000F0u, w1[w] & 0x00F000F0u, qf[2 * w][0],
+                  qf[2 * w][1]);
+          const uint32_t s0 = __byte_perm(w0[w], 0u, 0x4341u), s1 = __byte_perm(w1[w], 0u, 0x4341u);
+          mma_f16(acc, s0 & 0x000F000Fu, s1 & 0x000F000Fu, s0 & 0x00F000F0u, s1 & 0x00F000F0u, qf[2 * w + 1][0],
+                  qf[2 * w + 1][1]);
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {

@@ -124,3 +124,40 @@ def test_attend_mixed_magnitudes(kind, lens, wide, counters, page, group, dtype)
     if kind[0] == "group" and group == D:
         pytest.skip("one group")
     _run(kind, lens, page, group, dtype, 7, wide, counters)
+
+
+def _attend(q, pool, page, lens, scaling):
+    """decode_paged_q4 over rows whose pages lie one after the other, and its table."""
+    from directaccesskernel_b200 import kv4
+
+    n_pages = [-(-n // page) for n in lens]
+    table = torch.zeros(len(lens), max(n_pages), dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(n_pages):
+        table[b, :n] = torch.arange(at, at + n)
+        at += n
+    got = kv4.decode_paged_q4(q.cuda(), pool.cuda(), None, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), scaling)
+    return got.cpu().double(), table
+
+
+@pytest.mark.parametrize("ratio", [200.0, 1000.0, 30000.0])
+@pytest.mark.parametrize("channel", [4, 5])
+@pytest.mark.parametrize("page,group", [(16, 32), (32, 64), (64, 128)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attend_query_with_an_outlier_channel(ratio, channel, page, group, dtype):
+    """One channel of the query is far larger than the rest and meets keys of exactly 0
+    there: the scores are the other channels', whose bits must not be lost to it."""
+    g = torch.Generator().manual_seed(3)
+    lens, Hkv, share = [2, 40, 700], 2, 4
+    pages = sum(-(-n // page) for n in lens)
+    k = torch.randn(pages, Hkv, page, D, generator=g).abs()
+    k[..., channel] = 0  # its group's minimum: code 0, zero 0
+    v = torch.randn(pages, Hkv, page, D, generator=g)
+    q = torch.randn(len(lens), Hkv * share, D, generator=g)
+    q[..., channel] = ratio
+    q, pool = q.to(dtype), pack(k, v, page, group)
+    scaling = 1 / math.sqrt(D)
+    got, table = _attend(q, pool, page, lens, scaling)
+    ref, tol = _exact(q, pool, page, group, table, lens, scaling)
+    worst = ((got - ref).abs() / tol).amax()
+    assert ((got - ref).abs() <= tol).all(), f"{worst:.3g} times the bound"
