@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     bad += __shfl_xor_sync(0xffffffffu, bad, 1);
     bad += __shfl_xor_sync(0xffffffffu, bad, 2);
-    const int k = mx > 0.f ? max(-100, min(100, 13 - ((int)(__float_as_uint(mx) >> 23) - 127))) : 0;
+    const int k = mx > 0.f ? min(127, 13 - ((int)(__float_as_uint(mx) >> 23) - 127)) : 0;  // -114 (finite q) to 127
     // A negative scaling turns the query over, so that a larger raw score is
     // always a larger score.
     const float up = copysignf(__uint_as_float((uint32_t)(127 + k) << 23), p.scale_log2);
@@ -547,7 +547,12 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 1);
       sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 2);
     }
-    const float fh = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 + 24 - k) << 23) + bad;
+    // Back to the scores: |scaling| x 2^(24 - k), in two steps because the power alone
+    // may lie beyond FP32.  Above 2^100, raw scores that differ at all (by 2^-34 or more)
+    // leave one weight: a larger factor changes nothing, and scores stay finite.
+    const int up1 = (24 - k) / 2, up2 = 24 - k - up1;
+    float fh = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 + up1) << 23) * __uint_as_float((uint32_t)(127 + up2) << 23);
+    fh = (fh > 0x1p100f ? 0x1p100f : fh) + bad + p.scale_log2 * 0.f;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {  // lane 4h holds head h
       const int src = 4 * (2 * cq + e);

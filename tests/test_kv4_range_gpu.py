@@ -161,3 +161,37 @@ def test_attend_query_with_an_outlier_channel(ratio, channel, page, group, dtype
     ref, tol = _exact(q, pool, page, group, table, lens, scaling)
     worst = ((got - ref).abs() / tol).amax()
     assert ((got - ref).abs() <= tol).all(), f"{worst:.3g} times the bound"
+
+
+@pytest.mark.parametrize("size", [-126, -90, 100, 113, 118, 120, 126])
+@pytest.mark.parametrize("page,group", [(16, 32), (32, 64), (64, 128)])
+def test_attend_queries_over_the_whole_range_of_bfloat16(size, page, group):
+    """Queries of 2^size with a scaling that brings the scores back to ordinary size, and,
+    for large ones, a scaling that leaves the largest score's token alone."""
+    g = torch.Generator().manual_seed(size + 200)
+    lens, Hkv, share = [3, 130, 600], 1, 4
+    pages = sum(-(-n // page) for n in lens)
+    k, v = (torch.randn(pages, Hkv, page, D, generator=g) for _ in range(2))
+    q = torch.randn(len(lens), Hkv * share, D, generator=g).clamp(-1.9, 1.9).to(torch.bfloat16)
+    pool = pack(k, v, page, group)
+    scaling = 2.0 ** -(size + 3)
+    got, table = _attend(q * 2.0**size, pool, page, lens, scaling)
+    assert torch.isfinite(q * 2.0**size).all()
+    ref, tol = _exact(q * 2.0**size, pool, page, group, table, lens, scaling)
+    assert ((got - ref).abs() <= tol).all()
+    if size >= 100:
+        got, _ = _attend(q * 2.0**size, pool, page, lens, 0.5)
+        # Scores are 0.5 x 2^size times those of q, whose two largest lie further apart than
+        # FP32 sums of 128 products can be off; the other weights are 0.
+        kc, kp = parts(pool, page, group)[:2]
+        for b, n in enumerate(lens):
+            ids = table[b, :-(-n // page)].long()
+            keys = values(kc[ids], kp[ids])[:, 0].reshape(-1, D)[:n]
+            s = q[b].double() @ keys.T
+            two = s.topk(2, -1).values
+            assert (two[:, 0] - two[:, 1] > 2 * 136 * 2.0**-23 * (q[b].double().abs() @ keys.abs().T).amax()).all()
+            vc, vp = parts(pool, page, group)[2:]
+            rows = values(vc[ids], vp[ids])[:, 0].reshape(-1, D)[:n]
+            s16 = vp[ids][:, 0, ..., 0].double().repeat_interleave(group, -1).reshape(-1, D)[:n]
+            top = s.argmax(-1)
+            assert ((got[b] - rows[top]).abs() <= rounding(rows[top], torch.bfloat16) + 15 * s16[top] * 2.0**-11 + 2.0**-14).all()
