@@ -6,7 +6,8 @@
 //   zero  = fp16(min), scale = fp16((max - min) / 15)   (saturated at +-65504)
 //   code  = clamp(rint((x - zero) * (1 / scale)), 0, 15) (0 when scale is 0)
 // from the rounded zero and scale, in FP32 from the rotated FP32 values: k is
-// not rounded to 16 bits first.  Read-back: value = scale * code + zero, one
+// not rounded to 16 bits first.  A NaN takes no part in min and max and becomes code
+// 0; a group of nothing else has zero and scale 0.  Read-back: value = scale * code + zero, one
 // rounding to the 16-bit type.
 //
 // Both are bound by memory.  Eight lanes own a (token, head) row, 16 dims each
@@ -140,7 +141,8 @@ __device__ __forceinline__ void kv4_quantise(const float (&x)[16], int lane8, ui
     mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, m));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, m));
   }
-  const __half z = __float2half_rn(fminf(fmaxf(mn, -65504.f), 65504.f));
+  const float lo = mn == mn ? fminf(fmaxf(mn, -65504.f), 65504.f) : 0.f;  // nothing but NaN: zeros
+  const __half z = __float2half_rn(lo);
   const __half s = __float2half_rn(fminf(fmaxf(__fdiv_rn(mx - mn, 15.f), 0.f), 65504.f));
   const float zf = __half2float(z), sf = __half2float(s);
   const float inv = sf > 0.f ? __frcp_rn(sf) : 0.f;

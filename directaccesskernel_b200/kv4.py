@@ -126,8 +126,10 @@ def rope_kv_append_q4(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torc
     in order, as in a decode step; else any tokens of a prompt).  ``inv_freq``,
     ``interleaved`` and ``rope_scale`` are ``decode_ops.rotary``'s; inv_freq None
     rotates nothing.  Two tokens of one call must not share a sequence and
-    position.  A NaN is stored as code 0 and values beyond float16 saturate: the
-    cache holds finite numbers only."""
+    position.  The cache holds finite numbers only: a NaN is stored as code 0, the
+    minimum of its group's numbers (0 in a group of nothing but NaN), and a
+    group's zero and scale saturate at float16's largest value, so that a
+    read-back in float16 of numbers at its very end may be infinite."""
     device = current_device_of(qkv, "qkv")
     if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("qkv must be a 16-bit [tokens, (q_heads + 2 kv_heads) * 128] tensor, last dim contiguous")

@@ -458,7 +458,8 @@ typedef struct dak_kv4_cache {
  * into slot positions[t] of their sequence.  Per token, head and group:
  *   zero = fp16(min), scale = fp16((max - min) / 15), both within +-65504,
  *   code = clamp(round((x - zero) * (1 / scale)), 0, 15), 0 when scale is 0;
- * a NaN is stored as code 0.  rotary_dim 0 rotates nothing.  The (sequence,
+ * a NaN takes no part in min and max and is stored as code 0 (a group of nothing
+ * but NaN: zero and scale 0).  rotary_dim 0 rotates nothing.  The (sequence,
  * position) pairs of one call must differ. */
 typedef struct dak_kv4_append_args {
   const void *qkv;
