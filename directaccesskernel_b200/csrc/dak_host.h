@@ -29,6 +29,16 @@ int *device_status_word();
 int device_sms();
 // DAK_OK if `p` is memory of the current device or pinned host memory.
 int check_gpu_accessible(const void *p, const char *what);
+// A buffer as n0 x n1 blocks of `len` bytes, s0 and s1 bytes apart.
+struct BlockGrid {
+  const void *p;
+  int64_t n0, s0, n1, s1, len;
+};
+// Whether two blocks of one grid, or a block of one and a block of the other, share
+// a byte.  Exact; two grids of different shapes or strides whose ranges meet count as
+// overlapping where the comparison would take more than 2^20 steps.
+bool overlaps_itself(const BlockGrid &a);
+bool overlap(const BlockGrid &a, const BlockGrid &b);
 // DAK_OK if the rotary kernels serve this part of a head.
 int check_rotary_dim(int rotary_dim, int head_dim, int interleaved);
 // Checks a 4-bit cache's sizes (kv4_check), then its pointers, and fills the

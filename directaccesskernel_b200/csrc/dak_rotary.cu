@@ -93,9 +93,12 @@ extern "C" int dak_rotary(const dak_rotary_args *r, void *stream) {
   if (r->x_stride_t % 8 || r->x_stride_h % 8 || r->o_stride_t % 8 || r->o_stride_h % 8 ||
       ((reinterpret_cast<uintptr_t>(r->x) | reinterpret_cast<uintptr_t>(r->out)) & 15u))
     return fail(DAK_ERR_ALIGNMENT, "rotary: x and out must be 16-byte aligned, strides multiples of 8 elements");
-  auto overlaps = [&](int n, int64_t stride) { return n > 1 && stride > -r->head_dim && stride < r->head_dim; };
-  if (overlaps(r->tokens, r->o_stride_t) || overlaps(r->heads, r->o_stride_h))
-    return fail(DAK_ERR_INVALID_ARG, "rotary: heads of out overlap");
+  const BlockGrid x = {r->x, r->tokens, 2 * r->x_stride_t, r->heads, 2 * r->x_stride_h, 2 * r->head_dim};
+  const BlockGrid out = {r->out, r->tokens, 2 * r->o_stride_t, r->heads, 2 * r->o_stride_h, 2 * r->head_dim};
+  if (overlaps_itself(out)) return fail(DAK_ERR_INVALID_ARG, "rotary: heads of out overlap");
+  const bool in_place = r->x == r->out && (r->tokens <= 1 || r->x_stride_t == r->o_stride_t) &&
+                        (r->heads <= 1 || r->x_stride_h == r->o_stride_h);
+  if (!in_place && overlap(x, out)) return fail(DAK_ERR_INVALID_ARG, "rotary: out overlaps x without being x");
   const void *ptrs[4] = {r->x, r->out, r->positions, r->inv_freq};
   for (const void *q : ptrs)
     if ((st = check_gpu_accessible(q, "rotary buffer"))) return st;

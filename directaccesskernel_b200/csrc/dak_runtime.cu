@@ -162,6 +162,64 @@ int check_gpu_accessible(const void *p, const char *what) {
   return fail(DAK_ERR_INVALID_ARG, "%s must be device memory or pinned host memory (pageable memory given)", what);
 }
 
+// --------------------------------------------------- overlapping buffers
+namespace {
+typedef __int128 wide;
+
+// Whether base + i s is within (-below, above) for an i of [lo, hi].
+bool any_within(wide base, wide s, int64_t lo, int64_t hi, int64_t below, int64_t above) {
+  auto in = [&](wide i) {
+    const wide x = base + std::min<wide>(std::max<wide>(i, lo), hi) * s;
+    return x > -below && x < above;
+  };
+  if (s == 0) return in(lo);
+  const wide i = -base / s;  // x changes its sign next to it
+  return in(i - 1) || in(i) || in(i + 1);
+}
+
+// Dimensions of one block get stride 0; n0 >= n1.
+BlockGrid in_order(BlockGrid a) {
+  if (a.n0 <= 1) a.s0 = 0;
+  if (a.n1 <= 1) a.s1 = 0;
+  if (a.n0 < a.n1) std::swap(a.n0, a.n1), std::swap(a.s0, a.s1);
+  return a;
+}
+}  // namespace
+
+bool overlaps_itself(const BlockGrid &grid) {
+  const BlockGrid a = in_order(grid);
+  if (a.n0 > 1 && std::abs(a.s0) < a.len) return true;
+  for (int64_t j = 1; j < a.n1; ++j)
+    if (any_within((wide)j * a.s1, a.s0, 1 - a.n0, a.n0 - 1, a.len, a.len)) return true;
+  return false;
+}
+
+bool overlap(const BlockGrid &grid_a, const BlockGrid &grid_b) {
+  const BlockGrid a = in_order(grid_a), b = in_order(grid_b);
+  if (a.n0 <= 0 || a.n1 <= 0 || b.n0 <= 0 || b.n1 <= 0) return false;
+  auto first = [](const BlockGrid &g) {
+    return (wide)reinterpret_cast<uintptr_t>(g.p) + std::min<wide>(0, (wide)(g.n0 - 1) * g.s0) +
+           std::min<wide>(0, (wide)(g.n1 - 1) * g.s1);
+  };
+  auto last = [](const BlockGrid &g) {
+    return (wide)reinterpret_cast<uintptr_t>(g.p) + std::max<wide>(0, (wide)(g.n0 - 1) * g.s0) +
+           std::max<wide>(0, (wide)(g.n1 - 1) * g.s1) + g.len;
+  };
+  if (last(a) <= first(b) || last(b) <= first(a)) return false;
+  const wide delta = (wide)reinterpret_cast<uintptr_t>(b.p) - (wide)reinterpret_cast<uintptr_t>(a.p);
+  if (a.n0 == b.n0 && a.n1 == b.n1 && a.s0 == b.s0 && a.s1 == b.s1) {  // blocks (i, j) apart
+    for (int64_t j = 1 - a.n1; j < a.n1; ++j)
+      if (any_within(delta + (wide)j * a.s1, a.s0, 1 - a.n0, a.n0 - 1, b.len, a.len)) return true;
+    return false;
+  }
+  if ((wide)a.n0 * a.n1 * b.n1 > 1 << 20) return true;
+  for (int64_t i = 0; i < a.n0; ++i)
+    for (int64_t k = 0; k < a.n1; ++k)
+      for (int64_t j = 0; j < b.n1; ++j)
+        if (any_within(delta - (wide)i * a.s0 - (wide)k * a.s1 + (wide)j * b.s1, b.s0, 0, b.n0 - 1, b.len, a.len)) return true;
+  return false;
+}
+
 // ------------------------------------------------------ tile-map encoding
 namespace {
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
