@@ -1050,9 +1050,12 @@ extern "C" int dak_attn_decode_paged_q4(const dak_kv4_cache *cache, const dak_at
       ((reinterpret_cast<uintptr_t>(a->query) | reinterpret_cast<uintptr_t>(a->out) |
         reinterpret_cast<uintptr_t>(a->scratch)) & 15u))
     return fail(DAK_ERR_ALIGNMENT, "query, out and scratch must be 16-byte aligned, strides multiples of 8 elements");
-  auto overlaps = [](int n, int64_t stride) { return n > 1 && stride > -kKv4Dim && stride < kKv4Dim; };
-  if (overlaps(cache->batch, a->o_stride_b) || overlaps(a->num_q_heads, a->o_stride_h))
-    return fail(DAK_ERR_INVALID_ARG, "heads of out overlap");
+  const BlockGrid q = {a->query, cache->batch, 2 * a->q_stride_b, a->num_q_heads, 2 * a->q_stride_h, 2 * kKv4Dim};
+  const BlockGrid out = {a->out, cache->batch, 2 * a->o_stride_b, a->num_q_heads, 2 * a->o_stride_h, 2 * kKv4Dim};
+  if (overlaps_itself(out)) return fail(DAK_ERR_INVALID_ARG, "heads of out overlap");
+  const bool in_place = a->query == a->out && (cache->batch == 1 || a->q_stride_b == a->o_stride_b) &&
+                        (a->num_q_heads == 1 || a->q_stride_h == a->o_stride_h);
+  if (!in_place && overlap(q, out)) return fail(DAK_ERR_INVALID_ARG, "out overlaps the query without being it");
   const Q4Plan plan = q4_plan(cache, a->num_q_heads, a->max_seq_len);
   if (plan.rows > 0x7fffffffll / (((int64_t)a->max_seq_len + kQ4Chunk - 1) / kQ4Chunk))
     return fail(DAK_ERR_UNSUPPORTED, "batch x heads x max_seq_len is too large for one launch");

@@ -214,7 +214,7 @@ def decode_paged_q4(query: torch.Tensor, pool_dev: torch.Tensor | None, pool_hos
     ``merge_counters`` (int32 CUDA, ``merge_counter_count`` entries, zero before
     the first call and left zero by every call) rows that were split are merged
     inside the attention kernel instead of by a second launch; the result is the
-    same.  ``out`` may be the query itself.  Calls that may overlap on the GPU need
+    same.  ``out`` may be the query itself, else must not overlap it.  Calls that may overlap on the GPU need
     scratch and counters of their own."""
     device = current_device_of(query, "query")
     dtype = query.dtype

@@ -76,3 +76,28 @@ def test_rotary_outputs_against_all_pairs():
         assert (OVERLAP in _rotary(T, H, d, BUF, xs, out, os)) == want, (T, H, xs, os, out - BUF)
         seen[want] += 1
     assert min(seen.values()) > 300
+
+
+def _cache(**kw):
+    c = _lib.Kv4Cache()
+    for k, v in {**dict(pool_dev=1 << 40, dev_pages=4, block_table=1 << 41, table_stride=2, max_pages=2, batch=3, kv_heads=2,
+                        page_size=16, group=32), **kw}.items():
+        setattr(c, k, v)
+    return c
+
+
+@pytest.mark.parametrize("batch,heads,qs,out,os,refused", [
+    (3, 4, (512, 128), BUF, (512, 128), False),               # over the query itself
+    (3, 4, (512, 128), 1 << 30, (512, 128), False),
+    (3, 4, (512, 128), 1 << 30, (128, 128), True),            # the next sequence over head 1
+    (3, 4, (512, 128), 1 << 30, (384, 128), True),            # over the last head
+    (3, 4, (512, 128), 1 << 30, (128, 384), False),           # head-major
+    (3, 4, (512, 128), 1 << 30, (128, 256), True),
+    (3, 4, (768, 128), BUF + 2 * 128, (768, 128), True),      # a head on
+    (3, 4, (1024, 128), BUF + 2 * 512, (1024, 128), False),   # between the query's rows
+    (3, 4, (512, 128), BUF, (128, 384), True),                # over the query in another order
+    (1, 4, (0, 128), BUF, (9 * 8, 128), False),               # one sequence: its stride does not count
+])
+def test_attention_outputs(batch, heads, qs, out, os, refused):
+    a = _lib.AttnQ4Args(BUF, *qs, BUF, out, *os, None, 0, None, heads, 32, 0.1, _lib.DTYPE_F16)
+    assert (OVERLAP in _refusal(_lib.LIB.dak_attn_decode_paged_q4, ctypes.byref(_cache(batch=batch)), ctypes.byref(a), None)) == refused
