@@ -427,6 +427,10 @@ extern "C" int dak_rope_kv_append_q4(const dak_kv4_cache *cache, const dak_kv4_a
     return fail(DAK_ERR_ALIGNMENT, "qkv and q_out must be 16-byte aligned, the row stride a multiple of 8 elements");
   if ((st = check_rotary_dim(a->rotary_dim, kKv4Dim, a->interleaved))) return st;
   if (a->rotary_dim > 0 && !a->inv_freq) return fail(DAK_ERR_INVALID_ARG, "inv_freq is required to rotate");
+  const int64_t row = ((int64_t)a->q_heads + 2ll * cache->kv_heads) * kKv4Dim * 2;
+  if (a->q_heads > 0 && overlap({a->qkv, a->tokens, 2 * a->ld, 1, 0, row},
+                                {a->q_out, a->tokens > 0, 0, 1, 0, 2ll * a->tokens * a->q_heads * kKv4Dim}))
+    return fail(DAK_ERR_INVALID_ARG, "q_out must not overlap qkv");
   const void *ptrs[5] = {a->qkv, a->q_heads > 0 ? a->q_out : nullptr, a->rotary_dim > 0 ? a->inv_freq : nullptr,
                          a->positions, a->seq_index};
   for (const void *q : ptrs)

@@ -468,7 +468,7 @@ typedef struct dak_kv4_append_args {
   const int32_t *seq_index;   /* [tokens] or NULL                               */
   const float *inv_freq;      /* [rotary_dim / 2]                               */
   float rope_scale;
-  void *q_out;                /* [tokens, q_heads, 128]; NULL with q_heads 0    */
+  void *q_out;                /* [tokens, q_heads, 128], not over qkv; NULL with q_heads 0 */
   int tokens, q_heads, rotary_dim, interleaved, dtype;
 } dak_kv4_append_args;
 DAK_API int dak_rope_kv_append_q4(const dak_kv4_cache *cache, const dak_kv4_append_args *args, void *stream);

@@ -101,3 +101,22 @@ def _cache(**kw):
 def test_attention_outputs(batch, heads, qs, out, os, refused):
     a = _lib.AttnQ4Args(BUF, *qs, BUF, out, *os, None, 0, None, heads, 32, 0.1, _lib.DTYPE_F16)
     assert (OVERLAP in _refusal(_lib.LIB.dak_attn_decode_paged_q4, ctypes.byref(_cache(batch=batch)), ctypes.byref(a), None)) == refused
+
+
+@pytest.mark.parametrize("tokens,ld,q_out,refused", [
+    (3, 1024, BUF, True),
+    (3, 1024, BUF - 2 * 3 * 512, False),       # right before qkv
+    (3, 1024, BUF - 2 * 3 * 512 + 16, True),
+    (3, 1024, BUF + 2 * 3 * 1024, False),      # right behind it
+    (3, 1024, BUF + 2 * 3 * 1024 - 16, True),
+    (3, 4096, BUF + 2 * 1024, False),          # between its rows
+    (3, 2048, BUF + 2 * 1024, True),           # where they leave less room
+    (1, 4096, BUF + 2 * 512, True),
+    (0, 1024, BUF, False),
+])
+def test_append_outputs(tokens, ld, q_out, refused):
+    a = _lib.Kv4AppendArgs()
+    for k, v in dict(qkv=BUF, ld=ld, positions=BUF, seq_index=BUF, inv_freq=BUF, rope_scale=1.0, q_out=q_out, tokens=tokens,
+                     q_heads=4, rotary_dim=128, dtype=_lib.DTYPE_BF16).items():
+        setattr(a, k, v)
+    assert (OVERLAP in _refusal(_lib.LIB.dak_rope_kv_append_q4, ctypes.byref(_cache()), ctypes.byref(a), None)) == refused
