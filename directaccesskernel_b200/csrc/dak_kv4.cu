@@ -483,7 +483,9 @@ extern "C" int dak_kv_read_q4(const dak_kv4_cache *cache, const int32_t *positio
     return fail(DAK_ERR_UNSUPPORTED, "the 4-bit cache is read to float16 and bfloat16");
   if ((st = check_tokens(tokens, positions, seq_index, cache->batch))) return st;
   if (!k_out || !v_out) return fail(DAK_ERR_INVALID_ARG, "k_out and v_out are required");
-  if (k_out == v_out) return fail(DAK_ERR_INVALID_ARG, "k_out and v_out must not overlap");
+  const int64_t bytes = 2ll * tokens * cache->kv_heads * kKv4Dim;
+  if (k_out == v_out || overlap({k_out, 1, 0, 1, 0, bytes}, {v_out, 1, 0, 1, 0, bytes}))
+    return fail(DAK_ERR_INVALID_ARG, "k_out and v_out must not overlap");
   if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15u)
     return fail(DAK_ERR_ALIGNMENT, "k_out and v_out must be 16-byte aligned");
   const void *ptrs[4] = {k_out, v_out, positions, seq_index};

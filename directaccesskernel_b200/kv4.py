@@ -161,7 +161,7 @@ def kv_read_q4(pool_dev: torch.Tensor | None, pool_host: torch.Tensor | None, bl
                k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(k, v) [tokens, kv_heads, 128] that the cache holds for the given tokens, in
     16 bits: what attention over the cache sees, for a prompt whose prefix is
-    already cached."""
+    already cached.  ``k_out`` and ``v_out`` must not overlap."""
     device = current_device_of(block_table, "block_table")
     if dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError("dtype must be float16 or bfloat16")

@@ -474,7 +474,7 @@ typedef struct dak_kv4_append_args {
 DAK_API int dak_rope_kv_append_q4(const dak_kv4_cache *cache, const dak_kv4_append_args *args, void *stream);
 
 /* The cache's values at (seq_index[t] or t, positions[t]) in 16 bits: k_out and
- * v_out are [tokens, kv_heads, 128]. */
+ * v_out are [tokens, kv_heads, 128] and do not overlap. */
 DAK_API int dak_kv_read_q4(const dak_kv4_cache *cache, const int32_t *positions, const int32_t *seq_index,
                            void *k_out, void *v_out, int tokens, int dtype, void *stream);
 

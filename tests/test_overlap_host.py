@@ -120,3 +120,10 @@ def test_append_outputs(tokens, ld, q_out, refused):
                      q_heads=4, rotary_dim=128, dtype=_lib.DTYPE_BF16).items():
         setattr(a, k, v)
     assert (OVERLAP in _refusal(_lib.LIB.dak_rope_kv_append_q4, ctypes.byref(_cache()), ctypes.byref(a), None)) == refused
+
+
+@pytest.mark.parametrize("behind,refused", [(0, True), (16, True), (2 * 3 * 2 * 128 - 16, True), (2 * 3 * 2 * 128, False),
+                                            (16 - 2 * 3 * 2 * 128, True), (-2 * 3 * 2 * 128, False)])
+def test_read_outputs(behind, refused):
+    text = _refusal(_lib.LIB.dak_kv_read_q4, ctypes.byref(_cache()), BUF, BUF, BUF, BUF + behind, 3, _lib.DTYPE_F16, None)
+    assert (OVERLAP in text) == refused
