@@ -82,10 +82,7 @@ def _cache(device: int, pool_dev, pool_host, block_table: torch.Tensor) -> _lib.
     (rows, pages), (row_stride, stride) = block_table.shape, block_table.stride()
     if pages > 1 and stride != 1:
         raise RuntimeError("block_table must have contiguous rows")
-    fmt = _FORMATS.get(shape[2])
-    if fmt is None:
-        raise RuntimeError(f"{shape[2]} bytes per (page, head) is no page_bytes(page_size, group)")
-    c.page_size, c.group = fmt
+    c.page_size, c.group = page_format(pool_dev if pool_dev is not None else pool_host)
     c.kv_heads, c.batch, c.max_pages = shape[1], rows, pages
     c.block_table, c.table_stride = block_table.data_ptr(), row_stride if rows > 1 else pages
     return c
