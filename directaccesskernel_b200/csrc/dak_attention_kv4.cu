@@ -576,8 +576,9 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
   // chunk takes the exponent of its largest product (several groups: of the largest
   // sum over a lane's 8 tokens, one instruction less), so that products are below 2
   // and those above 2^-14 keep all of their bits.  The unit falls as well as rises,
-  // and O with it, exactly; it stays at 2^-90 or above so that FP32 holds O.
-  constexpr uint32_t kRefMin = (127 - 90) << 7 | (127 - 90) << 23;
+  // and O with it, exactly; it stays at 2^-104 of the largest weight or above so that
+  // FP32 holds O (2^16 x 255 x 2^-24 per token, over 2^23 tokens).
+  constexpr uint32_t kRefMin = (127 - 104) << 7 | (127 - 104) << 23;
   float o[8][4], m[2], l[2];
   uint32_t ref[NG];
 
@@ -739,7 +740,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
     // nothing cancels at the end.
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
-      const float2 even = make_float2(zs[0][n].x * up[0][n] * 0x1p-24f, zs[1][n].x * up[1][n] * 0x1p-24f);
+      const float2 even = make_float2(zs[0][n].x * (up[0][n] * 0x1p-24f), zs[1][n].x * (up[1][n] * 0x1p-24f));
       const float2 odd = make_float2(even.x * 17, even.y * 17), old = make_float2(beta[0][n], beta[1][n]);
 #pragma unroll
       for (int t = 8 * n / NG; t < 8 * (n + 1) / NG; ++t) {
