@@ -189,6 +189,10 @@ BlockGrid in_order(BlockGrid a) {
 bool overlaps_itself(const BlockGrid &grid) {
   const BlockGrid a = in_order(grid);
   if (a.n0 > 1 && std::abs(a.s0) < a.len) return true;
+  if (a.n1 > 1 && std::abs(a.s1) < a.len) return true;
+  // One dimension's span within the other's stride, as most buffers have it.
+  auto span = [&](int64_t n, int64_t s) { return (wide)(n - 1) * std::abs(s) + a.len; };
+  if (a.n1 <= 1 || std::abs(a.s0) >= span(a.n1, a.s1) || std::abs(a.s1) >= span(a.n0, a.s0)) return false;
   for (int64_t j = 1; j < a.n1; ++j)
     if (any_within((wide)j * a.s1, a.s0, 1 - a.n0, a.n0 - 1, a.len, a.len)) return true;
   return false;
