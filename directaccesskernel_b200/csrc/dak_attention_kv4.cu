@@ -22,19 +22,19 @@
 // + 16 odd, units of 2^-24), which a mask or a byte permutation each give; V's odd
 // dims are the difference, at the end (masks and shifts for each nibble took 1 to
 // 3% longer; K has no such form, because even - odd / 16 of a query does not fit
-// float16).  P is float16, in units of each
-// chunk's largest products (see "Statistics" below): for bfloat16 outputs in one
-// term (2^-11 relative, an eighth of the output's own rounding), for float16
-// outputs in two, because one made the output up to 1.9 times less exact than its
-// rounding and two do not show.  One unit for all chunks and groups, from the
-// largest score and the largest scale, was 1.5% (groups of 32: 7%) faster and lost
-// V's codes where large scales had small weights.
+// float16).  P is float16, in units of each chunk's largest products (see
+// "Statistics" below): for bfloat16 outputs in one term (2^-11 relative, an eighth
+// of the output's own rounding), for float16 outputs in two, because one made the
+// output up to 1.9 times less exact than its rounding and two do not show.  One unit
+// for all chunks and groups, from the largest score and the largest scale, was 1.5%
+// (float16 3%, groups of 32 6%) faster and lost V's codes where large scales had
+// small weights.
 //
 // Bound, at 32 x 16384 tokens of 8 KV heads (570 MB, 89 us at the measured copy
-// rate), in a graph of calls: 113 us in bfloat16, 121 us in float16.  The copies
-// alone take 91 us; the rest is arithmetic that two warps per scheduler do not
-// quite hide (4.3 cycles per instruction and warp, about 800 instructions per
-// chunk).  Plain bulk copies replaced tensor copies with a 64-byte swizzle: bank
+// rate): 113 us in bfloat16 and 119 us in float16 in a graph of twelve calls, 126 us
+// in bfloat16 over many calls back to back, when power limits the clocks.  The
+// copies alone take 91 us; the rest is arithmetic that two warps per scheduler do
+// not quite hide (4.4 cycles per instruction and warp, 870 instructions per chunk).  Plain bulk copies replaced tensor copies with a 64-byte swizzle: bank
 // conflicts cost less than the 64-byte rows did, and host pages come 15% faster
 // (46 GB/s).
 #include <cfloat>
@@ -202,9 +202,9 @@ __device__ __forceinline__ int chunks_of(int seq) { return (seq + kQ4Chunk - 1) 
 // pieces, which matters where one or two rows are all there is (one row of 131072
 // tokens: 57 us in 293 pieces, 27 in 79).  A range with chunks of two rows takes
 // longer than one of a single row, by the first row's end and warps without a chunk
-// there: pieces of up to kQ4Slack chunks more are taken before ranges.  24 ragged
-// sequences of up to 6001 tokens: 12.3 us, 19.7 in ranges; 16 of up to 20000: 16 and
-// 30; 32 x 16384 of one KV head: 23.3 and 24.9.
+// there: pieces of up to kQ4Slack chunks more are taken before ranges.  Side by side,
+// 24 ragged sequences of up to 6001 tokens: 12.3 us, 19.7 in ranges; 16 of up to
+// 20000: 16 and 30; 32 x 16384 of one KV head: 23.3 and 24.9.
 struct Q4Deal {
   int size;
   bool whole;
