@@ -34,9 +34,9 @@
 // rate): 113 us in bfloat16 and 119 us in float16 in a graph of twelve calls, 126 us
 // in bfloat16 over many calls back to back, when power limits the clocks.  The
 // copies alone take 91 us; the rest is arithmetic that two warps per scheduler do
-// not quite hide (4.4 cycles per instruction and warp, 870 instructions per chunk).  Plain bulk copies replaced tensor copies with a 64-byte swizzle: bank
-// conflicts cost less than the 64-byte rows did, and host pages come 15% faster
-// (46 GB/s).
+// not quite hide (4.4 cycles per instruction and warp, 870 instructions per chunk).
+// Plain bulk copies replaced tensor copies with a 64-byte swizzle: bank conflicts
+// cost less than the 64-byte rows did, and host pages come 15% faster (46 GB/s).
 #include <cfloat>
 #include <cstring>
 #include <type_traits>
@@ -502,10 +502,11 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
   if (!p.by_row) zero_rows();
 
   // Scores.  A query is scaled by a power of two so that its largest value lies
-  // between 2^13 and 2^14; float16 then holds the others exactly down to 2^-24 of it
-  // (a bfloat16 value's bits too).  Products and sums are FP32.  Integer MMAs over
-  // whole bytes, the query in 16 and 20 bits, were 2% faster with one group, no faster
-  // with two, and lost the bits of all other channels where one was far larger.
+  // between 2^13 and 2^14; float16 then holds the others exactly down to 2^-23 of it
+  // (bfloat16's too), and smaller ones to 2^-34 of it.  Products and sums are FP32.
+  // Integer MMAs over whole bytes, the query in 16 and 20 bits, were 2% faster with one
+  // group, no faster with two, and lost the bits of all other channels where one was
+  // far larger.
   uint32_t qf[8][2];
   float qs[2][NG], f[2];  // q summed over each group (for the zeros' share); raw scores to base 2
   auto ready_query = [&]() {

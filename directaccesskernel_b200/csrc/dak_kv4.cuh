@@ -6,7 +6,7 @@
 //   K (scale, zero) [P][NG][2] float16 (NG = 128 / group)
 //   V codes [P][64]
 //   V (scale, zero) [P][NG][2] float16
-// and the value of code n is scale * n + zero.  K and V of a page sit in one
+// and the value of code n is scale * n + zero, scale >= 0.  K and V of a page sit in one
 // slab so that one contiguous copy (2.1 to 10 KB) brings both.
 #pragma once
 

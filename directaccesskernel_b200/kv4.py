@@ -8,7 +8,7 @@ for every token and group of dims:
 
     K codes [P, 64] | K pairs [P, 128 / group, 2] | V codes [P, 64] | V pairs
 
-with dim 2i in the low nibble of byte i and value = scale * code + zero.
+with dim 2i in the low nibble of byte i and value = scale * code + zero, scale >= 0.
 ``page_bytes`` gives the slab's bytes; page size (16, 32 or 64 tokens) and group
 (32, 64 or 128 dims) follow from them.  Smaller groups are more exact: a page of
 group 128 takes 4.25 bits per value, 64: 4.5, 32: 5.  Block tables name pages as

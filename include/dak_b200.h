@@ -434,7 +434,7 @@ DAK_API int dak_rotary(const dak_rotary_args *args, void *stream);
  * page_size (16, 32 or 64) tokens of head_dim 128 holds K codes [page_size][64]
  * (dim 2i in the low half of byte i), K (scale, zero) float16 pairs
  * [page_size][128 / group][2], V codes and V pairs: the value of code n is
- * scale * n + zero.  group is 32, 64 or 128 dims.  block_table[b * table_stride
+ * scale * n + zero, scale never being negative.  group is 32, 64 or 128 dims.  block_table[b * table_stride
  * + j] names page j of sequence b (0 <= b < batch) as in dak_attn_paged_args;
  * entries outside their pool are recorded in the device error word
  * (DAK_ERR_INVALID_ARG), skipped by the append and read as zeros.  No reference
