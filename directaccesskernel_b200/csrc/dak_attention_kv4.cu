@@ -895,13 +895,15 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4PerSm) attn_q4_kernel(const __g
       gm[e] = sm_m[2 * cq + e];
 #pragma unroll
       for (int w = 1; w < W; ++w) gm[e] = fmaxf(gm[e], sm_m[w * kQ4Heads + 2 * cq + e]);
-      share[e] = ex2(m[e] - gm[e]) * 0x1p24f;
+      share[e] = ex2(m[e] - gm[e]);
     }
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
-      const float c0 = share[0] * ref_of(ref[t * NG / 8], 0), c1 = share[1] * ref_of(ref[t * NG / 8], 1);
-      sm_o[warp * kQ4Frags + t * 32 + lane] = make_float4(o[t][0] * c0, o[t][1] * c1, (o[t][2] - o[t][0]) * (c0 * 0.0625f),
-                                                          (o[t][3] - o[t][1]) * (c1 * 0.0625f));
+      // The unit first: it may be small and O large, and its product with the share below FP32.
+      const float c0 = ref_of(ref[t * NG / 8], 0) * 0x1p24f, c1 = ref_of(ref[t * NG / 8], 1) * 0x1p24f;
+      sm_o[warp * kQ4Frags + t * 32 + lane] =
+          make_float4(o[t][0] * c0 * share[0], o[t][1] * c1 * share[1], (o[t][2] - o[t][0]) * (c0 * 0.0625f) * share[0],
+                      (o[t][3] - o[t][1]) * (c1 * 0.0625f) * share[1]);
     }
     __syncthreads();
     float den[2] = {0.f, 0.f};

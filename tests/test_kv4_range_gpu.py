@@ -195,3 +195,25 @@ def test_attend_queries_over_the_whole_range_of_bfloat16(size, page, group):
             s16 = vp[ids][:, 0, ..., 0].double().repeat_interleave(group, -1).reshape(-1, D)[:n]
             top = s.argmax(-1)
             assert ((got[b] - rows[top]).abs() <= rounding(rows[top], torch.bfloat16) + 15 * s16[top] * 2.0**-11 + 2.0**-14).all()
+
+
+@pytest.mark.parametrize("nats", [20.0, 55.0, 65.0])
+@pytest.mark.parametrize("n", [357, 5000])
+@pytest.mark.parametrize("page,group", [(16, 32), (32, 64), (64, 128)])
+def test_attend_one_token_beside_a_silent_sink(nats, n, page, group):
+    """Token 255 has the largest score and no V, token 78 comes `nats` below it with all there
+    is of V, the others lie 160 nats further down: whole chunks with products of 0 follow 78's."""
+    g = torch.Generator().manual_seed(9)
+    pages, Hkv, share = -(-n // page), 2, 3
+    k, v = (torch.randn(pages, Hkv, page, D, generator=g) for _ in range(2))
+    k[..., 0] = -40.0
+    k[78 // page, :, 78 % page, 0] = 0.0
+    k[255 // page, :, 255 % page, 0] = nats / 4
+    v[255 // page, :, 255 % page] = 0
+    q = torch.zeros(1, Hkv * share, D)
+    q[..., 0] = 4.0
+    q, pool = q.to(torch.bfloat16), pack(k, v, page, group)
+    got, table = _attend(q, pool, page, [n], 1.0)
+    ref, tol = _exact(q, pool, page, group, table, [n], 1.0)
+    worst = ((got - ref).abs() / tol).amax()
+    assert ((got - ref).abs() <= tol).all(), f"{worst:.3g} times the bound"
